@@ -5,8 +5,12 @@ this package is the torch-facing host side: the functional ops and the
 reference-surface ``exts()`` modules.
 """
 from . import _lib
-from .ops import (CHUNK, DecodeModule, PrefillModule, ProjModule, RMSNormModule, decode_proj, decode_step, exts,
-                  gated_rmsnorm, prefill, prefill_varlen, proj_conv_silu, rmsnorm)
+from .ops import (CHUNK, DecodeModule, PrefillModule, ProjModule, RMSNormModule, block_norm, block_norm_autograd,
+                  block_norm_backward, decode_proj, decode_step, exts, gated_rmsnorm, paged_attention,
+                  paged_attention_workspace, prefill, prefill_varlen, proj_conv_silu, rmsnorm, rope, rope_append,
+                  rope_autograd)
 
-__all__ = ["CHUNK", "DecodeModule", "PrefillModule", "ProjModule", "RMSNormModule", "decode_proj", "decode_step", "exts",
-           "gated_rmsnorm", "prefill", "prefill_varlen", "proj_conv_silu", "rmsnorm", "_lib"]
+__all__ = ["CHUNK", "DecodeModule", "PrefillModule", "ProjModule", "RMSNormModule", "block_norm",
+           "block_norm_autograd", "block_norm_backward", "decode_proj", "decode_step", "exts", "gated_rmsnorm",
+           "paged_attention", "paged_attention_workspace", "prefill", "prefill_varlen", "proj_conv_silu", "rmsnorm",
+           "rope", "rope_append", "rope_autograd", "_lib"]

@@ -35,11 +35,14 @@ GDN_SCHEDULE_STREAM = 3
 GDN_DECODE_L2NORM_QK = 1
 GDN_GATES_BHT = 0
 GDN_GATES_BTH = 1
+GDN_ROPE_HALF = 0
+GDN_ROPE_INTERLEAVED = 1
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
+_L = ctypes.c_long
 
 class ProjOutSeg(ctypes.Structure):
     """gdn_proj_out_seg (include/gdn_b200.h): one output segment of gdn_proj_multi_fwd."""
@@ -56,6 +59,19 @@ class ProjSegment(ctypes.Structure):
     """gdn_proj_segment (include/gdn_b200.h): one channel segment of gdn_decode_proj_fwd."""
     _fields_ = [("W", _P), ("y", _P), ("conv_w", _P), ("conv_state_in", _P), ("conv_state_out", _P),
                 ("C", _I), ("ldy", _I), ("l2_group", _I)]
+
+
+class RopeSpec(ctypes.Structure):
+    """gdn_rope_spec (include/gdn_b200.h): positions, frequencies and sections of a rotation."""
+    _fields_ = [("positions", _P), ("positions_ld", _L), ("inv_freq", _P), ("sections", _P), ("axes", _I), ("rot", _I),
+                ("style", _I)]
+
+
+class PagedCache(ctypes.Structure):
+    """gdn_paged_cache (include/gdn_b200.h): a paged cache of keys and values."""
+    _fields_ = [("k", _P), ("v", _P), ("block_table", _P), ("table_ld", _L), ("page_stride", _L), ("token_stride", _L),
+                ("head_stride", _L), ("num_pages", _I), ("page_size", _I), ("max_pages", _I), ("n_kv", _I),
+                ("head_dim", _I)]
 
 
 # name -> argtypes (every entry returns int unless listed in _STR_FUNCS)
@@ -95,6 +111,15 @@ SIGNATURES = {
                               _I, _I, _I, _I, _I, _F, _I, _P],
     "gdn_rmsnorm_fwd": [_P, _P, _P, _I, _I, _F, _P],
     "gdn_gated_rmsnorm_fwd": [_P, _I, _P, _P, _P, _I, _I, _F, _P],
+    "gdn_block_norm_fwd": [_P, _P, _I, _P, _P, _I, _P, _F, _P, _P, _I, _I, _F, _P],
+    "gdn_block_norm_bwd": [_P, _P, _I, _P, _P, _P, _P, _I, _P, _F, _P, _P, _P, _I, _P, _P, _I, _I, _F, _P, _Z, _P],
+    "gdn_block_norm_bwd_workspace_bytes": [_I, _I, _I],
+    "gdn_rope_fwd": [_P, _L, _P, _L, _P, _P, ctypes.POINTER(RopeSpec), _I, _I, _I, _I, _I, _P],
+    "gdn_rope_append": [_P, _L, _P, _L, _P, _L, _P, ctypes.POINTER(RopeSpec), ctypes.POINTER(PagedCache), _P, _P,
+                        _I, _I, _I, _P],
+    "gdn_paged_attn_fwd": [_P, _L, ctypes.POINTER(PagedCache), _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z,
+                           _P],
+    "gdn_paged_attn_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
     "gdn_decode_proj_fwd": [_P, _P, _F, _I, _I, ctypes.POINTER(ProjSegment), _I, _P],
     "gdn_proj_conv_silu_fwd": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
     "gdn_proj_multi_fwd": [_P, _I, _I, _I, ctypes.POINTER(ProjOutSeg), _I, _P],
@@ -109,7 +134,8 @@ SIGNATURES = {
 }
 _STR_FUNCS = {"gdn_last_error", "gdn_version"}
 _SIZE_FUNCS = {"gdn_prefill_workspace_bytes", "gdn_prefill_varlen_workspace_bytes", "gdn_prefill_bwd_workspace_bytes",
-               "gdn_prefill_host_workspace_bytes"}
+               "gdn_prefill_host_workspace_bytes", "gdn_block_norm_bwd_workspace_bytes",
+               "gdn_paged_attn_workspace_bytes"}
 
 _lock = threading.Lock()
 _lib = None

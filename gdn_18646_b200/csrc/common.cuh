@@ -34,7 +34,7 @@ int prefill_segment(const void* q, const void* k, const void* v, const float* A_
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Device-side error flag bits.
-enum : unsigned int { DERR_TIMEOUT = 1u, DERR_VARLEN = 2u };
+enum : unsigned int { DERR_TIMEOUT = 1u, DERR_VARLEN = 2u, DERR_PAGED = 4u };
 
 // ---------------------------------------------------------------------------
 // device helpers

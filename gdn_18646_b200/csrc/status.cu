@@ -150,6 +150,11 @@ extern "C" int gdn_check_device_error(void) {
         cudaMemcpy(gdn::device_error_word(), &zero, sizeof(zero), cudaMemcpyHostToDevice);
         if (word & gdn::DERR_TIMEOUT)
             return gdn::fail(GDN_ERR_DEVICE_TIMEOUT, "a kernel gave up on a bounded wait (device error word 0x%x)", word);
+        if (word & gdn::DERR_PAGED)
+            return gdn::fail(GDN_ERR_SHAPE,
+                             "gdn_rope_append / gdn_paged_attn_fwd: block_table, kv_lens or cu_seqlens named pages or "
+                             "positions outside the cache; those were skipped (device error word 0x%x)",
+                             word);
         return gdn::fail(GDN_ERR_SHAPE,
                          "gdn_prefill_varlen_fwd: cu_seqlens held offsets that are negative, decreasing or past Ttot; "
                          "those sequences were skipped (device error word 0x%x)",

@@ -556,6 +556,347 @@ def decode_proj(x, segments, *, norm_gamma=None, eps=1e-6):
 
 
 # ---------------------------------------------------------------------------
+# the softmax-attention block of a hybrid stack: the norms around a block, rotary
+# positions, the paged cache and its attention
+# ---------------------------------------------------------------------------
+
+
+def _gate_rows(gate, R, D):
+    """(gate rows, whether the gate is per row) of a gate [D] or [G, D]; checks it."""
+    if gate is None:
+        return 0, False
+    _cuda_contig(gate, "gate", torch.bfloat16)
+    _need(gate.dim() in (1, 2) and gate.shape[-1] == D, f"gate must be [{D}] or [G, {D}]")
+    if gate.dim() == 1:
+        return 1, False
+    G = gate.shape[0]
+    _need(G >= 1 and R % G == 0, f"gate rows ({G}) must divide the {R} rows")
+    return G, G == R
+
+
+def _norm_weight(t, name, D):
+    if t is not None:
+        _cuda_contig(t, name, torch.bfloat16)
+        _need(t.dim() == 1 and t.shape[0] == D, f"{name} must be [{D}]")
+
+
+def block_norm(y, h, *, gamma_post=None, gate=None, gamma_pre=None, residual_scale=1.0, eps=1e-6, h_out=None,
+               x_out=None):
+    """The norms around a block, with its gate and the residual scale, in one pass
+    (gdn_block_norm_fwd): h' = residual_scale * h + gate * u with u = RMSNorm(y) *
+    gamma_post (u = y without it), and x = RMSNorm(h') * gamma_pre, the next block's input.
+
+    y [..., D] bf16; h [..., D] bf16 or f32 (the residual stream); gate None, [D], or
+    [G, D] bf16 with G dividing the rows (a gate row per sequence, or per token);
+    gammas [D] bf16.  Returns (h', x): h' in h's type, x bf16 or None without
+    gamma_pre.  ``h_out=h`` updates the residual stream in place."""
+    _cuda_contig(y, "y", torch.bfloat16)
+    _cuda_contig(h, "h")
+    _need(h.shape == y.shape and y.dim() >= 1, "h must have y's shape")
+    hdt = _gate_dtype(h, "h")
+    D = y.shape[-1]
+    _need(D > 0, "y must have at least one column")
+    R = y.numel() // D
+    G, _ = _gate_rows(gate, R, D)
+    _norm_weight(gamma_post, "gamma_post", D)
+    _norm_weight(gamma_pre, "gamma_pre", D)
+    if h_out is None:
+        h_out = torch.empty_like(h)
+    else:
+        _cuda_contig(h_out, "h_out", h.dtype)
+        _need(h_out.shape == h.shape, "h_out must have h's shape")
+    if gamma_pre is None:
+        x_out = None
+    elif x_out is None:
+        x_out = torch.empty_like(y)
+    else:
+        _cuda_contig(x_out, "x_out", torch.bfloat16)
+        _need(x_out.shape == y.shape, "x_out must have y's shape")
+    if R == 0:
+        return h_out, x_out
+    _lib.call("gdn_block_norm_fwd", _ptr(y), _ptr(h), hdt, _ptr(gamma_post), _ptr(gate), G, _ptr(gamma_pre),
+              float(residual_scale), _ptr(h_out), _ptr(x_out), R, D, float(eps), _stream())
+    return h_out, x_out
+
+
+def block_norm_backward(y, h_out, dh_out=None, dx=None, *, gamma_post=None, gate=None, gamma_pre=None,
+                        residual_scale=1.0, eps=1e-6):
+    """Gradients of ``block_norm`` from y and its stored result h_out (gdn_block_norm_bwd):
+    dh_out [..., D] in h_out's type or None (zero), dx bf16 (with gamma_pre).  Returns a
+    dict of dy bf16, dh in h_out's type, dgamma_post and dgamma_pre [D] f32 and dgate
+    (f32 [D] or [G, D], sums over the rows that share a gate row; bf16 [R, D] for a gate
+    row per row), None where there is no such input."""
+    _cuda_contig(y, "y", torch.bfloat16)
+    _cuda_contig(h_out, "h_out")
+    _need(h_out.shape == y.shape and y.dim() >= 1, "h_out must have y's shape")
+    hdt = _gate_dtype(h_out, "h_out")
+    D = y.shape[-1]
+    _need(D > 0, "y must have at least one column")
+    R = y.numel() // D
+    G, per_row = _gate_rows(gate, R, D)
+    _norm_weight(gamma_post, "gamma_post", D)
+    _norm_weight(gamma_pre, "gamma_pre", D)
+    if dh_out is not None:
+        _cuda_contig(dh_out, "dh_out", h_out.dtype)
+        _need(dh_out.shape == y.shape, "dh_out must have y's shape")
+    if gamma_pre is None:
+        dx = None
+    else:
+        _need(dx is not None, "dx is required with gamma_pre")
+        _cuda_contig(dx, "dx", torch.bfloat16)
+        _need(dx.shape == y.shape, "dx must have y's shape")
+    f32 = dict(dtype=torch.float32, device=y.device)
+    g = dict(dy=torch.empty_like(y), dh=torch.empty_like(h_out),
+             dgate=None if gate is None else torch.empty_like(gate) if per_row else torch.empty(gate.shape, **f32),
+             dgamma_post=None if gamma_post is None else torch.empty(D, **f32),
+             dgamma_pre=None if gamma_pre is None else torch.empty(D, **f32))
+    if R == 0:
+        return {n: None if t is None else t.zero_() for n, t in g.items()}
+    ws_bytes = int(_lib.lib().gdn_block_norm_bwd_workspace_bytes(R, D, G))
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=y.device)
+    _lib.call("gdn_block_norm_bwd", _ptr(y), _ptr(h_out), hdt, _ptr(dh_out), _ptr(dx), _ptr(gamma_post), _ptr(gate), G,
+              _ptr(gamma_pre), float(residual_scale), _ptr(g["dy"]), _ptr(g["dh"]), _ptr(g["dgate"]),
+              GDN_DTYPE_BF16 if per_row else GDN_DTYPE_F32, _ptr(g["dgamma_post"]), _ptr(g["dgamma_pre"]), R, D,
+              float(eps), _ptr(ws), ws_bytes, _stream())
+    return g
+
+
+class BlockNormFunction(torch.autograd.Function):
+    """``block_norm`` as an autograd op: differentiable in y, h, gamma_post, gate and
+    gamma_pre; outputs (h', x)."""
+
+    @staticmethod
+    def forward(ctx, y, h, gamma_post, gate, gamma_pre, residual_scale, eps):
+        h_out, x = block_norm(y, h, gamma_post=gamma_post, gate=gate, gamma_pre=gamma_pre,
+                              residual_scale=residual_scale, eps=eps)
+        ctx.save_for_backward(y, h_out, gamma_post, gate, gamma_pre)
+        ctx.scale, ctx.eps = residual_scale, eps
+        return h_out, x
+
+    @staticmethod
+    def backward(ctx, dh, dx):
+        y, h_out, gamma_post, gate, gamma_pre = ctx.saved_tensors
+        if dx is None and gamma_pre is not None:
+            dx = torch.zeros_like(y)
+        g = block_norm_backward(y, h_out, None if dh is None else dh.contiguous(),
+                                None if dx is None else dx.contiguous(), gamma_post=gamma_post, gate=gate,
+                                gamma_pre=gamma_pre, residual_scale=ctx.scale, eps=ctx.eps)
+        like = lambda d, p: None if p is None else d.to(p.dtype)  # noqa: E731
+        return (g["dy"], g["dh"], like(g["dgamma_post"], gamma_post), like(g["dgate"], gate),
+                like(g["dgamma_pre"], gamma_pre), None, None)
+
+
+def block_norm_autograd(y, h, *, gamma_post=None, gate=None, gamma_pre=None, residual_scale=1.0, eps=1e-6):
+    """Differentiable ``block_norm`` (see BlockNormFunction)."""
+    return BlockNormFunction.apply(y, h, gamma_post, gate, gamma_pre, residual_scale, eps)
+
+
+_ROPE_STYLES = {"half": _lib.GDN_ROPE_HALF, "interleaved": _lib.GDN_ROPE_INTERLEAVED}
+
+
+def _token_rows(t, name):
+    """(tokens, heads, D, elements between tokens) of [..., H, D] bf16 whose heads and
+    values are contiguous and whose tokens are rows of one stride (a slice of a fused
+    projection is one)."""
+    _need(t.is_cuda and t.dtype == torch.bfloat16, f"{name} must be a bfloat16 CUDA tensor")
+    _need(t.dim() >= 3, f"{name} must be [..., heads, head dim]")
+    H, D = t.shape[-2], t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // (H * D) if H * D else 0, H, D, H * D
+    _need(t.stride(-1) == 1 and (H == 1 or t.stride(-2) == D), f"{name}: heads and values must be contiguous")
+    T, ld = 1, None
+    for n, s in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld = s
+        else:
+            _need(s == ld * T, f"{name}: tokens must be rows of one stride")
+        T *= n
+    return T, H, D, (H * D if ld is None else ld)
+
+
+def _rope_spec(positions, inv_freq, sections, style, T):
+    _need(style in _ROPE_STYLES, f"style must be 'half' or 'interleaved', got {style!r}")
+    _need(positions.is_cuda and positions.dtype == torch.int32, "positions must be an int32 CUDA tensor")
+    _need(inv_freq.is_cuda and inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
+          "inv_freq must be a contiguous float32 CUDA vector")
+    pairs = inv_freq.shape[0]
+    sections = (pairs,) if sections is None else tuple(sections)
+    axes = len(sections)
+    _need(positions.is_contiguous() and positions.numel() == axes * T,
+          f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis)")
+    sec = (ctypes.c_int * axes)(*sections)
+    spec = _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.cast(sec, ctypes.c_void_p), axes, 2 * pairs,
+                         _ROPE_STYLES[style])
+    spec._keep = sec
+    return spec
+
+
+def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=False, q_out=None, k_out=None):
+    """Rotary positions with several axes (gdn_rope_fwd): pair i of the first
+    2 * len(inv_freq) values of each head is turned by positions[axis][t] * inv_freq[i],
+    where ``sections`` counts the pairs of each axis in turn (None: one axis).
+
+    q [..., Hq, D], k [..., Hk, D] bf16 or None (tokens may be strided rows); positions
+    int32 [axes, tokens]; inv_freq f32 [rot / 2]; style "half" pairs values (i, i + rot/2),
+    "interleaved" (2i, 2i + 1).  ``inverse`` turns back, which is the gradient.
+    Returns (q_out, k_out), contiguous; ``q_out=q`` works in place."""
+    T, Hq, D, q_ld = _token_rows(q, "q")
+    Hk = k_ld = 0
+    if k is not None:
+        Tk, Hk, Dk, k_ld = _token_rows(k, "k")
+        _need(Tk == T and Dk == D, "k must have q's tokens and head dim")
+    spec = _rope_spec(positions, inv_freq, sections, style, T)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _cuda_contig(q_out, "q_out", torch.bfloat16)
+        _need(q_out.shape == q.shape, "q_out must have q's shape")
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    elif k is not None:
+        _cuda_contig(k_out, "k_out", torch.bfloat16)
+        _need(k_out.shape == k.shape, "k_out must have k's shape")
+    if T == 0:
+        return q_out, (k_out if k is not None else None)
+    _lib.call("gdn_rope_fwd", _ptr(q), q_ld, _ptr(k), k_ld, _ptr(q_out), _ptr(k_out), ctypes.byref(spec),
+              1 if inverse else 0, T, Hq, Hk, D, _stream())
+    return q_out, (k_out if k is not None else None)
+
+
+class RopeFunction(torch.autograd.Function):
+    """``rope`` as an autograd op, differentiable in q and k."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, sections, style):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.sections, ctx.style = sections, style
+        return rope(q, k, positions, inv_freq, sections, style=style)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq = ctx.saved_tensors
+        dq, dk = rope(dq.contiguous(), None if dk is None else dk.contiguous(), positions, inv_freq, ctx.sections,
+                      style=ctx.style, inverse=True)
+        return dq, dk, None, None, None, None
+
+
+def rope_autograd(q, k, positions, inv_freq, sections=None, *, style="half"):
+    """Differentiable ``rope`` (see RopeFunction)."""
+    return RopeFunction.apply(q, k, positions, inv_freq, sections, style)
+
+
+def _paged_cache(k_cache, v_cache, block_table, layout):
+    _need(layout in ("bthd", "bhtd"), f"layout must be 'bthd' or 'bhtd', got {layout!r}")
+    _need(k_cache.is_cuda and v_cache.is_cuda and k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16,
+          "k_cache and v_cache must be bfloat16 CUDA tensors")
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+          "k_cache and v_cache must be 4-d and share shape and strides")
+    _need(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
+          and (block_table.stride(1) == 1 or block_table.shape[1] == 1), "block_table must be int32 [B, pages] CUDA rows")
+    st = k_cache.stride()
+    _need(st[3] == 1, "k_cache, v_cache: the values of a row must be contiguous")
+    if layout == "bthd":
+        pages, page_size, n_kv, D = k_cache.shape
+        token, head = st[1], st[2]
+    else:
+        pages, n_kv, page_size, D = k_cache.shape
+        token, head = st[2], st[1]
+    B, width = block_table.shape
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                           block_table.stride(0) if B > 1 else width, st[0], token, head, pages, page_size, width, n_kv, D)
+
+
+def _sequences(cu_seqlens, kv_lens, block_table):
+    _cuda_contig(cu_seqlens, "cu_seqlens", torch.int32)
+    _cuda_contig(kv_lens, "kv_lens", torch.int32)
+    B = kv_lens.numel()
+    _need(B >= 1 and cu_seqlens.numel() == B + 1 and block_table.shape[0] == B,
+          "cu_seqlens must have B + 1 entries, kv_lens and block_table B rows")
+    return B
+
+
+def rope_append(q, k, v, positions, inv_freq, sections, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *,
+                style="half", layout="bthd", q_out=None):
+    """The step before ``paged_attention`` (gdn_rope_append): q is turned as by ``rope``
+    and returned, the turned keys and the values are written into the paged cache.
+
+    q [T, Hq, D], k, v [T, Hkv, D] bf16: the new tokens of B sequences, packed
+    (cu_seqlens int32 [B + 1]); they are the last ones of kv_lens int32 [B] positions.
+    k_cache, v_cache [pages, page_size, Hkv, D] (layout "bthd") or [pages, Hkv, page_size,
+    D] ("bhtd"), strided slices of a larger pool too; block_table int32 [B, max_pages].
+    Sequence lengths live on the device, so the call can be captured in a CUDA graph."""
+    T, Hq, D, q_ld = _token_rows(q, "q")
+    Tk, Hk, Dk, k_ld = _token_rows(k, "k")
+    Tv, Hv, Dv, v_ld = _token_rows(v, "v")
+    cache = _paged_cache(k_cache, v_cache, block_table, layout)
+    B = _sequences(cu_seqlens, kv_lens, block_table)
+    _need(Tk == T and Tv == T and Hk == Hv == cache.n_kv and D == Dk == Dv == cache.head_dim,
+          "q, k, v must have the same tokens and the cache's heads and head dim")
+    spec = _rope_spec(positions, inv_freq, sections, style, T)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _cuda_contig(q_out, "q_out", torch.bfloat16)
+        _need(q_out.shape == q.shape, "q_out must have q's shape")
+    if T == 0:
+        return q_out
+    _lib.call("gdn_rope_append", _ptr(q), q_ld, _ptr(k), k_ld, _ptr(v), v_ld, _ptr(q_out), ctypes.byref(spec),
+              ctypes.byref(cache), _ptr(cu_seqlens), _ptr(kv_lens), B, T, Hq, _stream())
+    return q_out
+
+
+def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, max_q=None, max_kv=None, scale=0.0,
+                    causal=True, window=0, layout="bthd", out=None, return_lse=False, workspace=None):
+    """Softmax attention of new tokens over a paged cache that holds them already
+    (gdn_paged_attn_fwd): single tokens, drafted ones and chunks of a prompt alike.
+
+    q [T, Hq, D] bf16, the new tokens of B sequences, packed; caches, block_table,
+    cu_seqlens and kv_lens as ``rope_append``.  Token i of a sequence sees its positions
+    0 .. kv_len - q_len + i (``causal``; otherwise all), with ``window`` only the last
+    ``window`` of them.  max_q, max_kv: the longest new chunk and an upper bound of the
+    lengths, on the host (max_q is read from cu_seqlens with a device->host copy when not
+    given, max_kv defaults to the block table's width).  scale 0 -> 1/sqrt(D).
+    ``workspace``: uint8 CUDA tensor of at least paged_attention_workspace(...) bytes
+    (allocated per call if None).  Returns out [T, Hq, D] bf16, with ``return_lse`` also
+    the log of the softmax's sum, f32 [T, Hq].  A token that sees nothing gets zeros
+    and -inf."""
+    T, Hq, D, q_ld = _token_rows(q, "q")
+    cache = _paged_cache(k_cache, v_cache, block_table, layout)
+    B = _sequences(cu_seqlens, kv_lens, block_table)
+    _need(D == cache.head_dim, "q must have the cache's head dim")
+    if max_q is None:
+        max_q = int((cu_seqlens[1:] - cu_seqlens[:-1]).max())
+    if max_kv is None:
+        max_kv = cache.max_pages * cache.page_size
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _cuda_contig(out, "out", torch.bfloat16)
+        _need(out.shape == q.shape, "out must have q's shape")
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    if T == 0:
+        return (out, lse) if return_lse else out
+    ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
+    if workspace is None:
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    else:
+        _need(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.numel() >= ws_bytes,
+              f"workspace: uint8 CUDA tensor of at least {ws_bytes} bytes required")
+    _lib.call("gdn_paged_attn_fwd", _ptr(q), q_ld, ctypes.byref(cache), _ptr(cu_seqlens), _ptr(kv_lens), _ptr(out),
+              _ptr(lse), B, T, Hq, max_q, max_kv, 1 if causal else 0, window, float(scale), _ptr(workspace),
+              ws_bytes if workspace is not None else 0, _stream())
+    return (out, lse) if return_lse else out
+
+
+def paged_attention_workspace(B, T, Hq, n_kv, head_dim, max_q, max_kv, window=0):
+    """Bytes of workspace ``paged_attention`` needs for calls up to these sizes."""
+    return int(_lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, n_kv, head_dim, max_q, max_kv, window))
+
+
+# ---------------------------------------------------------------------------
 # reference-surface modules (drop-in for GDNLayerCustom's ``exts`` dict)
 # ---------------------------------------------------------------------------
 

@@ -405,6 +405,141 @@ int gdn_gated_rmsnorm_fwd(const void* x, int x_dtype, const void* z, const void*
                           int R, int D, float eps, void* stream);
 
 /*
+ * The norms around a block of a residual stack, fused with the block's gate and
+ * the residual scale.  With u = y, or RMSNorm(y) * gamma_post:
+ *   h_out = residual_scale * h + gate * u
+ *   x     = RMSNorm(h_out) * gamma_pre        (the next block's input; from the
+ *                                              fp32 h_out, before it is stored)
+ *   y          bf16 [R, D], the block's output
+ *   h, h_out   [R, D] in h_dtype (bf16 or f32), the residual stream; may be one buffer
+ *   gamma_post bf16 [D] or NULL (no norm after the block: u = y)
+ *   gate       bf16 [gate_rows, D] or NULL (1); row r uses gate row
+ *              r / (R / gate_rows): one for all, one per sequence or one per token
+ *   gamma_pre  bf16 [D] or NULL (x is not written and may be NULL)
+ *   x          bf16 [R, D]
+ * D % 8 == 0, D <= 8192, R % gate_rows == 0; pointers 16-byte aligned.
+ * No counterpart in the reference, whose layer has no residual stream.
+ */
+int gdn_block_norm_fwd(const void* y, const void* h, int h_dtype, const void* gamma_post, const void* gate,
+                       int gate_rows, const void* gamma_pre, float residual_scale, void* h_out, void* x,
+                       int R, int D, float eps, void* stream);
+
+/*
+ * Gradients of gdn_block_norm_fwd, from y and the stored h_out:
+ *   dh_out      [R, D] in h_dtype or NULL (0), dx bf16 [R, D] (NULL without gamma_pre)
+ *   dy          bf16 [R, D]; dh [R, D] in h_dtype (may be dh_out's buffer)
+ *   dgate       [gate_rows, D] in dgate_dtype: f32, or bf16 when every row has its
+ *               own gate (gate_rows == R, nothing is summed); NULL without a gate
+ *   dgamma_post, dgamma_pre  f32 [D], NULL without the norm
+ * Sums over rows are fp32 in a fixed order: the same call gives the same bits.
+ * workspace: gdn_block_norm_bwd_workspace_bytes(R, D, gate_rows) bytes (gate_rows
+ * 0 without a gate; 0 for invalid sizes), 16-byte aligned.
+ */
+int gdn_block_norm_bwd(const void* y, const void* h_out, int h_dtype, const void* dh_out, const void* dx,
+                       const void* gamma_post, const void* gate, int gate_rows, const void* gamma_pre,
+                       float residual_scale, void* dy, void* dh, void* dgate, int dgate_dtype,
+                       float* dgamma_post, float* dgamma_pre, int R, int D, float eps,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t gdn_block_norm_bwd_workspace_bytes(int R, int D, int gate_rows);
+
+/*
+ * Rotary positions with several axes.  Pair i of the first rot values of a head is
+ * turned by the angle positions[axis(i)][t] * inv_freq[i], where axis(i) is the
+ * section that i falls in (sections[0] pairs of axis 0, then sections[1] of axis 1, ...):
+ *   (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin);   values past rot are copied.
+ *   style      GDN_ROPE_HALF: pair i = values (i, i + rot / 2);
+ *              GDN_ROPE_INTERLEAVED: pair i = values (2 i, 2 i + 1)
+ *   positions  int32 [axes][T] (row stride positions_ld elements)
+ *   inv_freq   f32 [rot / 2]
+ *   sections   HOST pointer, axes ints, sum rot / 2; 1 <= axes <= 4
+ * D in {64, 128, 256}; rot % 16 == 0, 0 < rot <= D.
+ */
+enum { GDN_ROPE_HALF = 0, GDN_ROPE_INTERLEAVED = 1 };
+typedef struct {
+    const int* positions;
+    long positions_ld;
+    const float* inv_freq;
+    const int* sections;
+    int axes;
+    int rot;
+    int style;
+} gdn_rope_spec;
+
+/*
+ * Turns q [T, Hq, D] and k [T, Hk, D] bf16 (token rows q_ld / k_ld elements apart,
+ * heads and values contiguous) into q_out [T, Hq, D] and k_out [T, Hk, D]
+ * (contiguous; may be q and k when those are).  k may be NULL with Hk 0.  inverse: turned by the
+ * negative angles, which is the gradient of the rotation.  Strides in multiples
+ * of 8, pointers 16-byte aligned.  No counterpart in the reference (a linear
+ * layer without positions).
+ */
+int gdn_rope_fwd(const void* q, long q_ld, const void* k, long k_ld, void* q_out, void* k_out,
+                 const gdn_rope_spec* spec, int inverse, int T, int Hq, int Hk, int D, void* stream);
+
+/*
+ * A paged cache of keys and values: position p of sequence b is row p % page_size
+ * of page block_table[b * table_ld + p / page_size].  k and v bf16, element
+ * (page, row, head, i) at page * page_stride + row * token_stride + head *
+ * head_stride + i: [num_pages, page_size, Hkv, D], [num_pages, Hkv, page_size, D]
+ * or a slice of a larger pool.  page_size a power of two, at least 16; strides
+ * multiples of 8 and 16-byte aligned pointers.  block_table entries past a
+ * sequence's length are not read.
+ */
+typedef struct {
+    void* k;
+    void* v;
+    const int* block_table;
+    long table_ld;
+    long page_stride;
+    long token_stride;
+    long head_stride;
+    int num_pages;
+    int page_size;
+    int max_pages;                 /* entries of one block_table row */
+    int n_kv;
+    int head_dim;
+} gdn_paged_cache;
+
+/*
+ * The step before paged attention: q [T, Hq, D] turned into q_out, and the new
+ * keys (turned) and values [T, Hkv, D] written into the cache.  The T tokens are
+ * those of B sequences, packed: sequence b has tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1], the last ones of its kv_lens[b] positions (device int32).
+ * A token whose position or page is outside the table or the cache is not
+ * written, and gdn_check_device_error() reports it.  D in {64, 128, 256}.
+ */
+int gdn_rope_append(const void* q, long q_ld, const void* k, long k_ld, const void* v, long v_ld, void* q_out,
+                    const gdn_rope_spec* spec, const gdn_paged_cache* cache, const int* cu_seqlens,
+                    const int* kv_lens, int B, int T, int Hq, void* stream);
+
+/*
+ * Softmax attention of new tokens over a paged cache that holds them already.
+ * Token i of sequence b stands at position p = kv_lens[b] - q_len + i and sees the
+ * positions 0 .. p, with window > 0 only the last `window` of them (causal == 0:
+ * all kv_lens[b] positions, window must be 0):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,    lse = log sum_j exp(scale * q . k_j)
+ * A token that sees nothing (an empty cache, or more tokens than positions) gets
+ * zeros and an lse of -infinity.  Query head h reads kv head h / (Hq / n_kv).
+ *   q, out     bf16 [Ttot, Hq, D], q with token rows q_ld elements apart; out contiguous
+ *   lse        f32 [Ttot, Hq] or NULL
+ *   cu_seqlens int32 [B + 1], kv_lens int32 [B], on the device
+ *   max_q, max_kv  at least the longest q_len and kv_len (host; they size the launch)
+ *   scale      0.0f -> 1/sqrt(D)
+ * What the cache holds at positions that no token of a sequence sees may be
+ * anything, NaN included, and so may the block_table entries of pages that hold
+ * only such positions.  A longer q_len or kv_len than max_q or max_kv, and pages
+ * outside the cache, are reported by gdn_check_device_error(); the pages are
+ * taken as zeros.  D in {64, 128}, Hq / n_kv <= 64.
+ * workspace: gdn_paged_attn_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes).
+ * No counterpart in the reference (it has no softmax attention).
+ */
+int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cache* cache, const int* cu_seqlens,
+                       const int* kv_lens, void* out, float* lse, int B, int Ttot, int Hq, int max_q, int max_kv,
+                       int causal, int window, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t gdn_paged_attn_workspace_bytes(int B, int Ttot, int Hq, int n_kv, int head_dim, int max_q, int max_kv,
+                                      int window);
+
+/*
  * One channel segment of gdn_decode_proj_fwd: output channels c in [0, C) of
  * weight W [C, D] bf16, written to y[b * ldy + c] (bf16).
  *   conv_w         bf16 [C, 4] or NULL.  With it: y = SiLU(conv4(history, x.W[c]))
@@ -539,9 +674,10 @@ const char* gdn_version(void);
 
 /*
  * Reads and clears the device-side error word of the current device (set by a
- * kernel that gave up on a bounded wait, or by a varlen prefill that met
- * invalid offsets).  Synchronises the device.  Returns GDN_OK,
- * GDN_ERR_DEVICE_TIMEOUT, GDN_ERR_SHAPE (invalid varlen offsets) or GDN_ERR_CUDA.
+ * kernel that gave up on a bounded wait, by a varlen prefill that met invalid
+ * offsets, or by a paged operator that met a page or a position outside its
+ * cache).  Synchronises the device.  Returns GDN_OK, GDN_ERR_DEVICE_TIMEOUT,
+ * GDN_ERR_SHAPE (invalid varlen offsets, pages or positions) or GDN_ERR_CUDA.
  */
 int gdn_check_device_error(void);
 
