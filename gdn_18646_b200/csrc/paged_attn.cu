@@ -1,82 +1,781 @@
-// paged_attn.cu -- softmax attention of new tokens over a paged key/value cache.
+// paged_attn.cu -- softmax attention of new tokens over a paged key/value cache, on tcgen05.
 //
 // Token i of sequence b stands at position p = kv_len - q_len + i and sees the positions
-// lo .. hi of its mask; one pass over them with the running maximum m and sum l of the
-// softmax (fp32):
-//   s_j = scale q.k_j,  m' = max(m, s_j),  l' = l e^(m-m') + e^(s_j-m'),
-//   o' = o e^(m-m') + e^(s_j-m') v_j;   out = o / l, lse = m + log l
-// A row that sees nothing keeps l = 0: out 0, lse -inf.
+// lo .. hi of its mask.  One pass over them in tiles of 128, with a running reference
+// maximum m and sum l per row (fp32; c = scale log2 e):
+//   p_j = 2^(c (s_j - m)),   l = l a + sum p_j,   o = o a + sum p_j v_j,   s_j = q . k_j
+//   out = o / l,  lse = scale m + ln l;   a row that sees nothing keeps l = 0: out 0, lse -inf.
+// a = 2^(c (m_old - m_new)) is 1 unless the maximum grew by more than 2^8 in p: the sums
+// are exact for any m near the maximum, so a smaller growth leaves m and o where they are.
+//
+// Rows.  The G query heads that share a kv head are packed with their tokens into rows
+// (row = token G + g), floor(128 / G) tokens to a tile of 128, so a decode step and a
+// chunk run the same kernel and a key is read once for its whole group.
+//
+// Work.  An item is (sequence, kv head, QT row tiles); its kv tiles are the ones that some
+// row of it sees.  All kv tiles of all items, with a constant cost per item, form one line
+// that is cut into equal pieces, one per CTA: a long sequence is split over many CTAs and a
+// CTA may take many short ones.  An item cut by a piece's end leaves its o, m, l in the
+// workspace, and a second small kernel joins such parts in a fixed order.  The pieces follow
+// from the lengths on the device, so a captured launch serves every length.
+//
+// Roles.  A producer warp loads q, k, v by TMA (128-byte swizzle, a ring of stages; a
+// lane per page); one thread issues the MMAs; a warpgroup per row tile does the softmax,
+// a thread per row:
+//   S = Q K^T   M 128, N 128 (SS)      -> TMEM, 128 columns per S buffer
+//   P (bf16) overwrites S in TMEM      (rounded to bf16: 2^-9 rms of each weight)
+//   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
+// With two row tiles the tensor core works for one while the softmax of the other runs;
+// with one row tile (at most 128 rows, the decode step) S is double buffered instead.
+#include <cstring>
+
 #include "common.cuh"
 #include "paged.cuh"
+#include "tensormap.h"
 
 namespace gdn {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kTile = 128;            // positions per kv tile; rows per row tile
+constexpr int kMaxCtas = 148;         // pieces of the work line: one CTA per SM of a B200
+constexpr int kItemCost = 1;          // kv tiles that starting an item is worth
+constexpr int kMinPiece = 4;          // shortest piece: splitting finer costs more to join
 
 struct AttnArgs {
-    const uint16_t* q;
-    long q_ld;
     uint16_t* out;
     float* lse;
-    PagedView cache;
     const int* cu;
     const int* kv_lens;
-    int B, T, Hq, group;
-    int max_q, max_kv;
-    int causal, window;
+    const int* table;
+    long table_ld;
+    int num_pages, page_shift;
+    int B, T, Hq, n_kv, group;        // group: query heads per kv head
+    int tile_tokens;                  // floor(128 / group)
+    int max_q, max_kv, causal, window;
     float scale;
     unsigned int* err;
+    int* part_state;                  // [ctas][8]: what a CTA left unfinished
+    float* part_ml;                   // [ctas][2][QT 128][2]: m, l
+    float* part_o;                    // [ctas][2][QT 128][D]
 };
 
-// One warp per (token, query head); a lane owns D/32 consecutive values of a row.
-template <int D>
-__global__ void __launch_bounds__(32 * kWarps) paged_attn_rows_kernel(const AttnArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long job = static_cast<long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    if (job >= static_cast<long>(a.T) * a.Hq) return;
-    const int t = static_cast<int>(job / a.Hq), h = static_cast<int>(job % a.Hq), kh = h / a.group;
-    const int b = sequence_of(a.cu, a.B, t);
-    const int c0 = a.cu[b], c1 = a.cu[b + 1];
-    int len = a.kv_lens[b];
-    if (t < c0 || t >= c1 || c0 < 0 || c1 > a.T || c1 - c0 > a.max_q || len > a.max_kv || len < 0) {
-        if (lane == 0) atomicOr(a.err, DERR_PAGED);
-        len = min(max(len, 0), a.max_kv);
+struct alignas(64) AttnMaps {
+    CUtensorMap q, k, v;
+};
+
+// sum over i in [0, n) of floor((a i + b) / m), for a, b >= 0 (the Euclid-like reduction)
+__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+    long long s = 0;
+    while (n > 0) {
+        s += (n - 1) * n / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const long long y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const long long t = m;
+        m = a;
+        a = t;
     }
-    const int pos = len - c1 + t;
-    int hi = a.causal ? min(pos + 1, len) : len, lo = 0;
-    if (a.window > 0) lo = max(0, pos + 1 - a.window);
-    const uint16_t* qp = a.q + t * a.q_ld + h * D + lane * V;
-    float q[V], o[V] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) q[i] = bf16_bits_to_f32(qp[i]) * a.scale;
-    for (int j = lo; j < hi; ++j) {
-        const int page = a.cache.table[b * a.cache.table_ld + (j >> a.cache.page_shift)];
-        if (page < 0 || page >= a.cache.num_pages) {
-            if (lane == 0) atomicOr(a.err, DERR_PAGED);
+    return s;
+}
+
+// A wait that all lanes of a warp leave alike, also when it gives up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, dead));
+}
+
+// One sequence as the kernel sees it; tt: tokens per item.
+struct Seq {
+    int c0, n, kv, items;             // first packed token, new tokens, positions, row-tile groups
+    __device__ __forceinline__ void load(const AttnArgs& a, int b, int tt, bool report) {
+        c0 = a.cu[b];
+        const int c1 = a.cu[b + 1];
+        kv = a.kv_lens[b];
+        n = c1 - c0;
+        if (c0 < 0 || c1 > a.T || n < 0 || n > a.max_q || kv < 0 || kv > a.max_kv) {
+            if (report) atomicOr(a.err, DERR_PAGED);
+            c0 = n = kv = 0;
         }
-        const bool have = page >= 0 && page < a.cache.num_pages;
-        const long at = (have ? page : 0) * a.cache.page_stride +
-                        (j & ((1 << a.cache.page_shift) - 1)) * a.cache.token_stride + kh * a.cache.head_stride + lane * V;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += q[i] * (have ? bf16_bits_to_f32(a.cache.k[at + i]) : 0.f);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const float mn = fmaxf(m, s);
-        if (mn == -INFINITY) continue;
-        const float c = __expf(m - mn), p = __expf(s - mn);
-        m = mn;
-        l = l * c + p;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = o[i] * c + p * (have ? bf16_bits_to_f32(a.cache.v[at + i]) : 0.f);
+        items = (n + tt - 1) / tt;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint16_t* op = a.out + (static_cast<long>(t) * a.Hq + h) * D + lane * V;
+    // positions [lo, hi) that tokens first .. last of the chunk see between them
+    __device__ __forceinline__ void range(const AttnArgs& a, int first, int last, int& lo, int& hi) const {
+        const int p = kv - n;
+        hi = a.causal ? max(0, min(p + last + 1, kv)) : kv;
+        lo = a.window > 0 ? max(0, p + first + 1 - a.window) : 0;
+        if (hi <= lo) lo = hi = 0;
+    }
+    __device__ __forceinline__ void tiles(const AttnArgs& a, int item, int tt, int& first, int& count, int& lo, int& hi) const {
+        range(a, item * tt, min((item + 1) * tt, n) - 1, lo, hi);
+        first = lo / kTile;
+        count = hi > 0 ? (hi + kTile - 1) / kTile - first : 0;
+    }
+    // cost of the items before `q` of one kv head
+    __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
+        if (q == 0) return 0;
+        long long s = static_cast<long long>(q) * kItemCost;
+        const long long full = (kv + kTile - 1) / kTile;
+        if (!a.causal) return s + q * full;
+        const long long p = kv - n;
+        const int m = min(q, items - 1);
+        long long i0 = p + tt > 0 ? 0 : (-p) / tt;              // first item with p + (i + 1) tt > 0
+        if (i0 < m) s += floor_sum(m - i0, kTile, tt, p + (i0 + 1) * tt + kTile - 1);
+        if (q == items) s += full;
+        if (a.window > 0) {
+            const long long w = p + 1 - a.window;               // lo of item i: max(0, w + i tt)
+            long long i1 = w >= 0 ? 0 : (-w + tt - 1) / tt;
+            if (i1 < q) s -= floor_sum(q - i1, kTile, tt, w + i1 * tt);
+        }
+        return s;
+    }
+};
+
+// Where a CTA's piece of the work line starts, and its length.
+struct Piece {
+    int b, head, item;
+    int skip;                         // units of the first item that belong to earlier CTAs
+    long long units;
+};
+
+// Walks the items of a piece; every role of the CTA does so on its own.
+struct Walk {
+    Seq s;
+    int b, head, item, skip;
+    long long left;
+    int first, count, lo, hi;         // the item's kv tiles and positions
+    int t0, t1;                       // this CTA's part of its tiles: [t0, t1) of [0, count)
+    __device__ __forceinline__ void start(const AttnArgs& a, const Piece& p, int tt) {
+        b = p.b;
+        head = p.head;
+        item = p.item;
+        skip = p.skip;
+        left = p.units;
+        if (left > 0) {
+            s.load(a, b, tt, false);
+            set(a, tt);
+        }
+    }
+    __device__ __forceinline__ bool valid() const { return left > 0; }
+    __device__ __forceinline__ void set(const AttnArgs& a, int tt) {
+        s.tiles(a, item, tt, first, count, lo, hi);
+        const long long end = min(static_cast<long long>(count + kItemCost), skip + left);
+        t0 = max(skip - kItemCost, 0);
+        t1 = max(static_cast<int>(end) - kItemCost, 0);
+    }
+    __device__ __forceinline__ void next(const AttnArgs& a, int tt) {
+        left -= count + kItemCost - skip;
+        skip = 0;
+        if (left <= 0) return;
+        if (++item == s.items) {
+            item = 0;
+            if (++head == a.n_kv) {
+                head = 0;
+                do {
+                    ++b;
+                    s.load(a, b, tt, false);
+                } while (s.items == 0);
+            }
+        }
+        set(a, tt);
+    }
+};
+
+template <int D, int QT>
+struct Shape {
+    static constexpr int HALVES = D / 64;
+    static constexpr int Q_BYTES = QT * kTile * D * 2;
+    static constexpr int STAGE = kTile * D * 2;                 // one K or V tile
+    static constexpr int STAGES = (232448 - 2048 - Q_BYTES) / STAGE;
+    static constexpr int OFF_KV = Q_BYTES;
+    static constexpr int OFF_BAR = OFF_KV + STAGES * STAGE;
+    static constexpr int SMEM = OFF_BAR + 1024 + 1024;          // barriers and state; alignment
+    static constexpr int THREADS = QT * 128 + 64;
+    // TMEM columns: S buffers of 128, then O
+    static constexpr int T_O = 2 * kTile;
+    static constexpr int O_COLS = D;
+    static_assert(SMEM <= 232448, "shared memory");
+    static_assert(T_O + QT * O_COLS <= 512, "TMEM");
+};
+
+struct Bars {
+    uint64_t full[16], empty[16];     // kv ring
+    uint64_t q_full, q_empty;
+    uint64_t s_full[2], p_full[2];
+    uint64_t o_full[2];
+    uint64_t pv_done;
+    Piece piece;
+    long long scan[16];
+    long long total;
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(Bars) <= 1024, "barrier block");
+
+// This CTA's piece: sequences' costs are summed in order, the CTA's start is located.
+__device__ __forceinline__ void find_piece(const AttnArgs& a, Bars* sh, int tt) {
+    const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, nw = nt >> 5;
+    // total
+    long long mine = 0;
+    for (int b = tid; b < a.B; b += nt) {
+        Seq s;
+        s.load(a, b, tt, blockIdx.x == 0);
+        mine += s.cost(a, s.items, tt) * a.n_kv;
+    }
+    const long long single = mine;                              // B <= threads: the sequence's own cost
 #pragma unroll
-    for (int i = 0; i < V; ++i) op[i] = f32_to_bf16_bits(l > 0.f ? o[i] * inv : 0.f);
-    if (a.lse && lane == 0) a.lse[static_cast<long>(t) * a.Hq + h] = l > 0.f ? m + logf(l) : -INFINITY;
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sh->scan[warp] = mine;
+    if (tid == 0) {
+        sh->piece = Piece{0, 0, 0, 0, 0};
+    }
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < nw; ++w) total += sh->scan[w];
+    long long pieces = (total + kMinPiece - 1) / kMinPiece;
+    if (pieces > gridDim.x) pieces = gridDim.x;
+    if (blockIdx.x >= pieces) {
+        __syncthreads();
+        return;
+    }
+    const long long from = total * blockIdx.x / pieces, to = total * (blockIdx.x + 1) / pieces;
+    long long base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += nt) {
+        __syncthreads();
+        const int b = b0 + tid;
+        Seq s;
+        long long u = 0;
+        if (b < a.B) {
+            s.load(a, b, tt, false);
+            u = a.B <= nt ? single : s.cost(a, s.items, tt) * a.n_kv;
+        }
+        long long inc = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) sh->scan[warp] = inc;
+        __syncthreads();
+        long long before = base;
+        for (int w = 0; w < warp; ++w) before += sh->scan[w];
+        const long long start = before + inc - u;
+        if (u > 0 && from >= start && from < start + u) {
+            const long long per_head = u / a.n_kv;
+            long long off = from - start;
+            Piece p;
+            p.b = b;
+            p.head = static_cast<int>(off / per_head);
+            off %= per_head;
+            int lo = 0, hi = s.items;                            // last item whose start is <= off
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (s.cost(a, mid, tt) <= off)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            p.item = lo;
+            p.skip = static_cast<int>(off - s.cost(a, lo, tt));
+            p.units = to - from;
+            sh->piece = p;
+        }
+        for (int w = 0; w < nw; ++w) base += sh->scan[w];
+    }
+    __syncthreads();
+}
+
+template <int D, int QT>
+__global__ void __launch_bounds__(Shape<D, QT>::THREADS, 1)
+paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+    using S = Shape<D, QT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Bars* sh = reinterpret_cast<Bars*>(sm + S::OFF_BAR);
+    volatile int* dead = &sh->abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int MMA_WARP = QT * 4, LOAD_WARP = QT * 4 + 1;
+    const int tt = QT * a.tile_tokens;                          // tokens per item
+    const int cta = blockIdx.x;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&sh->full[i], 1);
+            mbar_init(&sh->empty[i], 1);
+        }
+        mbar_init(&sh->q_full, 1);
+        mbar_init(&sh->q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_full[i], 4);
+            mbar_init(&sh->o_full[i], 1);
+        }
+        mbar_init(&sh->pv_done, 1);
+        sh->abort = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc(&sh->tmem, 512);
+        tmem_relinquish();
+    }
+    pdl_launch_dependents();
+    pdl_wait_prior();                                           // q, the cache and the lengths come from earlier kernels
+    find_piece(a, sh, tt);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem;
+    const Piece piece = sh->piece;
+
+    uint32_t q_loads = 0, issued = 0;                           // of the producer
+    if (warp == LOAD_WARP) {
+        // ---------------- TMA producer: a lane per (page of the tile, 64-value half)
+        const int page_rows = min(1 << a.page_shift, kTile);
+        const int pages_per_tile = kTile / page_rows;
+        const int units = pages_per_tile * S::HALVES;           // <= 16
+        const int my_page = lane / S::HALVES, my_half = lane % S::HALVES;
+        int stage = 0;
+        uint32_t phase = 0;
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            if (w.t0 >= w.t1) continue;
+            // q: rows of the item's tokens, `group` heads each
+            if (!warp_wait(&sh->q_empty, (q_loads & 1u) ^ 1u, a.err, dead)) break;
+            ++q_loads;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sh->q_full, QT * S::HALVES * a.tile_tokens * a.group * 128);
+                for (int t = 0; t < QT; ++t)
+                    for (int h = 0; h < S::HALVES; ++h)
+                        tma_load_3d(sm + (t * S::HALVES + h) * 16384, &maps.q, &sh->q_full, h * 64, w.head * a.group,
+                                    w.s.c0 + w.item * tt + t * a.tile_tokens);
+            }
+            const int* row = a.table + w.b * a.table_ld;
+            bool stop = false;
+            for (int j = w.t0; j < w.t1 && !stop; ++j) {
+                const int j0 = (w.first + j) * kTile;
+                // pages of this tile that hold a position somebody sees
+                const int pos = j0 + my_page * page_rows;
+                const bool mine = lane < units && pos + page_rows > w.lo && pos < w.hi;
+                int page = 0;
+                if (mine) {
+                    page = row[pos >> a.page_shift];
+                    if (page < 0 || page >= a.num_pages) {
+                        page = a.num_pages;                     // outside: the copy fills zeros
+                        atomicOr(a.err, DERR_PAGED);
+                    }
+                }
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * page_rows * 128;
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (!warp_wait(&sh->empty[stage], phase ^ 1u, a.err, dead)) {
+                        stop = true;
+                        break;
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&sh->full[stage], bytes);
+                    __syncwarp();
+                    if (mine)
+                        tma_load_4d(sm + S::OFF_KV + stage * S::STAGE + my_half * 16384 + my_page * page_rows * 128,
+                                    kv ? &maps.v : &maps.k, &sh->full[stage], my_half * 64,
+                                    pos & ((1 << a.page_shift) - 1), w.head, page);
+                    ++issued;
+                    if (++stage == S::STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (stop) break;
+        }
+    } else if (warp == MMA_WARP) {
+        // ---------------- MMA issuer (lane 0; the warp together clears unseen value rows)
+        constexpr uint32_t id_s = idesc_bf16(128, kTile, false, false);
+        constexpr uint32_t id_o = idesc_bf16(128, D, false, true);
+        int stage = 0, items = 0;
+        uint32_t phase = 0;
+        uint32_t done = 0;                                      // kv tiles finished so far
+        auto step = [&]() {
+            if (++stage == S::STAGES) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        };
+        auto mma_s = [&](int t, int buf, int st) {              // S[buf] = Q[t] K^T
+            if (lane == 0) {
+                const uint32_t q = smem_u32(sm) + t * (S::HALVES * 16384);
+                const uint32_t k = smem_u32(sm) + S::OFF_KV + st * S::STAGE;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t o = (kk >> 2) * 16384 + (kk & 3) * 32;
+                    umma_bf16_ss(tmem + buf * kTile, sdesc_sw128(q + o, 16, 1024), sdesc_sw128(k + o, 16, 1024), id_s, kk > 0);
+                }
+                umma_commit(&sh->s_full[buf]);
+            }
+        };
+        auto mma_o = [&](int t, int buf, int st, bool add) {    // O[t] (+)= P[buf] V
+            if (lane == 0) {
+                const uint32_t v = smem_u32(sm) + S::OFF_KV + st * S::STAGE;
+#pragma unroll
+                for (int kk = 0; kk < kTile / 16; ++kk)
+                    umma_bf16_ts(tmem + S::T_O + t * S::O_COLS, tmem + buf * kTile + kk * 8,
+                                 sdesc_sw128(v + kk * 2048, 16384, 1024), id_o, (add || kk > 0) ? 1u : 0u);
+            }
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (lane == 0) umma_commit(bar);
+        };
+        // zero the value rows that no row of the item sees: a weight of 0 times what the cache
+        // holds there (NaN included) has to be 0
+        auto clear_rows = [&](const Walk& w, int j, int st) {
+            const int j0 = (w.first + j) * kTile;
+            if (j0 >= w.lo && j0 + kTile <= w.hi) return;
+            uint8_t* v = sm + S::OFF_KV + st * S::STAGE;
+            const int below = max(0, w.lo - j0), above = min(kTile, w.hi - j0);
+            for (int c = lane; c < kTile * 8 * S::HALVES; c += 32) {
+                const int r = (c >> 3) & (kTile - 1);
+                if (r < below || r >= above) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+            __syncwarp();
+        };
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            if (w.t0 >= w.t1) continue;
+            if (!warp_wait(&sh->q_full, static_cast<uint32_t>(items & 1), a.err, dead)) break;
+            ++items;
+            const int n = w.t1 - w.t0;
+            if (!warp_wait(&sh->full[stage], phase, a.err, dead)) break;
+            tc_fence_after();
+            bool stop = false;
+            if constexpr (QT == 2) {
+                mma_s(0, 0, stage);
+                mma_s(1, 1, stage);
+                commit(&sh->empty[stage]);
+                if (n == 1) commit(&sh->q_empty);
+                step();
+                for (int j = 0; j < n; ++j) {
+                    const int vst = stage;
+                    if (!warp_wait(&sh->full[vst], phase, a.err, dead)) { stop = true; break; }
+                    step();
+                    clear_rows(w, w.t0 + j, vst);
+                    const bool more = j + 1 < n;
+                    const int kst = stage;
+                    const uint32_t kph = phase;
+                    if (more) step();
+                    for (int t = 0; t < 2; ++t) {
+                        if (!warp_wait(&sh->p_full[t], done & 1u, a.err, dead)) { stop = true; break; }
+                        tc_fence_after();
+                        mma_o(t, t, vst, j > 0);
+                        if (t == 1) commit(&sh->empty[vst]);
+                        if (more) {
+                            if (t == 0 && !warp_wait(&sh->full[kst], kph, a.err, dead)) { stop = true; break; }
+                            tc_fence_after();
+                            mma_s(t, t, kst);
+                            if (t == 1) {
+                                commit(&sh->empty[kst]);
+                                if (j + 2 == n) commit(&sh->q_empty);
+                            }
+                        } else {
+                            commit(&sh->o_full[t]);
+                        }
+                    }
+                    if (stop) break;
+                    ++done;
+                }
+            } else {
+                mma_s(0, done & 1u, stage);
+                commit(&sh->empty[stage]);
+                if (n == 1) commit(&sh->q_empty);
+                step();
+                for (int j = 0; j < n; ++j) {
+                    const int vst = stage;
+                    const uint32_t vph = phase;
+                    step();
+                    if (j + 1 < n) {
+                        if (!warp_wait(&sh->full[stage], phase, a.err, dead)) { stop = true; break; }
+                        tc_fence_after();
+                        mma_s(0, (done + 1) & 1u, stage);
+                        commit(&sh->empty[stage]);
+                        if (j + 2 == n) commit(&sh->q_empty);
+                        step();
+                    }
+                    if (!warp_wait(&sh->full[vst], vph, a.err, dead)) { stop = true; break; }
+                    clear_rows(w, w.t0 + j, vst);
+                    if (!warp_wait(&sh->p_full[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
+                    tc_fence_after();
+                    mma_o(0, done & 1u, vst, j > 0);
+                    commit(&sh->empty[vst]);
+                    commit(&sh->pv_done);
+                    if (j + 1 == n) commit(&sh->o_full[0]);
+                    ++done;
+                }
+            }
+            if (stop) break;
+        }
+    } else {
+        // ---------------- softmax and epilogue: a thread per row
+        const int t = QT == 2 ? warp >> 2 : 0;                  // row tile
+        const int row = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const int tok = row / a.group, g = row - tok * a.group; // token within the row tile, head within the group
+        const float c = a.scale * 1.4426950408889634f;
+        const uint32_t o_col = tmem + lanes + S::T_O + t * S::O_COLS;
+        uint32_t done = 0, items = 0;
+        if (tid == 0)
+            for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            const int rel = w.item * tt + t * a.tile_tokens + tok;      // token within the chunk
+            const bool real = tok < a.tile_tokens && rel < w.s.n;
+            const int first_tok = w.item * tt + t * a.tile_tokens;
+            const int last_tok = min(first_tok + a.tile_tokens, w.s.n) - 1;
+            const bool busy = __any_sync(0xffffffffu, real);
+            const long at = static_cast<long>(w.s.c0 + rel) * a.Hq + w.head * a.group + g;
+            if (w.t0 >= w.t1) {
+                if (w.count == 0 && real) {                             // sees nothing
+                    uint4* o = reinterpret_cast<uint4*>(a.out + at * D);
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
+                    if (a.lse) a.lse[at] = -INFINITY;
+                }
+                continue;
+            }
+            int lo, hi, dummy, hi_first, lo_last;
+            w.s.range(a, rel, rel, lo, hi);
+            w.s.range(a, first_tok, first_tok, dummy, hi_first);
+            w.s.range(a, last_tok, last_tok, lo_last, dummy);
+            float m = -INFINITY, l = 0.f;
+            bool stop = false;
+            for (int j = w.t0; j < w.t1; ++j) {
+                const int buf = QT == 2 ? t : static_cast<int>(done & 1u);
+                const uint32_t ph = QT == 2 ? (done & 1u) : ((done >> 1) & 1u);
+                if (!warp_wait(&sh->s_full[buf], ph, a.err, dead)) {
+                    stop = true;
+                    break;
+                }
+                tc_fence_after();
+                if (busy) {
+                    const uint32_t s_col = tmem + lanes + buf * kTile;
+                    const int j0 = (w.first + j) * kTile;
+                    float s[kTile];
+                    auto load_s = [&]() {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) tmem_ld32(s_col + q * 32, reinterpret_cast<float(&)[32]>(s[q * 32]));
+                        tmem_ld_wait();
+                        if (j0 + kTile > hi_first || j0 < lo_last) {
+#pragma unroll
+                            for (int i = 0; i < kTile; ++i)
+                                if (j0 + i < lo || j0 + i >= hi) s[i] = -INFINITY;
+                        }
+                    };
+                    load_s();
+                    float mx = s[0];
+#pragma unroll
+                    for (int i = 1; i < kTile; ++i) mx = fmaxf(mx, s[i]);
+                    const bool grow = real && (mx - m) * c > 8.f;        // m = -inf: true for any finite mx
+                    if (j == w.t0) {
+                        m = mx;
+                    } else if (__any_sync(0xffffffffu, grow)) {
+                        const float r = grow ? ex2_approx((m - mx) * c) : 1.f;
+                        if (grow) m = mx;
+                        l *= r;
+                        // O is at rest: with two row tiles S(j) was issued after P V(j - 1); with one, wait
+                        if constexpr (QT == 1) {
+                            if (!warp_wait(&sh->pv_done, (done - 1) & 1u, a.err, dead)) {
+                                stop = true;
+                                break;
+                            }
+                            tc_fence_after();
+                        }
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            float o[32];
+                            tmem_ld32(o_col + q * 32, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= r;
+                            tmem_st32(o_col + q * 32, o);
+                        }
+                        load_s();                                        // again: a row of S and one of O do not fit the registers
+                    }
+                    const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float p0 = ex2_approx(fmaf(s[q * 32 + 2 * i], c, -mc));
+                            const float p1 = ex2_approx(fmaf(s[q * 32 + 2 * i + 1], c, -mc));
+                            l += p0 + p1;
+                            p[i] = cvt_bf16x2(p0, p1);
+                        }
+                        tmem_st16(s_col + q * 16, p);
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[buf]);
+                ++done;
+            }
+            if (stop) break;
+            if (!warp_wait(&sh->o_full[t], items & 1u, a.err, dead)) break;
+            ++items;
+            tc_fence_after();
+            if (busy) {
+                const bool whole = w.t0 == 0 && w.t1 == w.count;
+                if (whole) {
+                    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        float o[32];
+                        tmem_ld32(o_col + q * 32, o);
+                        tmem_ld_wait();
+                        if (real) {
+                            uint4* p = reinterpret_cast<uint4*>(a.out + at * D + q * 32);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float x[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : o[i * 8 + e] * inv;
+                                p[i] = make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]), cvt_bf16x2(x[4], x[5]),
+                                                  cvt_bf16x2(x[6], x[7]));
+                            }
+                        }
+                    }
+                    if (a.lse && real) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+                } else {
+                    // slot 0: a part that does not hold the item's first tile; 1: the first part
+                    const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * (QT * 128) + t * 128 + row;
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        float o[32];
+                        tmem_ld32(o_col + q * 32, o);
+                        tmem_ld_wait();
+                        if (real) {
+                            float4* p = reinterpret_cast<float4*>(a.part_o + slot * D + q * 32);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) p[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }
+                    if (real) {
+                        a.part_ml[slot * 2] = m;
+                        a.part_ml[slot * 2 + 1] = l;
+                    }
+                }
+                tc_fence_before();
+            }
+            if (tid == 0 && !(w.t0 == 0 && w.t1 == w.count)) {
+                int* ps = a.part_state + cta * 8;
+                if (w.t0 == 0) {
+                    ps[1] = 1;
+                    ps[2] = w.s.c0 + w.item * tt;                        // first token
+                    ps[3] = min(tt, w.s.n - w.item * tt);                // tokens
+                    ps[4] = w.head;
+                } else {
+                    ps[0] = w.t1 == w.count ? 2 : 1;                     // 2: the item's last part
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (sh->abort && warp == LOAD_WARP) {                       // gave up: let the copies in flight land
+        for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+            mbar_wait(&sh->full[i % S::STAGES], (i / S::STAGES) & 1u, a.err);
+        if (q_loads > 0) mbar_wait(&sh->q_full, (q_loads - 1) & 1u, a.err);
+    }
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
+// began and did not finish, rows 32 y .. 32 y + 31; a warp per row.
+template <int D, int QT>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    pdl_wait_prior();
+    constexpr int ROWS = QT * 128, V = D / 32;
+    const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (__ldcg(a.part_state + x * 8 + 1) == 0) return;
+    const int tok0 = __ldcg(a.part_state + x * 8 + 2), toks = __ldcg(a.part_state + x * 8 + 3), head = __ldcg(a.part_state + x * 8 + 4);
+    int parts = 1;                                              // CTAs x, x + 1, ...
+    while (x + parts < ctas) {
+        const int st = __ldcg(a.part_state + (x + parts) * 8);
+        if (st == 0) break;
+        ++parts;
+        if (st == 2) break;
+    }
+    const float c = a.scale * 1.4426950408889634f;
+    for (int k = warp; k < 32; k += 8) {
+        const int row = blockIdx.y * 32 + k, r = row & 127;
+        const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
+        if (tl >= a.tile_tokens || tok >= toks) continue;
+        auto slot = [&](int p) { return (static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + row; };
+        float m = -INFINITY;
+        for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(a.part_ml + slot(p) * 2));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        float l = 0.f, o[V] = {};
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) {
+            const float mp = __ldcg(a.part_ml + slot(p) * 2), lp = __ldcg(a.part_ml + slot(p) * 2 + 1);
+            const float f = lp == 0.f ? 0.f : ex2_approx(mp * c - mc);
+            l += lp * f;
+            const float* src = a.part_o + slot(p) * D + lane * V;
+            if constexpr (V == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+                o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
+            } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                o[0] += v.x * f; o[1] += v.y * f;
+            }
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            w[i] = l == 0.f ? 0u : cvt_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * V);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) dst[i] = w[i];
+        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    }
+}
+
+size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
+size_t ml_bytes(int qt) { return static_cast<size_t>(kMaxCtas) * 2 * qt * 128 * 2 * sizeof(float); }
+size_t o_bytes(int qt, int D) { return static_cast<size_t>(kMaxCtas) * 2 * qt * 128 * D * sizeof(float); }
+
+// One row tile per item when the longest chunk's rows fit one, else two.
+int row_tiles(int max_q, int group) { return static_cast<long>(max_q) <= 128 / group ? 1 : 2; }
+
+template <int D, int QT>
+int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
+    using S = Shape<D, QT>;
+    const char* name = "gdn_paged_attn_fwd";
+    const cudaError_t attr = cudaFuncSetAttribute(paged_attn_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (attr != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr));
+    paged_attn_kernel<D, QT><<<kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
+    int rc = launch_status(name);
+    if (rc != GDN_OK) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(kMaxCtas, QT * 4);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, QT>, a, kMaxCtas);
+    if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
+    return launch_status(name);
 }
 
 }  // namespace
@@ -84,8 +783,13 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attn_rows_kernel(const Attn
 
 extern "C" size_t gdn_paged_attn_workspace_bytes(int B, int Ttot, int Hq, int n_kv, int head_dim, int max_q, int max_kv,
                                                  int window) {
-    (void)B, (void)Ttot, (void)Hq, (void)n_kv, (void)head_dim, (void)max_q, (void)max_kv, (void)window;
-    return 0;
+    using namespace gdn;
+    (void)window;
+    if (B < 1 || Ttot < 1 || Hq < 1 || n_kv < 1 || Hq % n_kv != 0 || Hq / n_kv > 64 || max_q < 0 || max_kv < 0 ||
+        (head_dim != 64 && head_dim != 128))
+        return 0;
+    const int qt = row_tiles(max_q, Hq / n_kv);
+    return state_bytes() + ml_bytes(qt) + o_bytes(qt, head_dim);
 }
 
 extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cache* cache, const int* cu_seqlens,
@@ -94,9 +798,8 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
                                   size_t workspace_bytes, void* stream) {
     using namespace gdn;
     const char* name = "gdn_paged_attn_fwd";
-    (void)workspace, (void)workspace_bytes;
-    AttnArgs a = {};
-    int st = check_cache(name, cache, &a.cache);
+    PagedView pv;
+    int st = check_cache(name, cache, &pv);
     if (st != GDN_OK) return st;
     if (!q || !cu_seqlens || !kv_lens || !out)
         return fail(GDN_ERR_NULL, "%s: q, cu_seqlens, kv_lens and out are required", name);
@@ -111,32 +814,60 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
                     cache->max_pages * cache->page_size);
     if (Ttot > 1 && q_ld < static_cast<long>(Hq) * D) return fail(GDN_ERR_SHAPE, "%s: q rows of %ld elements overlap", name, q_ld);
     if (window < 0 || (window > 0 && !causal)) return fail(GDN_ERR_ARG, "%s: a window needs causal, and must not be negative", name);
+    if (!(scale >= 0.f) || scale > 3e38f) return fail(GDN_ERR_ARG, "%s: scale must be positive (0: 1/sqrt(D)), got %g", name, scale);
     if (!aligned16(q) || !aligned16(out) || q_ld % 8 != 0)
         return fail(GDN_ERR_ALIGN, "%s: q, its rows and out must be 16-byte aligned", name);
+    const size_t need = gdn_paged_attn_workspace_bytes(B, Ttot, Hq, cache->n_kv, D, max_q, max_kv, window);
+    if (Ttot > 0 && (!workspace || workspace_bytes < need))
+        return fail(GDN_ERR_SHAPE, "%s: workspace of %zu bytes is smaller than %zu", name, workspace ? workspace_bytes : 0, need);
+    if (!aligned16(workspace)) return fail(GDN_ERR_ALIGN, "%s: workspace must be 16-byte aligned", name);
     if ((st = check_sm100()) != GDN_OK) return st;
     if (Ttot == 0) return GDN_OK;
-    a.q = static_cast<const uint16_t*>(q);
-    a.q_ld = q_ld;
+    AttnArgs a = {};
     a.out = static_cast<uint16_t*>(out);
     a.lse = lse;
     a.cu = cu_seqlens;
     a.kv_lens = kv_lens;
+    a.table = pv.table;
+    a.table_ld = pv.table_ld;
+    a.num_pages = pv.num_pages;
+    a.page_shift = pv.page_shift;
     a.B = B;
     a.T = Ttot;
     a.Hq = Hq;
-    a.group = Hq / cache->n_kv;
+    a.n_kv = pv.n_kv;
+    a.group = Hq / pv.n_kv;
+    a.tile_tokens = kTile / a.group;
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.causal = causal != 0;
     a.window = window;
     a.scale = scale == 0.f ? 1.f / sqrtf(static_cast<float>(D)) : scale;
     a.err = device_error_word();
+    const int qt = row_tiles(max_q, a.group);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.part_state = reinterpret_cast<int*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + state_bytes());
+    a.part_o = reinterpret_cast<float*>(ws + state_bytes() + ml_bytes(qt));
+
+    AttnMaps maps;
+    {
+        const uint64_t ld = static_cast<uint64_t>(Ttot > 1 ? q_ld : static_cast<long>(Hq) * D) * 2;
+        const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(Hq), static_cast<uint64_t>(Ttot)};
+        const uint64_t strides[2] = {static_cast<uint64_t>(D) * 2, ld};
+        const uint32_t box[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(a.tile_tokens)};
+        if ((st = make_map_bf16(&maps.q, q, 3, dims, strides, box, true)) != GDN_OK) return st;
+    }
+    {
+        const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(cache->page_size),
+                                  static_cast<uint64_t>(pv.n_kv), static_cast<uint64_t>(pv.num_pages)};
+        const uint64_t strides[3] = {static_cast<uint64_t>(pv.token_stride) * 2, static_cast<uint64_t>(pv.head_stride) * 2,
+                                     static_cast<uint64_t>(pv.page_stride) * 2};
+        const uint32_t box[4] = {64, static_cast<uint32_t>(cache->page_size < kTile ? cache->page_size : kTile), 1, 1};
+        if ((st = make_map_bf16(&maps.k, pv.k, 4, dims, strides, box, true)) != GDN_OK) return st;
+        if ((st = make_map_bf16(&maps.v, pv.v, 4, dims, strides, box, true)) != GDN_OK) return st;
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const long jobs = static_cast<long>(Ttot) * Hq;
-    const unsigned grid = static_cast<unsigned>((jobs + kWarps - 1) / kWarps);
-    if (D == 64)
-        paged_attn_rows_kernel<64><<<grid, 32 * kWarps, 0, s>>>(a);
-    else
-        paged_attn_rows_kernel<128><<<grid, 32 * kWarps, 0, s>>>(a);
-    return launch_status(name);
+    if (D == 64) return qt == 1 ? launch<64, 1>(maps, a, s) : launch<64, 2>(maps, a, s);
+    return qt == 1 ? launch<128, 1>(maps, a, s) : launch<128, 2>(maps, a, s);
 }
