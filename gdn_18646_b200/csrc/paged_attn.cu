@@ -27,7 +27,7 @@
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // With two row tiles the tensor core works for one while the softmax of the other runs;
 // with one row tile (at most 128 rows, the decode step) S is double buffered instead.
-#include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -39,6 +39,8 @@ namespace {
 constexpr int kTile = 128;            // positions per kv tile; rows per row tile
 constexpr int kMaxCtas = 148;         // pieces of the work line: one CTA per SM of a B200
 constexpr int kItemCost = 1;          // kv tiles that starting an item is worth
+constexpr int kEarly = 2;             // quarters of a tile's P after which P V starts
+constexpr int kPolyPairs = 1, kPolyOf = 4;   // pairs of weights in every so many that take the polynomial
 constexpr int kMinPiece = 4;          // shortest piece: splitting finer costs more to join
 
 struct AttnArgs {
@@ -63,23 +65,87 @@ struct alignas(64) AttnMaps {
     CUtensorMap q, k, v;
 };
 
-// sum over i in [0, n) of floor((a i + b) / m), for a, b >= 0 (the Euclid-like reduction)
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+// packed pairs of fp32 (one instruction for two values)
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x for two x <= 128 on the FMA pipe: x = n + f, |f| <= 1/2, n by adding 1.5 2^23; 2^f by
+// the degree-4 polynomial of least relative error (2.7e-6, found by linear programming
+// over Chebyshev nodes); n goes into the exponent bits.  x below -125 counts as -125.
+__device__ __forceinline__ void exp2_poly2(float& x0, float& x1) {
+    constexpr float kRound = 12582912.f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-125.f));
+    const uint64_t x = pack2(x0, x1);
+    const uint64_t t = add2(x, pack2(kRound, kRound));
+    const uint64_t n = add2(t, pack2(-kRound, -kRound));
+    const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
+    uint64_t r = fma2(f, pack2(9.570102207362652e-3f, 9.570102207362652e-3f), pack2(5.591785907745361e-2f, 5.591785907745361e-2f));
+    r = fma2(f, r, pack2(0.240247443318367f, 0.240247443318367f));
+    r = fma2(f, r, pack2(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(f, r, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float t0, t1, r0, r1;
+    unpack2(t, t0, t1);
+    unpack2(r, r0, r1);
+    x0 = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23));
+    x1 = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
+}
+
+// sum over i in [0, n) of floor((a i + b) / 128) for a <= 256 (the Euclid-like reduction);
+// after the first reduction every operand is small, so the divisions are 32-bit
+__device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
+    uint32_t m = kTile;
     long long s = 0;
     while (n > 0) {
-        s += (n - 1) * n / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const long long y = a * n + b;
+        const uint32_t qa = a / m, qb = b / m;
+        s += static_cast<long long>(n - 1) * n / 2 * qa + static_cast<long long>(n) * qb;
+        a -= qa * m;
+        b -= qb * m;
+        const uint32_t y = a * n + b;                           // a < 128, n <= 2^24
         if (y < m) break;
         n = y / m;
-        b = y % m;
-        const long long t = m;
+        b = y - n * m;
+        const uint32_t t = m;
         m = a;
         a = t;
     }
     return s;
 }
+
+// One lane of the warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+// lane 0's value: tells the compiler that it is the same in the whole warp, so that MMA
+// descriptors built from it stay in uniform registers
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// sdesc_sw128 from its low word
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+    return static_cast<uint64_t>(kDescHi) << 32 | lo;
+}
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3FFFFu) >> 4) | (lbo_bytes >> 4) << 16; }
 
 // A wait that all lanes of a warp leave alike, also when it gives up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* dead) {
@@ -116,17 +182,17 @@ struct Seq {
     __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
         if (q == 0) return 0;
         long long s = static_cast<long long>(q) * kItemCost;
-        const long long full = (kv + kTile - 1) / kTile;
-        if (!a.causal) return s + q * full;
-        const long long p = kv - n;
+        const int full = (kv + kTile - 1) / kTile;
+        if (!a.causal) return s + static_cast<long long>(q) * full;
+        const int p = kv - n;
         const int m = min(q, items - 1);
-        long long i0 = p + tt > 0 ? 0 : (-p) / tt;              // first item with p + (i + 1) tt > 0
-        if (i0 < m) s += floor_sum(m - i0, kTile, tt, p + (i0 + 1) * tt + kTile - 1);
+        const int i0 = p + tt > 0 ? 0 : (-p) / tt;              // first item with p + (i + 1) tt > 0
+        if (i0 < m) s += floor_sum(m - i0, tt, p + (i0 + 1) * tt + kTile - 1);
         if (q == items) s += full;
         if (a.window > 0) {
-            const long long w = p + 1 - a.window;               // lo of item i: max(0, w + i tt)
-            long long i1 = w >= 0 ? 0 : (-w + tt - 1) / tt;
-            if (i1 < q) s -= floor_sum(q - i1, kTile, tt, w + i1 * tt);
+            const int w = p + 1 - a.window;                     // lo of item i: max(0, w + i tt)
+            const int i1 = w >= 0 ? 0 : (-w + tt - 1) / tt;
+            if (i1 < q) s -= floor_sum(q - i1, tt, w + i1 * tt);
         }
         return s;
     }
@@ -134,6 +200,7 @@ struct Seq {
 
 // Where a CTA's piece of the work line starts, and its length.
 struct Piece {
+    Seq s;
     int b, head, item;
     int skip;                         // units of the first item that belong to earlier CTAs
     long long units;
@@ -153,7 +220,7 @@ struct Walk {
         skip = p.skip;
         left = p.units;
         if (left > 0) {
-            s.load(a, b, tt, false);
+            s = p.s;
             set(a, tt);
         }
     }
@@ -202,7 +269,7 @@ struct Shape {
 struct Bars {
     uint64_t full[16], empty[16];     // kv ring
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2];
+    uint64_t s_full[2], p_part[2], p_full[2];
     uint64_t o_full[2];
     uint64_t pv_done;
     Piece piece;
@@ -213,75 +280,75 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
-// This CTA's piece: sequences' costs are summed in order, the CTA's start is located.
+// This CTA's piece: a thread sums the costs of a sequence, a scan over the threads finds
+// the sequence in which the piece starts, and all threads together the item in it.
 __device__ __forceinline__ void find_piece(const AttnArgs& a, Bars* sh, int tt) {
     const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, nw = nt >> 5;
-    // total
-    long long mine = 0;
-    for (int b = tid; b < a.B; b += nt) {
-        Seq s;
-        s.load(a, b, tt, blockIdx.x == 0);
-        mine += s.cost(a, s.items, tt) * a.n_kv;
-    }
-    const long long single = mine;                              // B <= threads: the sequence's own cost
+    if (tid == 0) sh->piece.units = 0;
+    long long total = 0, from = 0, to = 0, base = 0;
+    const int chunks = (a.B + nt - 1) / nt;
+    // with more sequences than threads: a first pass for the total
+    for (int pass = chunks > 1 ? 0 : 1; pass < 2; ++pass) {
+        for (int k = 0; k < chunks; ++k) {
+            const int b = k * nt + tid;
+            Seq s;
+            long long u = 0;
+            if (b < a.B) {
+                s.load(a, b, tt, pass == 1 && blockIdx.x == 0);
+                u = s.cost(a, s.items, tt) * a.n_kv;
+            }
+            long long inc = u;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sh->scan[warp] = mine;
-    if (tid == 0) {
-        sh->piece = Piece{0, 0, 0, 0, 0};
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            __syncthreads();
+            if (lane == 31) sh->scan[warp] = inc;
+            __syncthreads();
+            long long start = base + inc - u, all = 0;
+            for (int w = 0; w < nw; ++w) {
+                const long long v = sh->scan[w];
+                if (w < warp) start += v;
+                all += v;
+            }
+            if (pass == 0) {
+                total += all;
+                continue;
+            }
+            if (chunks == 1) total = all;
+            if (k == 0) {
+                long long pieces = (total + kMinPiece - 1) / kMinPiece;
+                if (pieces > gridDim.x) pieces = gridDim.x;
+                if (blockIdx.x < pieces) {
+                    from = total * blockIdx.x / pieces;
+                    to = total * (blockIdx.x + 1) / pieces;
+                }
+            }
+            base += all;
+            if (from < to && from >= start && from < start + u) {
+                const long long per_head = u / a.n_kv, off = from - start;
+                Piece& p = sh->piece;
+                p.s = s;
+                p.b = b;
+                p.head = static_cast<int>(off / per_head);
+                p.item = 0;
+                p.skip = static_cast<int>(off % per_head);      // within the head, so far
+                p.units = to - from;
+            }
+        }
     }
     __syncthreads();
-    long long total = 0;
-    for (int w = 0; w < nw; ++w) total += sh->scan[w];
-    long long pieces = (total + kMinPiece - 1) / kMinPiece;
-    if (pieces > gridDim.x) pieces = gridDim.x;
-    if (blockIdx.x >= pieces) {
-        __syncthreads();
-        return;
-    }
-    const long long from = total * blockIdx.x / pieces, to = total * (blockIdx.x + 1) / pieces;
-    long long base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += nt) {
-        __syncthreads();
-        const int b = b0 + tid;
-        Seq s;
-        long long u = 0;
-        if (b < a.B) {
-            s.load(a, b, tt, false);
-            u = a.B <= nt ? single : s.cost(a, s.items, tt) * a.n_kv;
+    if (sh->piece.units == 0) return;
+    const Seq s = sh->piece.s;
+    const int off = sh->piece.skip;
+    __syncthreads();
+    for (int i = tid; i < s.items; i += nt) {
+        const long long c0 = s.cost(a, i, tt);
+        if (c0 <= off && off < s.cost(a, i + 1, tt)) {
+            sh->piece.item = i;
+            sh->piece.skip = off - static_cast<int>(c0);
         }
-        long long inc = u;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        if (lane == 31) sh->scan[warp] = inc;
-        __syncthreads();
-        long long before = base;
-        for (int w = 0; w < warp; ++w) before += sh->scan[w];
-        const long long start = before + inc - u;
-        if (u > 0 && from >= start && from < start + u) {
-            const long long per_head = u / a.n_kv;
-            long long off = from - start;
-            Piece p;
-            p.b = b;
-            p.head = static_cast<int>(off / per_head);
-            off %= per_head;
-            int lo = 0, hi = s.items;                            // last item whose start is <= off
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s.cost(a, mid, tt) <= off)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            p.item = lo;
-            p.skip = static_cast<int>(off - s.cost(a, lo, tt));
-            p.units = to - from;
-            sh->piece = p;
-        }
-        for (int w = 0; w < nw; ++w) base += sh->scan[w];
     }
     __syncthreads();
 }
@@ -308,6 +375,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         mbar_init(&sh->q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_part[i], 4);
             mbar_init(&sh->p_full[i], 4);
             mbar_init(&sh->o_full[i], 1);
         }
@@ -390,7 +458,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             if (stop) break;
         }
     } else if (warp == MMA_WARP) {
-        // ---------------- MMA issuer (lane 0; the warp together clears unseen value rows)
+        // ---------------- MMA issuer (one lane; the warp together clears unseen value rows)
         constexpr uint32_t id_s = idesc_bf16(128, kTile, false, false);
         constexpr uint32_t id_o = idesc_bf16(128, D, false, true);
         int stage = 0, items = 0;
@@ -402,29 +470,35 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 phase ^= 1u;
             }
         };
+        const uint32_t q_lo = desc_lo(smem_u32(sm), 16);
+        const uint32_t k_lo = desc_lo(smem_u32(sm) + S::OFF_KV, 16), v_lo = desc_lo(smem_u32(sm) + S::OFF_KV, 16384);
         auto mma_s = [&](int t, int buf, int st) {              // S[buf] = Q[t] K^T
-            if (lane == 0) {
-                const uint32_t q = smem_u32(sm) + t * (S::HALVES * 16384);
-                const uint32_t k = smem_u32(sm) + S::OFF_KV + st * S::STAGE;
+            const uint32_t q = uniform(q_lo + t * (S::HALVES * 1024)), k = uniform(k_lo + st * (S::STAGE >> 4));
+            const uint32_t d = uniform(tmem + buf * kTile);
+            if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t o = (kk >> 2) * 16384 + (kk & 3) * 32;
-                    umma_bf16_ss(tmem + buf * kTile, sdesc_sw128(q + o, 16, 1024), sdesc_sw128(k + o, 16, 1024), id_s, kk > 0);
+                    const uint32_t o = (kk >> 2) * 1024 + (kk & 3) * 2;
+                    umma_bf16_ss(d, desc_of(q + o), desc_of(k + o), id_s, kk > 0);
                 }
                 umma_commit(&sh->s_full[buf]);
             }
         };
-        auto mma_o = [&](int t, int buf, int st, bool add) {    // O[t] (+)= P[buf] V
-            if (lane == 0) {
-                const uint32_t v = smem_u32(sm) + S::OFF_KV + st * S::STAGE;
+        auto mma_o = [&](int t, int buf, int st, bool add, auto part) {   // O[t] (+)= P[buf] V, first or second part
+            const uint32_t v = uniform(v_lo + st * (S::STAGE >> 4));
+            const uint32_t d = uniform(tmem + S::T_O + t * S::O_COLS), pm = uniform(tmem + buf * kTile);
+            const uint32_t acc = uniform(add);
+            if (elect_one()) {
+                constexpr int k0 = decltype(part)::value == 0 ? 0 : kEarly * 2, k1 = decltype(part)::value == 0 ? kEarly * 2 : kTile / 16;
 #pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)
-                    umma_bf16_ts(tmem + S::T_O + t * S::O_COLS, tmem + buf * kTile + kk * 8,
-                                 sdesc_sw128(v + kk * 2048, 16384, 1024), id_o, (add || kk > 0) ? 1u : 0u);
+                for (int kk = k0; kk < k1; ++kk)
+                    umma_bf16_ts(d, pm + kk * 8, desc_of(v + kk * 128), id_o, kk > 0 ? 1u : acc);
             }
         };
+        constexpr std::integral_constant<int, 0> first_part{};
+        constexpr std::integral_constant<int, 1> second_part{};
         auto commit = [&](uint64_t* bar) {
-            if (lane == 0) umma_commit(bar);
+            if (elect_one()) umma_commit(bar);
         };
         // zero the value rows that no row of the item sees: a weight of 0 times what the cache
         // holds there (NaN included) has to be 0
@@ -465,9 +539,12 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     const uint32_t kph = phase;
                     if (more) step();
                     for (int t = 0; t < 2; ++t) {
+                        if (!warp_wait(&sh->p_part[t], done & 1u, a.err, dead)) { stop = true; break; }
+                        tc_fence_after();
+                        mma_o(t, t, vst, j > 0, first_part);
                         if (!warp_wait(&sh->p_full[t], done & 1u, a.err, dead)) { stop = true; break; }
                         tc_fence_after();
-                        mma_o(t, t, vst, j > 0);
+                        mma_o(t, t, vst, j > 0, second_part);
                         if (t == 1) commit(&sh->empty[vst]);
                         if (more) {
                             if (t == 0 && !warp_wait(&sh->full[kst], kph, a.err, dead)) { stop = true; break; }
@@ -503,9 +580,12 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     }
                     if (!warp_wait(&sh->full[vst], vph, a.err, dead)) { stop = true; break; }
                     clear_rows(w, w.t0 + j, vst);
+                    if (!warp_wait(&sh->p_part[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
+                    tc_fence_after();
+                    mma_o(0, done & 1u, vst, j > 0, first_part);
                     if (!warp_wait(&sh->p_full[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
                     tc_fence_after();
-                    mma_o(0, done & 1u, vst, j > 0);
+                    mma_o(0, done & 1u, vst, j > 0, second_part);
                     commit(&sh->empty[vst]);
                     commit(&sh->pv_done);
                     if (j + 1 == n) commit(&sh->o_full[0]);
@@ -559,21 +639,34 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 if (busy) {
                     const uint32_t s_col = tmem + lanes + buf * kTile;
                     const int j0 = (w.first + j) * kTile;
+                    const bool masked = j0 + kTile > hi_first || j0 < lo_last;
                     float s[kTile];
                     auto load_s = [&]() {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) tmem_ld32(s_col + q * 32, reinterpret_cast<float(&)[32]>(s[q * 32]));
                         tmem_ld_wait();
-                        if (j0 + kTile > hi_first || j0 < lo_last) {
+                        if (j0 + kTile > hi_first) {
+                            const int end = hi - j0;
 #pragma unroll
                             for (int i = 0; i < kTile; ++i)
-                                if (j0 + i < lo || j0 + i >= hi) s[i] = -INFINITY;
+                                if (i >= end) s[i] = -INFINITY;
+                        }
+                        if (j0 < lo_last) {
+                            const int begin = lo - j0;
+#pragma unroll
+                            for (int i = 0; i < kTile; ++i)
+                                if (i < begin) s[i] = -INFINITY;
                         }
                     };
                     load_s();
-                    float mx = s[0];
+                    // four chains, two values an instruction
+                    float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 1; i < kTile; ++i) mx = fmaxf(mx, s[i]);
+                    for (int i = 4; i < kTile; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mx4[e] = i + 4 + e < kTile ? max3(mx4[e], s[i + e], s[i + 4 + e]) : fmaxf(mx4[e], s[i + e]);
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                     const bool grow = real && (mx - m) * c > 8.f;        // m = -inf: true for any finite mx
                     if (j == w.t0) {
                         m = mx;
@@ -601,19 +694,45 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         load_s();                                        // again: a row of S and one of O do not fit the registers
                     }
                     const float mc = m == -INFINITY ? 0.f : m * c;
+                    const uint64_t c2 = pack2(c, c), mc2 = pack2(-mc, -mc);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    auto weights = [&](auto mixed) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t p[16];
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float p0 = ex2_approx(fmaf(s[q * 32 + 2 * i], c, -mc));
-                            const float p1 = ex2_approx(fmaf(s[q * 32 + 2 * i + 1], c, -mc));
-                            l += p0 + p1;
-                            p[i] = cvt_bf16x2(p0, p1);
+                            for (int i = 0; i < 16; ++i) {
+                                float x0, x1;
+                                unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), c2, mc2), x0, x1);
+                                if (decltype(mixed)::value && (i % kPolyOf) < kPolyPairs) {
+                                    exp2_poly2(x0, x1);
+                                } else {
+                                    x0 = ex2_approx(x0);
+                                    x1 = ex2_approx(x1);
+                                }
+                                sum[i & 3] = add2(sum[i & 3], pack2(x0, x1));
+                                p[i] = cvt_bf16x2(x0, x1);
+                            }
+                            tmem_st16(s_col + q * 16, p);
+                            if (q == kEarly - 1) {               // the first part of P V may start
+                                tmem_st_wait();
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&sh->p_part[buf]);
+                            }
                         }
-                        tmem_st16(s_col + q * 16, p);
-                    }
+                    };
+                    if (QT == 2 && !masked)
+                        weights(std::true_type{});
+                    else
+                        weights(std::false_type{});
+                    float l0, l1;
+                    unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+                    l += l0 + l1;
                     tmem_st_wait();
+                } else {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->p_part[buf]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -694,58 +813,85 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
 }
 
 // Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
-// began and did not finish, rows 32 y .. 32 y + 31; a warp per row.
+// began and did not finish, rows 32 y .. 32 y + 31; eight lanes per row.
 template <int D, int QT>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
     pdl_wait_prior();
-    constexpr int ROWS = QT * 128, V = D / 32;
+    constexpr int ROWS = QT * 128, V = D / 32;                  // V float4 per lane
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (__ldcg(a.part_state + x * 8 + 1) == 0) return;
-    const int tok0 = __ldcg(a.part_state + x * 8 + 2), toks = __ldcg(a.part_state + x * 8 + 3), head = __ldcg(a.part_state + x * 8 + 4);
-    int parts = 1;                                              // CTAs x, x + 1, ...
-    while (x + parts < ctas) {
-        const int st = __ldcg(a.part_state + (x + parts) * 8);
-        if (st == 0) break;
-        ++parts;
-        if (st == 2) break;
+    // the states of this CTA and of the 31 after it in one go
+    const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
+    const int head = __ldcg(a.part_state + x * 8 + 4);
+    int st = x + 1 + lane < ctas ? __ldcg(a.part_state + (x + 1 + lane) * 8) : 0;
+    if (mine.y == 0) return;
+    const int tok0 = mine.z, toks = mine.w;
+    int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
+    for (int at = x + 1;;) {
+        const uint32_t end = __ballot_sync(0xffffffffu, st != 1);
+        if (end) {
+            const int k = __ffs(end) - 1;
+            parts += k + (__shfl_sync(0xffffffffu, st, k) == 2 ? 1 : 0);
+            break;
+        }
+        parts += 32;
+        at += 32;
+        st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
     }
     const float c = a.scale * 1.4426950408889634f;
-    for (int k = warp; k < 32; k += 8) {
-        const int row = blockIdx.y * 32 + k, r = row & 127;
-        const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
-        if (tl >= a.tile_tokens || tok >= toks) continue;
-        auto slot = [&](int p) { return (static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + row; };
-        float m = -INFINITY;
-        for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(a.part_ml + slot(p) * 2));
+    const int sub = lane >> 3, l8 = lane & 7;
+    const int row = blockIdx.y * 32 + warp * 4 + sub, r = row & 127;
+    const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
+    const bool real = tl < a.tile_tokens && tok < toks;
+    if (!__any_sync(0xffffffffu, real)) return;
+    auto slot = [&](int p) { return (static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + row; };
+    // eight parts at a time, a lane each for m and l; then their rows, weighted
+    float m = -INFINITY, l = 0.f;
+    float4 o[V];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        float l = 0.f, o[V] = {};
+    for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < parts; p0 += 8) {
+        float mp = -INFINITY, lp = 0.f;
+        if (real && p0 + l8 < parts) {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot(p0 + l8) * 2));
+            mp = v.x;
+            lp = v.y;
+        }
+        float mx = lp == 0.f ? -INFINITY : mp;
+#pragma unroll
+        for (int s = 4; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+        const float mn = fmaxf(m, mx), mc = mn == -INFINITY ? 0.f : mn * c;
+        const float keep = ex2_approx(m * c - mc);              // m = -inf: 0
+        const float f = lp == 0.f ? 0.f : ex2_approx(mp * c - mc);
+        float add = lp * f;
+#pragma unroll
+        for (int s = 4; s > 0; s >>= 1) add += __shfl_xor_sync(0xffffffffu, add, s);
+        l = l * keep + add;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
+        }
 #pragma unroll 4
-        for (int p = 0; p < parts; ++p) {
-            const float mp = __ldcg(a.part_ml + slot(p) * 2), lp = __ldcg(a.part_ml + slot(p) * 2 + 1);
-            const float f = lp == 0.f ? 0.f : ex2_approx(mp * c - mc);
-            l += lp * f;
-            const float* src = a.part_o + slot(p) * D + lane * V;
-            if constexpr (V == 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-                o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
-            } else {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                o[0] += v.x * f; o[1] += v.y * f;
+        for (int p = 0; p < 8; ++p) {
+            const float w = __shfl_sync(0xffffffffu, f, p, 8);
+            if (!real || p0 + p >= parts) continue;
+            const float4* src = reinterpret_cast<const float4*>(a.part_o + slot(p0 + p) * D) + l8;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float4 v = __ldcg(src + 8 * i);
+                o[i].x += v.x * w; o[i].y += v.y * w; o[i].z += v.z * w; o[i].w += v.w * w;
             }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
-        uint32_t w[V / 2];
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i)
-            w[i] = l == 0.f ? 0u : cvt_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * V);
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) dst[i] = w[i];
-        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
     }
+    if (!real) return;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
+    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + l8;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        dst[8 * i] = l == 0.f ? make_uint2(0u, 0u)
+                              : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
+    if (a.lse && l8 == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
 size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
