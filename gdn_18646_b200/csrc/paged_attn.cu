@@ -38,9 +38,10 @@ namespace {
 
 constexpr int kTile = 128;            // positions per kv tile; rows per row tile
 constexpr int kMaxCtas = 148;         // pieces of the work line: one CTA per SM of a B200
-constexpr int kItemCost = 1;          // kv tiles that starting an item is worth
-constexpr int kEarly = 2;             // quarters of a tile's P after which P V starts
-constexpr int kPolyPairs = 1, kPolyOf = 4;   // pairs of weights in every so many that take the polynomial
+// kv tiles that starting and ending an item is worth, beside the tiles themselves
+__host__ __device__ constexpr int item_cost(int qt) { return qt == 2 ? 2 : 1; }
+constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
+constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
 constexpr int kMinPiece = 4;          // shortest piece: splitting finer costs more to join
 
 struct AttnArgs {
@@ -55,10 +56,11 @@ struct AttnArgs {
     int tile_tokens;                  // floor(128 / group)
     int max_q, max_kv, causal, window;
     float scale;
+    int item_cost;
     unsigned int* err;
     int* part_state;                  // [ctas][8]: what a CTA left unfinished
     float* part_ml;                   // [ctas][2][QT 128][2]: m, l
-    float* part_o;                    // [ctas][2][QT 128][D]
+    float* part_o;                    // [ctas][2][D / 4][QT 128][4]
 };
 
 struct alignas(64) AttnMaps {
@@ -181,7 +183,7 @@ struct Seq {
     // cost of the items before `q` of one kv head
     __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
         if (q == 0) return 0;
-        long long s = static_cast<long long>(q) * kItemCost;
+        long long s = static_cast<long long>(q) * a.item_cost;
         const int full = (kv + kTile - 1) / kTile;
         if (!a.causal) return s + static_cast<long long>(q) * full;
         const int p = kv - n;
@@ -227,12 +229,12 @@ struct Walk {
     __device__ __forceinline__ bool valid() const { return left > 0; }
     __device__ __forceinline__ void set(const AttnArgs& a, int tt) {
         s.tiles(a, item, tt, first, count, lo, hi);
-        const long long end = min(static_cast<long long>(count + kItemCost), skip + left);
-        t0 = max(skip - kItemCost, 0);
-        t1 = max(static_cast<int>(end) - kItemCost, 0);
+        const long long end = min(static_cast<long long>(count + a.item_cost), skip + left);
+        t0 = max(skip - a.item_cost, 0);
+        t1 = max(static_cast<int>(end) - a.item_cost, 0);
     }
     __device__ __forceinline__ void next(const AttnArgs& a, int tt) {
-        left -= count + kItemCost - skip;
+        left -= count + a.item_cost - skip;
         skip = 0;
         if (left <= 0) return;
         if (++item == s.items) {
@@ -254,9 +256,12 @@ struct Shape {
     static constexpr int HALVES = D / 64;
     static constexpr int Q_BYTES = QT * kTile * D * 2;
     static constexpr int STAGE = kTile * D * 2;                 // one K or V tile
-    static constexpr int STAGES = (232448 - 2048 - Q_BYTES) / STAGE;
+    static constexpr int OUT_BYTES = QT * 4 * 4096;             // 32 rows x 64 values per softmax warp
+    static constexpr int STAGES_FIT = (232448 - 2048 - Q_BYTES - OUT_BYTES) / STAGE;
+    static constexpr int STAGES = STAGES_FIT < 10 ? STAGES_FIT : 10;
     static constexpr int OFF_KV = Q_BYTES;
-    static constexpr int OFF_BAR = OFF_KV + STAGES * STAGE;
+    static constexpr int OFF_OUT = OFF_KV + STAGES * STAGE;
+    static constexpr int OFF_BAR = OFF_OUT + OUT_BYTES;
     static constexpr int SMEM = OFF_BAR + 1024 + 1024;          // barriers and state; alignment
     static constexpr int THREADS = QT * 128 + 64;
     // TMEM columns: S buffers of 128, then O
@@ -280,68 +285,66 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
-// This CTA's piece: a thread sums the costs of a sequence, a scan over the threads finds
-// the sequence in which the piece starts, and all threads together the item in it.
+// This CTA's piece: a thread sums the costs of its share of the sequences, a scan over the
+// threads finds the sequence in which the piece starts, and all threads together the item in it.
 __device__ __forceinline__ void find_piece(const AttnArgs& a, Bars* sh, int tt) {
     const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, nw = nt >> 5;
     if (tid == 0) sh->piece.units = 0;
-    long long total = 0, from = 0, to = 0, base = 0;
-    const int chunks = (a.B + nt - 1) / nt;
-    // with more sequences than threads: a first pass for the total
-    for (int pass = chunks > 1 ? 0 : 1; pass < 2; ++pass) {
-        for (int k = 0; k < chunks; ++k) {
-            const int b = k * nt + tid;
-            Seq s;
-            long long u = 0;
-            if (b < a.B) {
-                s.load(a, b, tt, pass == 1 && blockIdx.x == 0);
-                u = s.cost(a, s.items, tt) * a.n_kv;
-            }
-            long long inc = u;
+    const int each = (a.B + nt - 1) / nt, b0 = tid * each, b1 = min(b0 + each, a.B);
+    long long mine = 0, u = 0;
+    Seq s = {};
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) {
+        s.load(a, b, tt, blockIdx.x == 0);
+        u = s.cost(a, s.items, tt);
+        mine += u * a.n_kv;
+    }
+    long long inc = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
-            }
-            __syncthreads();
-            if (lane == 31) sh->scan[warp] = inc;
-            __syncthreads();
-            long long start = base + inc - u, all = 0;
-            for (int w = 0; w < nw; ++w) {
-                const long long v = sh->scan[w];
-                if (w < warp) start += v;
-                all += v;
-            }
-            if (pass == 0) {
-                total += all;
-                continue;
-            }
-            if (chunks == 1) total = all;
-            if (k == 0) {
-                long long pieces = (total + kMinPiece - 1) / kMinPiece;
-                if (pieces > gridDim.x) pieces = gridDim.x;
-                if (blockIdx.x < pieces) {
-                    from = total * blockIdx.x / pieces;
-                    to = total * (blockIdx.x + 1) / pieces;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) sh->scan[warp] = inc;
+    __syncthreads();
+    long long start = inc - mine, total = 0;
+    for (int w = 0; w < nw; ++w) {
+        const long long v = sh->scan[w];
+        if (w < warp) start += v;
+        total += v;
+    }
+    const long long most = (total + kMinPiece - 1) / kMinPiece;
+    const int pieces = most < gridDim.x ? static_cast<int>(most) : gridDim.x;
+    if (blockIdx.x < pieces) {
+        // total x / pieces without a wide product
+        const long long q = total / pieces;
+        const int r = static_cast<int>(total - q * pieces), x = blockIdx.x;
+        const long long from = q * x + r * x / pieces, to = q * (x + 1) + r * (x + 1) / pieces;
+        if (from >= start && from < start + mine) {
+            int b = b0;
+            if (each > 1) {
+                for (;; ++b) {
+                    s.load(a, b, tt, false);
+                    u = s.cost(a, s.items, tt);
+                    if (from < start + u * a.n_kv) break;
+                    start += u * a.n_kv;
                 }
             }
-            base += all;
-            if (from < to && from >= start && from < start + u) {
-                const long long per_head = u / a.n_kv, off = from - start;
-                Piece& p = sh->piece;
-                p.s = s;
-                p.b = b;
-                p.head = static_cast<int>(off / per_head);
-                p.item = 0;
-                p.skip = static_cast<int>(off % per_head);      // within the head, so far
-                p.units = to - from;
-            }
+            const long long off = from - start;
+            Piece& p = sh->piece;
+            p.s = s;
+            p.b = b;
+            p.head = static_cast<int>(off / u);
+            p.item = 0;
+            p.skip = static_cast<int>(off - p.head * u);        // within the head, so far
+            p.units = to - from;
         }
     }
     __syncthreads();
     if (sh->piece.units == 0) return;
-    const Seq s = sh->piece.s;
+    s = sh->piece.s;
     const int off = sh->piece.skip;
+    if (s.items == 1) return;
     __syncthreads();
     for (int i = tid; i < s.items; i += nt) {
         const long long c0 = s.cost(a, i, tt);
@@ -746,38 +749,53 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             if (busy) {
                 const bool whole = w.t0 == 0 && w.t1 == w.count;
                 if (whole) {
+                    // through shared memory, so that a store instruction writes whole lines: 64
+                    // values of the warp's 32 rows at a time, 16-byte pieces swizzled by the row
                     const float inv = l > 0.f ? 1.f / l : 0.f;
+                    const long mine = real ? at : -1;
+                    uint8_t* buf = sm + S::OFF_OUT + warp * 4096;
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {
-                        float o[32];
-                        tmem_ld32(o_col + q * 32, o);
-                        tmem_ld_wait();
-                        if (real) {
-                            uint4* p = reinterpret_cast<uint4*>(a.out + at * D + q * 32);
+                    for (int hf = 0; hf < S::HALVES; ++hf) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            float o[32];
+                            tmem_ld32(o_col + hf * 64 + q * 32, o);
+                            tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 float x[8];
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : o[i * 8 + e] * inv;
-                                p[i] = make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]), cvt_bf16x2(x[4], x[5]),
-                                                  cvt_bf16x2(x[6], x[7]));
+                                *reinterpret_cast<uint4*>(buf + sw128_chunk(lane, q * 4 + i)) =
+                                    make_uint4(cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]), cvt_bf16x2(x[4], x[5]),
+                                               cvt_bf16x2(x[6], x[7]));
                             }
                         }
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = i * 4 + (lane >> 3);
+                            const long to = __shfl_sync(0xffffffffu, mine, r);
+                            if (to >= 0)
+                                reinterpret_cast<uint4*>(a.out + to * D + hf * 64)[lane & 7] =
+                                    *reinterpret_cast<const uint4*>(buf + sw128_chunk(r, lane & 7));
+                        }
+                        __syncwarp();
                     }
                     if (a.lse && real) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
                 } else {
                     // slot 0: a part that does not hold the item's first tile; 1: the first part
-                    const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * (QT * 128) + t * 128 + row;
+                    const long part = static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0), slot = part * (QT * 128) + t * 128 + row;
+                    float4* dst = reinterpret_cast<float4*>(a.part_o) + part * (D / 4) * (QT * 128) + t * 128 + row;
 #pragma unroll
                     for (int q = 0; q < D / 32; ++q) {
                         float o[32];
                         tmem_ld32(o_col + q * 32, o);
                         tmem_ld_wait();
-                        if (real) {
-                            float4* p = reinterpret_cast<float4*>(a.part_o + slot * D + q * 32);
+                        if (real)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) p[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                        }
+                            for (int i = 0; i < 8; ++i)
+                                dst[(q * 8 + i) * (QT * 128)] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                     if (real) {
                         a.part_ml[slot * 2] = m;
@@ -813,11 +831,14 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
 }
 
 // Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
-// began and did not finish, rows 32 y .. 32 y + 31; eight lanes per row.
+// began and did not finish, rows 32 y .. 32 y + 31.  Lanes go along rows, as the parts lie
+// in memory; a warp takes D / 8 columns.
+constexpr int kJoinParts = 160;       // parts of an item: at most one per CTA
 template <int D, int QT>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    __shared__ float weight[kJoinParts][32], sums[kJoinParts][32], row_m[8][32];
     pdl_wait_prior();
-    constexpr int ROWS = QT * 128, V = D / 32;                  // V float4 per lane
+    constexpr int ROWS = QT * 128, V = D / 32;                  // V float4 per thread
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the states of this CTA and of the 31 after it in one go
     const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
@@ -825,6 +846,10 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     int st = x + 1 + lane < ctas ? __ldcg(a.part_state + (x + 1 + lane) * 8) : 0;
     if (mine.y == 0) return;
     const int tok0 = mine.z, toks = mine.w;
+    const int row = blockIdx.y * 32 + lane, r = row & 127;
+    const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
+    const bool real = tl < a.tile_tokens && tok < toks;
+    if (!__any_sync(0xffffffffu, real)) return;                 // the same in every warp
     int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
     for (int at = x + 1;;) {
         const uint32_t end = __ballot_sync(0xffffffffu, st != 1);
@@ -838,47 +863,36 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
         st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
     }
     const float c = a.scale * 1.4426950408889634f;
-    const int sub = lane >> 3, l8 = lane & 7;
-    const int row = blockIdx.y * 32 + warp * 4 + sub, r = row & 127;
-    const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
-    const bool real = tl < a.tile_tokens && tok < toks;
-    if (!__any_sync(0xffffffffu, real)) return;
-    auto slot = [&](int p) { return (static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + row; };
-    // eight parts at a time, a lane each for m and l; then their rows, weighted
-    float m = -INFINITY, l = 0.f;
+    auto part = [&](int p) { return static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0); };
+    // m and l of every part (a warp takes every eighth), then the weights from the largest m
+    float m = -INFINITY;
+    for (int p = warp; p < parts; p += 8) {
+        const float2 v = real ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + part(p) * ROWS + row) : make_float2(0.f, 0.f);
+        const float mp = v.y == 0.f ? -INFINITY : v.x;
+        weight[p][lane] = mp;
+        sums[p][lane] = v.y;
+        m = fmaxf(m, mp);
+    }
+    row_m[warp][lane] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, row_m[i][lane]);
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    for (int p = warp; p < parts; p += 8) weight[p][lane] = ex2_approx(weight[p][lane] * c - mc);
+    __syncthreads();
+    float l = 0.f;                                              // in the order of the parts, in every warp alike
+    for (int p = 0; p < parts; ++p) l += weight[p][lane] * sums[p][lane];
     float4 o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < parts; p0 += 8) {
-        float mp = -INFINITY, lp = 0.f;
-        if (real && p0 + l8 < parts) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot(p0 + l8) * 2));
-            mp = v.x;
-            lp = v.y;
-        }
-        float mx = lp == 0.f ? -INFINITY : mp;
-#pragma unroll
-        for (int s = 4; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-        const float mn = fmaxf(m, mx), mc = mn == -INFINITY ? 0.f : mn * c;
-        const float keep = ex2_approx(m * c - mc);              // m = -inf: 0
-        const float f = lp == 0.f ? 0.f : ex2_approx(mp * c - mc);
-        float add = lp * f;
-#pragma unroll
-        for (int s = 4; s > 0; s >>= 1) add += __shfl_xor_sync(0xffffffffu, add, s);
-        l = l * keep + add;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
-        }
-#pragma unroll 4
-        for (int p = 0; p < 8; ++p) {
-            const float w = __shfl_sync(0xffffffffu, f, p, 8);
-            if (!real || p0 + p >= parts) continue;
-            const float4* src = reinterpret_cast<const float4*>(a.part_o + slot(p0 + p) * D) + l8;
+    if (real) {
+#pragma unroll 6
+        for (int p = 0; p < parts; ++p) {
+            const float w = weight[p][lane];
+            const float4* src = reinterpret_cast<const float4*>(a.part_o) + (part(p) * (D / 4) + warp * V) * ROWS + row;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float4 v = __ldcg(src + 8 * i);
+                const float4 v = __ldcg(src + i * ROWS);
                 o[i].x += v.x * w; o[i].y += v.y * w; o[i].z += v.z * w; o[i].w += v.w * w;
             }
         }
@@ -886,12 +900,12 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     if (!real) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
-    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + l8;
+    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + warp * V;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        dst[8 * i] = l == 0.f ? make_uint2(0u, 0u)
-                              : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
-    if (a.lse && l8 == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+        dst[i] = l == 0.f ? make_uint2(0u, 0u)
+                          : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
+    if (a.lse && warp == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
 size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
@@ -991,6 +1005,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.scale = scale == 0.f ? 1.f / sqrtf(static_cast<float>(D)) : scale;
     a.err = device_error_word();
     const int qt = row_tiles(max_q, a.group);
+    a.item_cost = item_cost(qt);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_state = reinterpret_cast<int*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + state_bytes());
