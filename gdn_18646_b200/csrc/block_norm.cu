@@ -33,6 +33,7 @@ struct BlockNormArgs {
     uint16_t* x;                      // backward: dy
     const void* dh_out;
     const uint16_t* dx;
+    unsigned int* err;                // backward
     float alpha, eps;
     int R, D;
     int rows_per_gate;                // rows that share a gate row (R: one gate row for all)
@@ -46,24 +47,33 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&f)[8]) {
         f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void load8_bf16(const uint16_t* p, float (&f)[8]) {
-    unpack8(__ldcg(reinterpret_cast<const uint4*>(p)), f);
-}
-__device__ __forceinline__ void store8_bf16(uint16_t* p, const float (&f)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                              pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-}
+// Eight consecutive values of a row as loaded: bf16 stays packed until it is used.
 template <bool F32>
-__device__ __forceinline__ void load8(const void* base, long at, float (&f)[8]) {
-    if constexpr (F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-        const float4 a = __ldcg(p), b = __ldcg(p + 1);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-        load8_bf16(static_cast<const uint16_t*>(base) + at, f);
+struct Piece {
+    uint4 w[F32 ? 2 : 1];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-}
+    __device__ __forceinline__ void load(const void* base, long at) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at * (F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = __ldcg(p + i);
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f[4 * i] = __uint_as_float(w[i].x);
+                f[4 * i + 1] = __uint_as_float(w[i].y);
+                f[4 * i + 2] = __uint_as_float(w[i].z);
+                f[4 * i + 3] = __uint_as_float(w[i].w);
+            }
+        } else {
+            unpack8(w[0], f);
+        }
+    }
+};
 template <bool F32>
 __device__ __forceinline__ void store8(void* base, long at, const float (&f)[8]) {
     if constexpr (F32) {
@@ -71,90 +81,109 @@ __device__ __forceinline__ void store8(void* base, long at, const float (&f)[8])
         p[0] = make_float4(f[0], f[1], f[2], f[3]);
         p[1] = make_float4(f[4], f[5], f[6], f[7]);
     } else {
-        store8_bf16(static_cast<uint16_t*>(base) + at, f);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) =
+            make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
     }
 }
+// a weight's eight values, 1 without it
+__device__ __forceinline__ void weight8(const uint16_t* p, long at, bool on, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 1.f;
+    if (on && p) unpack8(__ldg(reinterpret_cast<const uint4*>(p + at)), f);
+}
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Sum over the row's threads: one warp, or the whole CTA through `red` ([2][32] floats,
+// used in turn so that one barrier per sum is enough).
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* red, int& turn) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (!WARP) {
+        float* mine = red + turn * 32;
+        turn ^= 1;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+        if (lane == 0) mine[warp] = v;
+        __syncthreads();
+        v = lane < nw ? mine[lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
     return v;
 }
 
-// Sum of N values over the row's threads: one warp, or the whole CTA through `red`
-// ([2][N][32] floats, used in turn so that one barrier per sum is enough).
-template <int N, bool WARP>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& turn) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-    if constexpr (!WARP) {
-        float* mine = red + turn * (N * 32);
-        turn ^= 1;
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-        if (lane == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) mine[i * 32 + warp] = v[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < nw ? mine[i * 32 + lane] : 0.f);
-    }
-}
-
+// A CTA walks over rows with the weights in registers (a gate row too, where all rows
+// share it) and the next row's loads in flight while it works on one.
 template <bool F32, bool WARP, int NT>
-__global__ void __launch_bounds__(NT) block_norm_fwd_kernel(const BlockNormArgs a) {
+__global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) block_norm_fwd_kernel(const BlockNormArgs a) {
     __shared__ float red[2][32];
     pdl_launch_dependents();
-    pdl_wait_prior();                          // y and h come from earlier kernels
-    const int piece = WARP ? (threadIdx.x & 31) : threadIdx.x;
-    const bool on = piece * 8 < a.D;
+    const int piece = WARP ? (threadIdx.x & 31) : threadIdx.x, col = piece * 8;
+    const bool on = col < a.D;
     const long row0 = WARP ? static_cast<long>(blockIdx.x) * kNarrowRows + (threadIdx.x >> 5) : blockIdx.x;
     const long step = WARP ? static_cast<long>(gridDim.x) * kNarrowRows : gridDim.x;
     const float inv_d = 1.f / static_cast<float>(a.D);
+    const bool one_gate = a.gate && a.rows_per_gate == a.R, row_gate = a.gate && !one_gate;
+    float wp[8], wq[8];                        // gamma_post (times the gate that all rows share), gamma_pre
+    weight8(a.gamma_post, col, on, wp);
+    weight8(a.gamma_pre, col, on, wq);
+    if (one_gate && on) {
+        float g[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(a.gate + col)), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wp[i] *= g[i];
+    }
+    pdl_wait_prior();                          // y and h come from earlier kernels
+    Piece<false> ny, ng;
+    Piece<F32> nh;
+    ny.zero();
+    nh.zero();
+    ng.zero();
+    auto fetch = [&](long r) {
+        if (!on || r >= a.R) return;
+        ny.load(a.y, r * a.D + col);
+        nh.load(a.h, r * a.D + col);
+        if (row_gate) ng.load(a.gate, (r / a.rows_per_gate) * a.D + col);
+    };
+    fetch(row0);
     int turn = 0;
     for (long r = row0; r < a.R; r += step) {
-        const long at = r * a.D + piece * 8;
-        float u[8] = {}, h[8] = {}, w[8];
-        if (on) {
-            load8_bf16(a.y + at, u);
-            load8<F32>(a.h, at, h);
-        }
+        const long at = r * a.D + col;
+        float u[8], h[8], g[8];
+        ny.get(u);
+        nh.get(h);
+        ng.get(g);
+        fetch(r + step);
+        float r1 = 1.f;
         if (a.gamma_post) {
-            float ss[1] = {0.f};
+            float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss[0] += u[i] * u[i];
-            row_sum<1, WARP>(ss, &red[0][0], turn);
-            const float r1 = rsqrtf(ss[0] * inv_d + a.eps);
-            if (on) {
-                unpack8(__ldg(reinterpret_cast<const uint4*>(a.gamma_post + piece * 8)), w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] *= r1 * w[i];
-            }
+            for (int i = 0; i < 8; ++i) ss += u[i] * u[i];
+            r1 = rsqrtf(row_sum<WARP>(ss, &red[0][0], turn) * inv_d + a.eps);
         }
-        if (a.gate && on) {
-            load8_bf16(a.gate + (r / a.rows_per_gate) * a.D + piece * 8, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] *= w[i];
-        }
+        for (int i = 0; i < 8; ++i) u[i] *= r1 * wp[i];
+        if (row_gate)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] *= g[i];
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] = fmaf(a.alpha, h[i], u[i]);
         if (on) store8<F32>(a.h_out, at, h);
         if (a.gamma_pre) {
-            float ss[1] = {0.f};
+            float ss = 0.f;
+            if (on)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss[0] += h[i] * h[i];
-            row_sum<1, WARP>(ss, &red[0][0], turn);
-            const float r2 = rsqrtf(ss[0] * inv_d + a.eps);
+                for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
+            const float r2 = rsqrtf(row_sum<WARP>(ss, &red[0][0], turn) * inv_d + a.eps);
             if (on) {
-                unpack8(__ldg(reinterpret_cast<const uint4*>(a.gamma_pre + piece * 8)), w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] *= r2 * w[i];
-                store8_bf16(a.x + at, h);
+                for (int i = 0; i < 8; ++i) h[i] *= r2 * wq[i];
+                store8<false>(a.x, at, h);
             }
         }
     }
 }
 
-// The rows a backward work item covers: one of `per_gate` parts of one gate row's rows,
+// The rows a backward work item covers: one of `parts` parts of one gate row's rows,
 // so the column sums of an item belong to one gate row.
 struct BwdPlan {
     int groups;                       // gate rows that are summed over rows (1 when none are)
@@ -162,134 +191,326 @@ struct BwdPlan {
     int ctas;
 };
 
-// dgamma partials: [ctas][2][D]; dgate partials: [groups * parts][D] (after them).
-template <bool F32, bool WARP, int NT>
-__global__ void __launch_bounds__(NT)
-block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, void* dgate_rows, int dgate_f32, float* part_gamma,
-                      float* part_gate) {
-    __shared__ float red[2][2][32];
-    __shared__ float red1[2][32];
-    const int piece = WARP ? (threadIdx.x & 31) : threadIdx.x;
-    const int sub = WARP ? (threadIdx.x >> 5) : 0, nsub = WARP ? kNarrowRows : 1;
-    const bool on = piece * 8 < a.D;
-    const float inv_d = 1.f / static_cast<float>(a.D);
+// The six sums of a backward row in one round: after three steps of exchanging halves a
+// lane holds one of the (eight) values for four lanes, two more steps finish it.
+template <bool WARP>
+__device__ __forceinline__ void row_sums6(float (&v)[8], float* red, int& turn) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int n = 4, o = 16; n >= 1; n >>= 1, o >>= 1) {
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    float s = v[0];
+    s += __shfl_xor_sync(0xffffffffu, s, 2);
+    s += __shfl_xor_sync(0xffffffffu, s, 1);
+    // value index of a lane: bits 4, 3, 2
+    if constexpr (!WARP) {
+        float* mine = red + turn * 256;                         // [8 values][32 warps]
+        turn ^= 1;
+        const int idx = lane >> 2, nw = blockDim.x >> 5;
+        if ((lane & 3) == 0) mine[idx * 32 + warp] = s;
+        __syncthreads();
+        s = 0.f;
+        for (int w = lane & 3; w < nw; w += 4) s += mine[idx * 32 + w];
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * 4);
+}
+
+__device__ __forceinline__ uint64_t twice(float x) { return pack2(x, x); }
+__device__ __forceinline__ void pairs_of(const uint4& w, uint64_t (&p)[4]) {          // 8 bf16
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 bf16_of(const uint64_t (&p)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x, y;
+        unpack2(p[i], x, y);
+        w[i] = pack_bf16x2(x, y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// eight values of a row in memory (global or shared) as pairs, and back
+template <bool F32>
+__device__ __forceinline__ void read_pairs(const void* at, uint64_t (&p)[4]) {
+    if constexpr (F32) {
+        const ulonglong2 a = *static_cast<const ulonglong2*>(at), b = *(static_cast<const ulonglong2*>(at) + 1);
+        p[0] = a.x; p[1] = a.y; p[2] = b.x; p[3] = b.y;
+    } else {
+        pairs_of(*static_cast<const uint4*>(at), p);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void write_pairs(void* base, long at, const uint64_t (&p)[4]) {
+    if constexpr (F32) {
+        ulonglong2* d = reinterpret_cast<ulonglong2*>(static_cast<float*>(base) + at);
+        d[0] = make_ulonglong2(p[0], p[1]);
+        d[1] = make_ulonglong2(p[2], p[3]);
+    } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) = bf16_of(p);
+    }
+}
+__device__ __forceinline__ void weight_pairs(const uint16_t* p, long at, bool on, uint64_t (&w)[4]) {
+    float f[8];
+    weight8(p, at, on, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2(f[2 * i], f[2 * i + 1]);
+}
+
+// A backward row and the column sums of the rows before it, eight columns a thread.
+// All sums that a row's result needs come before any of it (so one barrier per row): with
+// w = gate gamma_post, g2 = dx gamma_pre
+//   sum y^2, sum h'^2, A = sum g2 h', B = sum w y dh', C = sum w y g2, E = sum w y h'
+//   mean(g2 n2) = r2 A / D,  sum g1 n1 = r1 (B + r2 C - r2^3 (A / D) E)
+// Where the rows of an item share their gate row, dgate and dgamma_post both follow from
+// q = sum dt n1, so one sum serves both.
+template <bool F32, bool WARP>
+struct BwdRow {
+    uint64_t gq[4], w[4], q[4], sum_pre[4];    // gamma_pre; gate gamma_post; column sums
+    // y, h, dx, dt (dh'): the row's values; gate, sum_post: of a row with a gate row of its own
+    template <class AfterSums>
+    __device__ __forceinline__ void run(const BlockNormArgs& a, uint64_t (&y)[4], uint64_t (&h)[4], uint64_t (&dx)[4],
+                                        uint64_t (&dt)[4], const uint64_t* gate, const uint64_t* gp, uint64_t* sum_post,
+                                        void* dgate_rows, int dgate_f32, long at, bool on, float* red, int& turn,
+                                        AfterSums after) {
+        const float inv_d = 1.f / static_cast<float>(a.D);
+        uint64_t t[6] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t x = mul2(dx[i], gq[i]), wy = mul2(w[i], y[i]);
+            t[0] = fma2(y[i], y[i], t[0]);
+            t[1] = fma2(h[i], h[i], t[1]);
+            t[2] = fma2(x, h[i], t[2]);
+            t[3] = fma2(wy, dt[i], t[3]);
+            t[4] = fma2(wy, x, t[4]);
+            t[5] = fma2(wy, h[i], t[5]);
+        }
+        float s[8];
+        s[6] = s[7] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) {
+            float lo, hi;
+            unpack2(t[i], lo, hi);
+            s[i] = lo + hi;
+        }
+        row_sums6<WARP>(s, red, turn);
+        after();
+        const float r1 = a.gamma_post ? rsqrtf(s[0] * inv_d + a.eps) : 1.f;
+        const float r2 = a.gamma_pre ? rsqrtf(s[1] * inv_d + a.eps) : 0.f;          // 0: dt = dh'
+        const float k = r2 * r2 * r2 * s[2] * inv_d;
+        const float m1 = a.gamma_post ? r1 * (s[3] + r2 * s[4] - k * s[5]) * inv_d : 0.f;
+        const uint64_t r1_2 = twice(r1), r2_2 = twice(r2), k_2 = twice(-k), m_2 = twice(-m1), al = twice(a.alpha);
+        uint64_t out[4], dg[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t n1 = mul2(y[i], r1_2), xr = mul2(dx[i], r2_2);
+            sum_pre[i] = fma2(xr, h[i], sum_pre[i]);
+            dt[i] = fma2(h[i], k_2, fma2(xr, gq[i], dt[i]));
+            out[i] = mul2(al, dt[i]);
+            if (gate) {
+                const uint64_t e = mul2(dt[i], n1);
+                dg[i] = mul2(e, gp[i]);
+                sum_post[i] = fma2(e, gate[i], sum_post[i]);
+            } else {
+                q[i] = fma2(dt[i], n1, q[i]);
+            }
+            y[i] = mul2(r1_2, fma2(n1, m_2, mul2(dt[i], w[i])));                    // dy
+        }
+        if (!on) return;
+        write_pairs<F32>(a.h_out, at, out);
+        write_pairs<false>(a.x, at, y);
+        if (gate) {
+            if (dgate_f32)
+                write_pairs<true>(dgate_rows, at, dg);
+            else
+                write_pairs<false>(dgate_rows, at, dg);
+        }
+    }
+};
+
+// The walk over items shared by the two backward kernels: dgamma partials [ctas][2][D],
+// dgate partials [groups * parts][D]; write_cols(v, dst) adds up and stores a CTA's columns.
+template <bool F32, bool WARP, class Rows, class WriteCols>
+__device__ __forceinline__ void bwd_items(const BlockNormArgs& a, const BwdPlan& plan, int col, bool on, bool row_gate,
+                                          float* part_gamma, float* part_gate, Rows rows, WriteCols write_cols) {
+    BwdRow<F32, WARP> st;
+    uint64_t sum_post[4] = {};
+    weight_pairs(a.gamma_pre, col, on, st.gq);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st.sum_pre[i] = 0;
     const int items = plan.groups * plan.parts;
     const long group_rows = a.R / plan.groups;
-    const int col = piece * 8;
-    int turn = 0, turn1 = 0;
-    float gp[8], gq[8], sum_post[8] = {}, sum_pre[8] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) gp[i] = gq[i] = 1.f;
-    if (on && a.gamma_post) unpack8(__ldg(reinterpret_cast<const uint4*>(a.gamma_post + col)), gp);
-    if (on && a.gamma_pre) unpack8(__ldg(reinterpret_cast<const uint4*>(a.gamma_pre + col)), gq);
-    extern __shared__ float cols[];            // WARP: [rows of the CTA][D] for the column sums
-    // sum over the CTA's warps of the lanes' 8 columns, in warp order, into dst (WARP only)
-    auto write_cols = [&](const float (&v)[8], float* dst) {
-        if constexpr (WARP) {
-            __syncthreads();
-            if (on)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) cols[sub * a.D + col + i] = v[i];
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-                float s = 0.f;
-                for (int w = 0; w < kNarrowRows; ++w) s += cols[w * a.D + c];
-                dst[c] = s;
-            }
-        } else if (on) {
-            float4* p = reinterpret_cast<float4*>(dst + col);
-            p[0] = make_float4(v[0], v[1], v[2], v[3]);
-            p[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    };
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
         const int g = it / plan.parts, part = it % plan.parts;
-        const long r0 = g * group_rows + group_rows * part / plan.parts;
-        const long r1_ = g * group_rows + group_rows * (part + 1) / plan.parts;
-        float sum_gate[8] = {};
-        // every warp of the CTA runs the same number of turns (WARP has no barrier in the loop)
-        for (long r = r0 + sub; r < r1_; r += nsub) {
-            const long at = r * a.D + col;
-            float y[8] = {}, h[8] = {}, dx[8] = {}, dt[8] = {}, gt[8];
+        uint64_t gp[4], gt[4];
+        weight_pairs(a.gamma_post, col, on, gp);
+        weight_pairs(row_gate ? nullptr : a.gate, static_cast<long>(g) * a.D + col, on, gt);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) gt[i] = 1.f;
-            if (on) {
-                load8_bf16(a.y + at, y);
-                load8<F32>(a.h, at, h);
-                if (a.gamma_pre) load8_bf16(a.dx + at, dx);
-                if (a.dh_out) load8<F32>(a.dh_out, at, dt);
-                if (a.gate) load8_bf16(a.gate + (r / a.rows_per_gate) * a.D + col, gt);
-            }
-            float s[2] = {0.f, 0.f}, s2[1] = {0.f};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s[0] += y[i] * y[i];
-                s[1] += h[i] * h[i];
-            }
-            row_sum<2, WARP>(s, &red[0][0][0], turn);
-            if (a.gamma_pre) {
-                const float r2 = rsqrtf(s[1] * inv_d + a.eps);
-                float m[1] = {0.f};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    h[i] *= r2;                                 // n2
-                    sum_pre[i] += dx[i] * h[i];
-                    dx[i] *= gq[i];                             // g2
-                    m[0] += dx[i] * h[i];
-                }
-                row_sum<1, WARP>(m, &red1[0][0], turn1);
-                m[0] *= inv_d;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dt[i] += r2 * (dx[i] - h[i] * m[0]);
-            }
-            const float r1 = a.gamma_post ? rsqrtf(s[0] * inv_d + a.eps) : 1.f;
-            float dg[8], out[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] *= r1;                                     // n1
-                dg[i] = dt[i] * y[i] * gp[i];
-                out[i] = a.alpha * dt[i];
-                dt[i] *= gt[i];                                 // du
-                sum_post[i] += dt[i] * y[i];
-                sum_gate[i] += dg[i];
-                dt[i] *= gp[i];                                 // g1
-                s2[0] += dt[i] * y[i];
-            }
-            if (on) {
-                store8<F32>(a.h_out, at, out);
-                if (dgate_rows) {
-                    if (dgate_f32)
-                        store8<true>(dgate_rows, at, dg);
-                    else
-                        store8<false>(dgate_rows, at, dg);
-                }
-            }
-            if (a.gamma_post) {
-                row_sum<1, WARP>(s2, &red1[0][0], turn1);
-                s2[0] *= inv_d;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dt[i] = r1 * (dt[i] - y[i] * s2[0]);
-            }
-            if (on) store8_bf16(a.x + at, dt);
+        for (int i = 0; i < 4; ++i) {
+            st.w[i] = mul2(gp[i], gt[i]);
+            st.q[i] = 0;
         }
-        if (part_gate) write_cols(sum_gate, part_gate + static_cast<long>(it) * a.D);
+        rows(st, gp, sum_post, g * group_rows + group_rows * part / plan.parts, g * group_rows + group_rows * (part + 1) / plan.parts);
+        if (!row_gate) {
+            // read again: they are not kept over the rows
+            weight_pairs(a.gamma_post, col, on, gp);
+            weight_pairs(a.gate, static_cast<long>(g) * a.D + col, on, gt);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum_post[i] = fma2(st.q[i], gt[i], sum_post[i]);
+                st.q[i] = mul2(st.q[i], gp[i]);
+            }
+            if (part_gate) write_cols(st.q, part_gate + static_cast<long>(it) * a.D);
+        }
     }
     if (part_gamma) {
         write_cols(sum_post, part_gamma + (static_cast<long>(blockIdx.x) * 2) * a.D);
-        write_cols(sum_pre, part_gamma + (static_cast<long>(blockIdx.x) * 2 + 1) * a.D);
+        write_cols(st.sum_pre, part_gamma + (static_cast<long>(blockIdx.x) * 2 + 1) * a.D);
     }
 }
 
-// out[o][c] = sum over n of in[(o * n_stride_o + n * n_stride)][c], in the order of n:
-// 32 columns x 8 partial sums a CTA, then their sum in order.
+// Narrow rows: a warp each.
+template <bool F32>
+__global__ void __launch_bounds__(32 * kNarrowRows, 2)
+block_norm_bwd_narrow_kernel(const BlockNormArgs a, const BwdPlan plan, void* dgate_rows, int dgate_f32, float* part_gamma,
+                             float* part_gate) {
+    extern __shared__ float cols[];                             // [rows of the CTA][D] for the column sums
+    const int sub = threadIdx.x >> 5, col = (threadIdx.x & 31) * 8;
+    const bool on = col < a.D, row_gate = dgate_rows != nullptr;
+    pdl_launch_dependents();
+    auto rows = [&](BwdRow<F32, true>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1) {
+        int turn = 0;
+        for (long r = r0 + sub; r < r1; r += kNarrowRows) {
+            const long at = r * a.D + col;
+            uint64_t y[4] = {}, h[4] = {}, dx[4] = {}, dt[4] = {}, gt[4] = {};
+            if (on) {
+                read_pairs<false>(a.y + at, y);
+                read_pairs<F32>(static_cast<const uint8_t*>(a.h) + at * (F32 ? 4 : 2), h);
+                if (a.gamma_pre) read_pairs<false>(a.dx + at, dx);
+                if (a.dh_out) read_pairs<F32>(static_cast<const uint8_t*>(a.dh_out) + at * (F32 ? 4 : 2), dt);
+                if (row_gate) {
+                    read_pairs<false>(a.gate + at, gt);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st.w[i] = mul2(gp[i], gt[i]);
+                }
+            }
+            st.run(a, y, h, dx, dt, row_gate ? gt : nullptr, gp, sum_post, dgate_rows, dgate_f32, at, on, nullptr, turn, [] {});
+        }
+    };
+    // sum over the CTA's warps of the lanes' columns, in warp order
+    auto write_cols = [&](const uint64_t (&v)[4], float* dst) {
+        __syncthreads();
+        if (on) write_pairs<true>(cols, sub * a.D + col, v);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
+            float s = 0.f;
+            for (int w = 0; w < kNarrowRows; ++w) s += cols[w * a.D + c];
+            dst[c] = s;
+        }
+    };
+    bwd_items<F32, true>(a, plan, col, on, row_gate, part_gamma, part_gate, rows, write_cols);
+}
+
+// Wide rows: a CTA each, through a ring of `stages` rows in shared memory that bulk copies
+// fill (y, dx, h', dh', gate row), so that several rows are in flight without registers.
+// A thread has its row in registers before the barrier of the sums, so behind that barrier the
+// stage is free and takes the row `stages` further on.
+struct BwdRing {
+    int stages, bytes;                // bytes of a stage
+    int off_dx, off_h, off_dh, off_gate;
+};
+constexpr int kMaxStages = 8;
+
+template <bool F32, int NT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1)
+block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, const BwdRing ring, void* dgate_rows, int dgate_f32,
+                      float* part_gamma, float* part_gate) {
+    extern __shared__ __align__(128) uint8_t ring_mem[];
+    __shared__ float red[2][256];
+    __shared__ uint64_t full[kMaxStages];
+    __shared__ int dead_flag;
+    volatile int* dead = &dead_flag;
+    const int tid = threadIdx.x, col = tid * 8;
+    const bool on = col < a.D, row_gate = dgate_rows != nullptr;
+    if (tid == 0) {
+        for (int i = 0; i < ring.stages; ++i) mbar_init(&full[i], 1);
+        dead_flag = 0;
+        fence_mbar_init();
+    }
+    pdl_launch_dependents();
+    __syncthreads();
+    constexpr int HB = F32 ? 4 : 2;
+    uint32_t used = 0;                                          // rows taken from the ring so far
+    int turn = 0;
+    auto issue = [&](long r, uint32_t n) {                      // one thread: row r as the ring's n-th
+        uint8_t* s = ring_mem + (n % ring.stages) * ring.bytes;
+        uint64_t* bar = &full[n % ring.stages];
+        const uint32_t e = a.D;
+        const long at = r * a.D;
+        mbar_arrive_expect_tx(bar, e * (2 + HB) + (a.gamma_pre ? e * 2 : 0) + (a.dh_out ? e * HB : 0) + (row_gate ? e * 2 : 0));
+        bulk_load(s, a.y + at, e * 2, bar);
+        bulk_load(s + ring.off_h, static_cast<const uint8_t*>(a.h) + at * HB, e * HB, bar);
+        if (a.gamma_pre) bulk_load(s + ring.off_dx, a.dx + at, e * 2, bar);
+        if (a.dh_out) bulk_load(s + ring.off_dh, static_cast<const uint8_t*>(a.dh_out) + at * HB, e * HB, bar);
+        if (row_gate) bulk_load(s + ring.off_gate, a.gate + at, e * 2, bar);
+    };
+    auto rows = [&](BwdRow<F32, false>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1) {
+        if (tid == 0)
+            for (long r = r0; r < r1 && r < r0 + ring.stages; ++r) issue(r, used + static_cast<uint32_t>(r - r0));
+        for (long r = r0; r < r1; ++r, ++used) {
+            const long at = r * a.D + col;
+            const uint8_t* s = ring_mem + (used % ring.stages) * ring.bytes;
+            // gives up with the error word set; the rows then hold anything, the walk ends as usual
+            mbar_wait_or_abort(&full[used % ring.stages], (used / ring.stages) & 1u, a.err, dead);
+            uint64_t y[4] = {}, h[4] = {}, dx[4] = {}, dt[4] = {}, gt[4] = {};
+            if (on) {
+                read_pairs<false>(s + col * 2, y);
+                read_pairs<F32>(s + ring.off_h + col * HB, h);
+                if (a.gamma_pre) read_pairs<false>(s + ring.off_dx + col * 2, dx);
+                if (a.dh_out) read_pairs<F32>(s + ring.off_dh + col * HB, dt);
+                if (row_gate) {
+                    read_pairs<false>(s + ring.off_gate + col * 2, gt);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st.w[i] = mul2(gp[i], gt[i]);
+                }
+            }
+            st.run(a, y, h, dx, dt, row_gate ? gt : nullptr, gp, sum_post, dgate_rows, dgate_f32, at, on, &red[0][0], turn, [&] {
+                if (tid == 0 && r + ring.stages < r1) issue(r + ring.stages, used + ring.stages);
+            });
+        }
+    };
+    auto write_cols = [&](const uint64_t (&v)[4], float* dst) {
+        if (on) write_pairs<true>(dst, col, v);
+    };
+    bwd_items<F32, false>(a, plan, col, on, row_gate, part_gamma, part_gate, rows, write_cols);
+    __syncthreads();
+    if (dead_flag && tid == 0)                                  // gave up: let the copies in flight land
+        for (uint32_t n = used > static_cast<uint32_t>(ring.stages) ? used - ring.stages : 0; n < used; ++n)
+            mbar_wait(&full[n % ring.stages], (n / ring.stages) & 1u, a.err);
+}
+
+// out[o][c] = sum over n of in[(o * n_stride_o + n * n_stride)][c]: 32 columns a CTA, each of
+// its 16 warps every 16th n (loads in batches of 8), then the warps' sums in order.
 struct SumJob {
     const float* in;
     float* out;
     long o_stride, n_stride;          // elements
     int n;
 };
-__global__ void __launch_bounds__(256) column_sum_kernel(const SumJob j0, const SumJob j1, const SumJob j2, int D) {
-    __shared__ float part[8][32];
+constexpr int kSumWarps = 16;
+__global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const SumJob j0, const SumJob j1, const SumJob j2, int D) {
+    __shared__ float part[kSumWarps][32];
+    pdl_wait_prior();
     // blockIdx.y 0: dgamma_post, 1: dgamma_pre, 2 + g: gate row g
     const SumJob& j = blockIdx.y == 0 ? j0 : blockIdx.y == 1 ? j1 : j2;
     if (!j.out) return;
@@ -298,25 +519,34 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const SumJob j0, const 
     float s = 0.f;
     if (c < D) {
         const float* p = j.in + o * j.o_stride + c;
-        for (int n = k; n < j.n; n += 8) s += __ldcg(p + n * j.n_stride);
+        for (int n0 = k; n0 < j.n; n0 += 8 * kSumWarps) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = n0 + i * kSumWarps < j.n ? __ldcg(p + (n0 + i * kSumWarps) * j.n_stride) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
     }
     part[k][threadIdx.x & 31] = s;
     __syncthreads();
     if (k == 0 && c < D) {
-        for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x & 31];
+#pragma unroll
+        for (int i = 1; i < kSumWarps; ++i) s += part[i][threadIdx.x & 31];
         j.out[o * D + c] = s;
     }
 }
 
 int block_threads(int D) { return D <= kNarrow ? 32 * kNarrowRows : (D / 8 + 31) / 32 * 32; }
 
+// backward CTAs per SM, at 128 registers a thread
+int bwd_resident(int D) { return block_threads(D) < 512 ? 512 / block_threads(D) : 1; }
+
 // `groups`: gate rows whose gradient is a sum over rows (1 without such a sum).
 BwdPlan bwd_plan(int R, int D, int groups) {
     BwdPlan p;
     p.groups = groups;
     const int per_cta = D <= kNarrow ? kNarrowRows : 1;
-    const int resident = 2048 / block_threads(D) > 4 ? 4 : 2048 / block_threads(D);
-    const int want = 148 * (resident < 1 ? 1 : resident);
+    const int want = 148 * bwd_resident(D);
     const long group_rows = R / groups;
     long parts = (want + groups - 1) / groups;
     if (parts > (group_rows + per_cta - 1) / per_cta) parts = (group_rows + per_cta - 1) / per_cta;
@@ -352,7 +582,9 @@ int launch_fwd(const BlockNormArgs& a, cudaStream_t st) {
     const int nt = block_threads(a.D);
     cfg.blockDim = dim3(nt);
     const int rows = a.D <= kNarrow ? kNarrowRows : 1;
-    cfg.gridDim = dim3((a.R + rows - 1) / rows);
+    // as many CTAs as are resident at once (48 registers a thread), each for several rows
+    const int most = 148 * (1024 / nt > 0 ? 1024 / nt : 1), need = (a.R + rows - 1) / rows;
+    cfg.gridDim = dim3(need < most ? need : most);
     cudaError_t e;
     if (a.D <= kNarrow)
         e = cudaLaunchKernelEx(&cfg, block_norm_fwd_kernel<F32, true, 256>, a);
@@ -364,20 +596,41 @@ int launch_fwd(const BlockNormArgs& a, cudaStream_t st) {
     return launch_status("gdn_block_norm_fwd");
 }
 
+// The ring of a wide backward row: as many stages as the SM's CTAs leave room for.
+BwdRing bwd_ring(const BlockNormArgs& a, bool f32, bool row_gate) {
+    BwdRing r;
+    const int row = a.D * 2, hrow = a.D * (f32 ? 4 : 2);
+    r.off_dx = row;
+    r.off_h = r.off_dx + (a.gamma_pre ? row : 0);
+    r.off_dh = r.off_h + hrow;
+    r.off_gate = r.off_dh + (a.dh_out ? hrow : 0);
+    r.bytes = r.off_gate + (row_gate ? row : 0);
+    const int room = (220 * 1024) / bwd_resident(a.D) - (bwd_resident(a.D) > 1 ? 4096 : 0);
+    r.stages = room / r.bytes < kMaxStages ? room / r.bytes : kMaxStages;
+    return r;
+}
+
 template <bool F32>
 int launch_bwd(const BlockNormArgs& a, const BwdPlan& p, void* dgate_rows, int dgate_f32, float* part_gamma,
                float* part_gate, cudaStream_t st) {
+    const char* name = "gdn_block_norm_bwd";
     const int nt = block_threads(a.D);
-    if (a.D <= kNarrow)
-        block_norm_bwd_kernel<F32, true, 256>
+    if (a.D <= kNarrow) {
+        block_norm_bwd_narrow_kernel<F32>
             <<<p.ctas, nt, kNarrowRows * a.D * sizeof(float), st>>>(a, p, dgate_rows, dgate_f32, part_gamma, part_gate);
-    else if (nt <= 256)
-        block_norm_bwd_kernel<F32, false, 256><<<p.ctas, nt, 0, st>>>(a, p, dgate_rows, dgate_f32, part_gamma, part_gate);
-    else if (nt <= 512)
-        block_norm_bwd_kernel<F32, false, 512><<<p.ctas, nt, 0, st>>>(a, p, dgate_rows, dgate_f32, part_gamma, part_gate);
-    else
-        block_norm_bwd_kernel<F32, false, 1024><<<p.ctas, nt, 0, st>>>(a, p, dgate_rows, dgate_f32, part_gamma, part_gate);
-    return launch_status("gdn_block_norm_bwd");
+        return launch_status(name);
+    }
+    const BwdRing ring = bwd_ring(a, F32, dgate_rows != nullptr);
+    const size_t smem = static_cast<size_t>(ring.stages) * ring.bytes;
+    auto go = [&](auto kernel) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 221 * 1024);
+        if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(e));
+        kernel<<<p.ctas, nt, smem, st>>>(a, p, ring, dgate_rows, dgate_f32, part_gamma, part_gate);
+        return launch_status(name);
+    };
+    if (nt <= 256) return go(block_norm_bwd_kernel<F32, 256>);
+    if (nt <= 512) return go(block_norm_bwd_kernel<F32, 512>);
+    return go(block_norm_bwd_kernel<F32, 1024>);
 }
 
 // Gate rows whose gradient is a sum (a gate row of its own for every row needs none).
@@ -471,11 +724,13 @@ extern "C" int gdn_block_norm_bwd(const void* y, const void* h_out, int h_dtype,
     a.x = static_cast<uint16_t*>(dy);
     a.dh_out = dh_out;
     a.dx = static_cast<const uint16_t*>(dx);
+    a.err = device_error_word();
     a.alpha = residual_scale;
     a.eps = eps;
     a.R = R;
     a.D = D;
     a.rows_per_gate = gate ? R / gate_rows : R;
+    if (!gamma_pre) a.dx = nullptr;
     float* part_gamma = (gamma_post || gamma_pre) ? static_cast<float*>(workspace) : nullptr;
     float* part_gate = sg ? static_cast<float*>(workspace) + static_cast<size_t>(p.ctas) * 2 * D : nullptr;
     void* dgate_rows = gate && !sg ? dgate : nullptr;
@@ -487,7 +742,16 @@ extern "C" int gdn_block_norm_bwd(const void* y, const void* h_out, int h_dtype,
     const SumJob j0 = {part_gamma, gamma_post ? dgamma_post : nullptr, 0, 2l * D, p.ctas};
     const SumJob j1 = {part_gamma ? part_gamma + D : nullptr, gamma_pre ? dgamma_pre : nullptr, 0, 2l * D, p.ctas};
     const SumJob j2 = {part_gate, part_gate ? static_cast<float*>(dgate) : nullptr, static_cast<long>(p.parts) * D, D, p.parts};
-    const dim3 grid((D + 31) / 32, 2 + (part_gate ? groups : 0));
-    column_sum_kernel<<<grid, 256, 0, s>>>(j0, j1, j2, D);
+    cudaLaunchConfig_t cfg = {};                               // starts while the row kernel ends
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.stream = s;
+    cfg.gridDim = dim3((D + 31) / 32, 2 + (part_gate ? groups : 0));
+    cfg.blockDim = dim3(32 * kSumWarps);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, column_sum_kernel, j0, j1, j2, D);
+    if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
     return launch_status("gdn_block_norm_bwd (column sums)");
 }

@@ -27,6 +27,7 @@
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // With two row tiles the tensor core works for one while the softmax of the other runs;
 // with one row tile (at most 128 rows, the decode step) S is double buffered instead.
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -59,31 +60,15 @@ struct AttnArgs {
     int item_cost;
     unsigned int* err;
     int* part_state;                  // [ctas][8]: what a CTA left unfinished
-    float* part_ml;                   // [ctas][2][QT 128][2]: m, l
-    float* part_o;                    // [ctas][2][D / 4][QT 128][4]
+    int part_rows;                    // rows of a part
+    float* part_ml;                   // [ctas][2][part_rows][2]: m, l
+    float* part_o;                    // [ctas][2][D / 4][part_rows][4]
 };
 
 struct alignas(64) AttnMaps {
     CUtensorMap q, k, v;
 };
 
-// packed pairs of fp32 (one instruction for two values)
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -785,8 +770,8 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     if (a.lse && real) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
                 } else {
                     // slot 0: a part that does not hold the item's first tile; 1: the first part
-                    const long part = static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0), slot = part * (QT * 128) + t * 128 + row;
-                    float4* dst = reinterpret_cast<float4*>(a.part_o) + part * (D / 4) * (QT * 128) + t * 128 + row;
+                    const long part = static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0), slot = part * a.part_rows + t * 128 + row;
+                    float4* dst = reinterpret_cast<float4*>(a.part_o) + part * (D / 4) * a.part_rows + t * 128 + row;
 #pragma unroll
                     for (int q = 0; q < D / 32; ++q) {
                         float o[32];
@@ -795,7 +780,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         if (real)
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                dst[(q * 8 + i) * (QT * 128)] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                dst[(q * 8 + i) * a.part_rows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                     if (real) {
                         a.part_ml[slot * 2] = m;
@@ -830,15 +815,16 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     }
 }
 
-// Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
-// began and did not finish, rows 32 y .. 32 y + 31.  Lanes go along rows, as the parts lie
-// in memory; a warp takes D / 8 columns.
-constexpr int kJoinParts = 160;       // parts of an item: at most one per CTA
-template <int D, int QT>
+// Joins the parts of the items that pieces cut: block (x, y, z) takes the item that CTA x
+// began and did not finish, rows 32 y .. 32 y + 31 (a lane each, as the parts lie in memory)
+// and 32 V columns (a warp takes V float4).  All loads of a thread are independent of one
+// another but for the first, of the states.  V = 1 spreads the columns of few rows with
+// many parts over blocks; more blocks than that cost more to start than they save (4 us
+// for 4 x as many at one short sequence).
+template <int D, int QT, int V>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
-    __shared__ float weight[kJoinParts][32], sums[kJoinParts][32], row_m[8][32];
     pdl_wait_prior();
-    constexpr int ROWS = QT * 128, V = D / 32;                  // V float4 per thread
+    const int rows = a.part_rows;
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the states of this CTA and of the 31 after it in one go
     const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
@@ -849,7 +835,6 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     const int row = blockIdx.y * 32 + lane, r = row & 127;
     const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
     const bool real = tl < a.tile_tokens && tok < toks;
-    if (!__any_sync(0xffffffffu, real)) return;                 // the same in every warp
     int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
     for (int at = x + 1;;) {
         const uint32_t end = __ballot_sync(0xffffffffu, st != 1);
@@ -862,65 +847,84 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
         at += 32;
         st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
     }
+    if (!real) return;
     const float c = a.scale * 1.4426950408889634f;
-    auto part = [&](int p) { return static_cast<long>(x + p) * 2 + (p == 0 ? 1 : 0); };
-    // m and l of every part (a warp takes every eighth), then the weights from the largest m
-    float m = -INFINITY;
-    for (int p = warp; p < parts; p += 8) {
-        const float2 v = real ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + part(p) * ROWS + row) : make_float2(0.f, 0.f);
-        const float mp = v.y == 0.f ? -INFINITY : v.x;
-        weight[p][lane] = mp;
-        sums[p][lane] = v.y;
-        m = fmaxf(m, mp);
-    }
-    row_m[warp][lane] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, row_m[i][lane]);
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    for (int p = warp; p < parts; p += 8) weight[p][lane] = ex2_approx(weight[p][lane] * c - mc);
-    __syncthreads();
-    float l = 0.f;                                              // in the order of the parts, in every warp alike
-    for (int p = 0; p < parts; ++p) l += weight[p][lane] * sums[p][lane];
+    // part 0 is CTA x's slot 1, part p the slot 0 of CTA x + p
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (static_cast<long>(x) * 2) * rows + row;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) +
+                       (static_cast<long>(x) * 2 * (D / 4) + (blockIdx.z * 8 + warp) * V) * rows + row;
+    auto slot = [](int p) { return p == 0 ? 1 : 2 * p; };
+    // one pass with a running maximum; loads in batches under a predicate (a remainder loop
+    // would wait for each of them)
+    constexpr int N = V == 1 ? 16 : 4;
+    float m = -INFINITY, l = 0.f;
     float4 o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (real) {
-#pragma unroll 6
-        for (int p = 0; p < parts; ++p) {
-            const float w = weight[p][lane];
-            const float4* src = reinterpret_cast<const float4*>(a.part_o) + (part(p) * (D / 4) + warp * V) * ROWS + row;
+    for (int p0 = 0; p0 < parts; p0 += N) {
+        float2 v[N];
+        float4 u[N][V];
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] = p0 + k < parts ? __ldcg(ml + slot(p0 + k) * rows) : make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                u[k][i] = p0 + k < parts ? __ldcg(po + (static_cast<long>(slot(p0 + k)) * (D / 4) + i) * rows)
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
+        const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
+        m = mn;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float w = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
+            l += v[k].y * w;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float4 v = __ldcg(src + i * ROWS);
-                o[i].x += v.x * w; o[i].y += v.y * w; o[i].z += v.z * w; o[i].w += v.w * w;
+                o[i].x += u[k][i].x * w; o[i].y += u[k][i].y * w; o[i].z += u[k][i].z * w; o[i].w += u[k][i].w * w;
             }
         }
     }
-    if (!real) return;
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
-    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + warp * V;
+    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + (blockIdx.z * 8 + warp) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i)
         dst[i] = l == 0.f ? make_uint2(0u, 0u)
                           : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
-    if (a.lse && warp == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    if (a.lse && warp == 0 && blockIdx.z == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
 
 size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
-size_t ml_bytes(int qt) { return static_cast<size_t>(kMaxCtas) * 2 * qt * 128 * 2 * sizeof(float); }
-size_t o_bytes(int qt, int D) { return static_cast<size_t>(kMaxCtas) * 2 * qt * 128 * D * sizeof(float); }
+size_t ml_bytes(int rows) { return static_cast<size_t>(kMaxCtas) * 2 * rows * 2 * sizeof(float); }
+size_t o_bytes(int rows, int D) { return static_cast<size_t>(kMaxCtas) * 2 * rows * D * sizeof(float); }
 
 // One row tile per item when the longest chunk's rows fit one, else two.
 int row_tiles(int max_q, int group) { return static_cast<long>(max_q) <= 128 / group ? 1 : 2; }
+// Rows of an unfinished item's part: both row tiles, or the rows that the longest chunk has
+// (compact, so that the parts of a decode step lie close together).
+int part_rows(int max_q, int group) { return row_tiles(max_q, group) == 2 ? 256 : max((max_q * group + 7) / 8 * 8, 8); }
 
 template <int D, int QT>
 int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     using S = Shape<D, QT>;
     const char* name = "gdn_paged_attn_fwd";
-    const cudaError_t attr = cudaFuncSetAttribute(paged_attn_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (attr != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr));
+    static std::once_flag once[64];                             // once per device
+    static cudaError_t attr[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(GDN_ERR_CUDA, "%s: no current device", name);
+    std::call_once(once[dev], [dev] {
+        attr[dev] = cudaFuncSetAttribute(paged_attn_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    });
+    if (attr[dev] != cudaSuccess)
+        return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr[dev]));
     paged_attn_kernel<D, QT><<<kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
     int rc = launch_status(name);
     if (rc != GDN_OK) return rc;
@@ -930,10 +934,14 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3(kMaxCtas, QT * 4);
+    const int rows = min(a.max_q, QT * a.tile_tokens) * a.group, slices = QT == 2 ? 8 : max((rows + 31) / 32, 1);
+    cfg.gridDim = dim3(kMaxCtas, slices, slices == 1 ? D / 32 : 1);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D, QT>, a, kMaxCtas);
+    void (*join)(AttnArgs, int) = paged_attn_join_kernel<D, QT, D / 32>;
+    if constexpr (QT == 1)
+        if (slices == 1) join = paged_attn_join_kernel<D, QT, 1>;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a, static_cast<int>(kMaxCtas));
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
     return launch_status(name);
 }
@@ -948,8 +956,8 @@ extern "C" size_t gdn_paged_attn_workspace_bytes(int B, int Ttot, int Hq, int n_
     if (B < 1 || Ttot < 1 || Hq < 1 || n_kv < 1 || Hq % n_kv != 0 || Hq / n_kv > 64 || max_q < 0 || max_kv < 0 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    const int qt = row_tiles(max_q, Hq / n_kv);
-    return state_bytes() + ml_bytes(qt) + o_bytes(qt, head_dim);
+    const int rows = part_rows(max_q, Hq / n_kv);
+    return state_bytes() + ml_bytes(rows) + o_bytes(rows, head_dim);
 }
 
 extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cache* cache, const int* cu_seqlens,
@@ -1006,10 +1014,11 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.err = device_error_word();
     const int qt = row_tiles(max_q, a.group);
     a.item_cost = item_cost(qt);
+    a.part_rows = part_rows(max_q, a.group);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_state = reinterpret_cast<int*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + state_bytes());
-    a.part_o = reinterpret_cast<float*>(ws + state_bytes() + ml_bytes(qt));
+    a.part_o = reinterpret_cast<float*>(ws + state_bytes() + ml_bytes(a.part_rows));
 
     AttnMaps maps;
     {

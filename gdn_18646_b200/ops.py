@@ -18,6 +18,7 @@ the sm_100a kernels of the library.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -29,7 +30,8 @@ CHUNK = 64
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream of the current device as a handle, without building a Stream object
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t):
@@ -561,23 +563,49 @@ def decode_proj(x, segments, *, norm_gamma=None, eps=1e-6):
 # ---------------------------------------------------------------------------
 
 
-def _gate_rows(gate, R, D):
-    """(gate rows, whether the gate is per row) of a gate [D] or [G, D]; checks it."""
+def _dense(t, name, dtype):
+    """A contiguous CUDA tensor of that type (one test on the way that is right)."""
+    if not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
+        _cuda_contig(t, name, dtype)
+
+
+def _shaped(t, name, shape, dtype):
+    _dense(t, name, dtype)
+    if t.shape != shape:
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _like(t):
+    """An uninitialised contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _norm_args(y, h, hname, gamma_post, gate, gamma_pre):
+    """Checks shared by block_norm and its backward; returns (rows, columns, residual type
+    code, gate rows, whether every row has its own gate row)."""
+    _dense(y, "y", torch.bfloat16)
+    hdt = _gate_dtype(h, hname)
+    if h.shape != y.shape or y.dim() < 1 or y.shape[-1] == 0:
+        raise RuntimeError(f"{hname} must have y's shape, with at least one column")
+    _dense(h, hname, h.dtype)
+    D = y.shape[-1]
+    R = y.numel() // D
+    for name, w in (("gamma_post", gamma_post), ("gamma_pre", gamma_pre)):
+        if w is not None:
+            _dense(w, name, torch.bfloat16)
+            if w.dim() != 1 or w.shape[0] != D:
+                raise RuntimeError(f"{name} must be [{D}]")
     if gate is None:
-        return 0, False
-    _cuda_contig(gate, "gate", torch.bfloat16)
-    _need(gate.dim() in (1, 2) and gate.shape[-1] == D, f"gate must be [{D}] or [G, {D}]")
+        return R, D, hdt, 0, False
+    _dense(gate, "gate", torch.bfloat16)
+    if gate.dim() not in (1, 2) or gate.shape[-1] != D:
+        raise RuntimeError(f"gate must be [{D}] or [G, {D}]")
     if gate.dim() == 1:
-        return 1, False
+        return R, D, hdt, 1, False
     G = gate.shape[0]
-    _need(G >= 1 and R % G == 0, f"gate rows ({G}) must divide the {R} rows")
-    return G, G == R
-
-
-def _norm_weight(t, name, D):
-    if t is not None:
-        _cuda_contig(t, name, torch.bfloat16)
-        _need(t.dim() == 1 and t.shape[0] == D, f"{name} must be [{D}]")
+    if G < 1 and R > 0 or G > 0 and R % G != 0:
+        raise RuntimeError(f"gate rows ({G}) must divide the {R} rows")
+    return R, D, hdt, G, G == R
 
 
 def block_norm(y, h, *, gamma_post=None, gate=None, gamma_pre=None, residual_scale=1.0, eps=1e-6, h_out=None,
@@ -590,32 +618,21 @@ def block_norm(y, h, *, gamma_post=None, gate=None, gamma_pre=None, residual_sca
     [G, D] bf16 with G dividing the rows (a gate row per sequence, or per token);
     gammas [D] bf16.  Returns (h', x): h' in h's type, x bf16 or None without
     gamma_pre.  ``h_out=h`` updates the residual stream in place."""
-    _cuda_contig(y, "y", torch.bfloat16)
-    _cuda_contig(h, "h")
-    _need(h.shape == y.shape and y.dim() >= 1, "h must have y's shape")
-    hdt = _gate_dtype(h, "h")
-    D = y.shape[-1]
-    _need(D > 0, "y must have at least one column")
-    R = y.numel() // D
-    G, _ = _gate_rows(gate, R, D)
-    _norm_weight(gamma_post, "gamma_post", D)
-    _norm_weight(gamma_pre, "gamma_pre", D)
+    R, D, hdt, G, _ = _norm_args(y, h, "h", gamma_post, gate, gamma_pre)
     if h_out is None:
         h_out = torch.empty_like(h)
     else:
-        _cuda_contig(h_out, "h_out", h.dtype)
-        _need(h_out.shape == h.shape, "h_out must have h's shape")
+        _shaped(h_out, "h_out", h.shape, h.dtype)
     if gamma_pre is None:
         x_out = None
     elif x_out is None:
         x_out = torch.empty_like(y)
     else:
-        _cuda_contig(x_out, "x_out", torch.bfloat16)
-        _need(x_out.shape == y.shape, "x_out must have y's shape")
+        _shaped(x_out, "x_out", y.shape, torch.bfloat16)
     if R == 0:
         return h_out, x_out
-    _lib.call("gdn_block_norm_fwd", _ptr(y), _ptr(h), hdt, _ptr(gamma_post), _ptr(gate), G, _ptr(gamma_pre),
-              float(residual_scale), _ptr(h_out), _ptr(x_out), R, D, float(eps), _stream())
+    _lib.call("gdn_block_norm_fwd", y.data_ptr(), h.data_ptr(), hdt, _ptr(gamma_post), _ptr(gate), G, _ptr(gamma_pre),
+              float(residual_scale), h_out.data_ptr(), _ptr(x_out), R, D, float(eps), _stream())
     return h_out, x_out
 
 
@@ -626,38 +643,30 @@ def block_norm_backward(y, h_out, dh_out=None, dx=None, *, gamma_post=None, gate
     dict of dy bf16, dh in h_out's type, dgamma_post and dgamma_pre [D] f32 and dgate
     (f32 [D] or [G, D], sums over the rows that share a gate row; bf16 [R, D] for a gate
     row per row), None where there is no such input."""
-    _cuda_contig(y, "y", torch.bfloat16)
-    _cuda_contig(h_out, "h_out")
-    _need(h_out.shape == y.shape and y.dim() >= 1, "h_out must have y's shape")
-    hdt = _gate_dtype(h_out, "h_out")
-    D = y.shape[-1]
-    _need(D > 0, "y must have at least one column")
-    R = y.numel() // D
-    G, per_row = _gate_rows(gate, R, D)
-    _norm_weight(gamma_post, "gamma_post", D)
-    _norm_weight(gamma_pre, "gamma_pre", D)
+    R, D, hdt, G, per_row = _norm_args(y, h_out, "h_out", gamma_post, gate, gamma_pre)
     if dh_out is not None:
-        _cuda_contig(dh_out, "dh_out", h_out.dtype)
-        _need(dh_out.shape == y.shape, "dh_out must have y's shape")
+        _shaped(dh_out, "dh_out", y.shape, h_out.dtype)
     if gamma_pre is None:
         dx = None
+    elif dx is None:
+        raise RuntimeError("dx is required with gamma_pre")
     else:
-        _need(dx is not None, "dx is required with gamma_pre")
-        _cuda_contig(dx, "dx", torch.bfloat16)
-        _need(dx.shape == y.shape, "dx must have y's shape")
-    f32 = dict(dtype=torch.float32, device=y.device)
+        _shaped(dx, "dx", y.shape, torch.bfloat16)
+    # the sums over rows share an allocation
+    summed = gate is not None and not per_row
+    rows = torch.empty(2 + (G if summed else 0), D, dtype=torch.float32, device=y.device)
     g = dict(dy=torch.empty_like(y), dh=torch.empty_like(h_out),
-             dgate=None if gate is None else torch.empty_like(gate) if per_row else torch.empty(gate.shape, **f32),
-             dgamma_post=None if gamma_post is None else torch.empty(D, **f32),
-             dgamma_pre=None if gamma_pre is None else torch.empty(D, **f32))
+             dgate=None if gate is None else torch.empty_like(gate) if per_row else rows[2:].view(gate.shape),
+             dgamma_post=None if gamma_post is None else rows[0], dgamma_pre=None if gamma_pre is None else rows[1])
     if R == 0:
         return {n: None if t is None else t.zero_() for n, t in g.items()}
-    ws_bytes = int(_lib.lib().gdn_block_norm_bwd_workspace_bytes(R, D, G))
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=y.device)
-    _lib.call("gdn_block_norm_bwd", _ptr(y), _ptr(h_out), hdt, _ptr(dh_out), _ptr(dx), _ptr(gamma_post), _ptr(gate), G,
-              _ptr(gamma_pre), float(residual_scale), _ptr(g["dy"]), _ptr(g["dh"]), _ptr(g["dgate"]),
-              GDN_DTYPE_BF16 if per_row else GDN_DTYPE_F32, _ptr(g["dgamma_post"]), _ptr(g["dgamma_pre"]), R, D,
-              float(eps), _ptr(ws), ws_bytes, _stream())
+    ws_bytes = _lib.lib().gdn_block_norm_bwd_workspace_bytes(R, D, G)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=y.device)
+    at = rows.data_ptr()
+    _lib.call("gdn_block_norm_bwd", y.data_ptr(), h_out.data_ptr(), hdt, _ptr(dh_out), _ptr(dx), _ptr(gamma_post),
+              _ptr(gate), G, _ptr(gamma_pre), float(residual_scale), g["dy"].data_ptr(), g["dh"].data_ptr(),
+              _ptr(g["dgate"]), GDN_DTYPE_BF16 if per_row else GDN_DTYPE_F32, None if gamma_post is None else at,
+              None if gamma_pre is None else at + 4 * D, R, D, float(eps), ws.data_ptr(), ws_bytes, _stream())
     return g
 
 
@@ -698,39 +707,48 @@ def _token_rows(t, name):
     """(tokens, heads, D, elements between tokens) of [..., H, D] bf16 whose heads and
     values are contiguous and whose tokens are rows of one stride (a slice of a fused
     projection is one)."""
-    _need(t.is_cuda and t.dtype == torch.bfloat16, f"{name} must be a bfloat16 CUDA tensor")
-    _need(t.dim() >= 3, f"{name} must be [..., heads, head dim]")
-    H, D = t.shape[-2], t.shape[-1]
+    if not (t.is_cuda and t.dtype is torch.bfloat16):
+        raise RuntimeError(f"{name} must be a bfloat16 CUDA tensor")
+    shape = t.shape
+    if len(shape) < 3:
+        raise RuntimeError(f"{name} must be [..., heads, head dim]")
+    H, D = shape[-2], shape[-1]
     if t.is_contiguous():
-        return t.numel() // (H * D) if H * D else 0, H, D, H * D
+        return (shape[0] if len(shape) == 3 else t.numel() // (H * D) if H * D else 0), H, D, H * D
     _need(t.stride(-1) == 1 and (H == 1 or t.stride(-2) == D), f"{name}: heads and values must be contiguous")
     T, ld = 1, None
-    for n, s in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+    for n, s in zip(reversed(shape[:-2]), reversed(t.stride()[:-2])):
         if n == 1:
             continue
         if ld is None:
             ld = s
-        else:
-            _need(s == ld * T, f"{name}: tokens must be rows of one stride")
+        elif s != ld * T:
+            raise RuntimeError(f"{name}: tokens must be rows of one stride")
         T *= n
     return T, H, D, (H * D if ld is None else ld)
 
 
+@functools.lru_cache(maxsize=64)
+def _int_array(values):
+    """A C array of these ints (they are few and known at the call)."""
+    return (ctypes.c_int * len(values))(*values)
+
+
 def _rope_spec(positions, inv_freq, sections, style, T):
-    _need(style in _ROPE_STYLES, f"style must be 'half' or 'interleaved', got {style!r}")
-    _need(positions.is_cuda and positions.dtype == torch.int32, "positions must be an int32 CUDA tensor")
-    _need(inv_freq.is_cuda and inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
-          "inv_freq must be a contiguous float32 CUDA vector")
+    code = _ROPE_STYLES.get(style)
+    if code is None:
+        raise RuntimeError(f"style must be 'half' or 'interleaved', got {style!r}")
+    if not (positions.is_cuda and positions.dtype is torch.int32):
+        raise RuntimeError("positions must be an int32 CUDA tensor")
+    if not (inv_freq.is_cuda and inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+        raise RuntimeError("inv_freq must be a contiguous float32 CUDA vector")
     pairs = inv_freq.shape[0]
     sections = (pairs,) if sections is None else tuple(sections)
     axes = len(sections)
-    _need(positions.is_contiguous() and positions.numel() == axes * T,
-          f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis)")
-    sec = (ctypes.c_int * axes)(*sections)
-    spec = _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.cast(sec, ctypes.c_void_p), axes, 2 * pairs,
-                         _ROPE_STYLES[style])
-    spec._keep = sec
-    return spec
+    if not positions.is_contiguous() or positions.numel() != axes * T:
+        raise RuntimeError(f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis)")
+    return _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.addressof(_int_array(sections)), axes,
+                         2 * pairs, code)
 
 
 def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=False, q_out=None, k_out=None):
@@ -749,20 +767,20 @@ def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=Fals
         _need(Tk == T and Dk == D, "k must have q's tokens and head dim")
     spec = _rope_spec(positions, inv_freq, sections, style, T)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = _like(q)
     else:
-        _cuda_contig(q_out, "q_out", torch.bfloat16)
-        _need(q_out.shape == q.shape, "q_out must have q's shape")
-    if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    elif k is not None:
-        _cuda_contig(k_out, "k_out", torch.bfloat16)
-        _need(k_out.shape == k.shape, "k_out must have k's shape")
+        _shaped(q_out, "q_out", q.shape, torch.bfloat16)
+    if k is None:
+        k_out = None
+    elif k_out is None:
+        k_out = _like(k)
+    else:
+        _shaped(k_out, "k_out", k.shape, torch.bfloat16)
     if T == 0:
-        return q_out, (k_out if k is not None else None)
-    _lib.call("gdn_rope_fwd", _ptr(q), q_ld, _ptr(k), k_ld, _ptr(q_out), _ptr(k_out), ctypes.byref(spec),
+        return q_out, k_out
+    _lib.call("gdn_rope_fwd", q.data_ptr(), q_ld, _ptr(k), k_ld, q_out.data_ptr(), _ptr(k_out), ctypes.byref(spec),
               1 if inverse else 0, T, Hq, Hk, D, _stream())
-    return q_out, (k_out if k is not None else None)
+    return q_out, k_out
 
 
 class RopeFunction(torch.autograd.Function):
@@ -788,32 +806,34 @@ def rope_autograd(q, k, positions, inv_freq, sections=None, *, style="half"):
 
 
 def _paged_cache(k_cache, v_cache, block_table, layout):
-    _need(layout in ("bthd", "bhtd"), f"layout must be 'bthd' or 'bhtd', got {layout!r}")
-    _need(k_cache.is_cuda and v_cache.is_cuda and k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16,
-          "k_cache and v_cache must be bfloat16 CUDA tensors")
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
-          "k_cache and v_cache must be 4-d and share shape and strides")
-    _need(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
-          and (block_table.stride(1) == 1 or block_table.shape[1] == 1), "block_table must be int32 [B, pages] CUDA rows")
-    st = k_cache.stride()
-    _need(st[3] == 1, "k_cache, v_cache: the values of a row must be contiguous")
+    if not (k_cache.is_cuda and v_cache.is_cuda and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16):
+        raise RuntimeError("k_cache and v_cache must be bfloat16 CUDA tensors")
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != st or st[3] != 1:
+        raise RuntimeError("k_cache and v_cache must be 4-d and share shape and strides, the values of a row contiguous")
+    ts = block_table.shape
+    if not (block_table.is_cuda and block_table.dtype is torch.int32 and len(ts) == 2
+            and (block_table.is_contiguous() or block_table.stride(1) == 1)):
+        raise RuntimeError("block_table must be int32 [B, pages] CUDA rows")
     if layout == "bthd":
-        pages, page_size, n_kv, D = k_cache.shape
+        pages, page_size, n_kv, D = shape
         token, head = st[1], st[2]
-    else:
-        pages, n_kv, page_size, D = k_cache.shape
+    elif layout == "bhtd":
+        pages, n_kv, page_size, D = shape
         token, head = st[2], st[1]
-    B, width = block_table.shape
+    else:
+        raise RuntimeError(f"layout must be 'bthd' or 'bhtd', got {layout!r}")
     return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                           block_table.stride(0) if B > 1 else width, st[0], token, head, pages, page_size, width, n_kv, D)
+                           block_table.stride(0) if ts[0] > 1 else ts[1], st[0], token, head, pages, page_size, ts[1],
+                           n_kv, D)
 
 
 def _sequences(cu_seqlens, kv_lens, block_table):
-    _cuda_contig(cu_seqlens, "cu_seqlens", torch.int32)
-    _cuda_contig(kv_lens, "kv_lens", torch.int32)
+    _dense(cu_seqlens, "cu_seqlens", torch.int32)
+    _dense(kv_lens, "kv_lens", torch.int32)
     B = kv_lens.numel()
-    _need(B >= 1 and cu_seqlens.numel() == B + 1 and block_table.shape[0] == B,
-          "cu_seqlens must have B + 1 entries, kv_lens and block_table B rows")
+    if B < 1 or cu_seqlens.numel() != B + 1 or block_table.shape[0] != B:
+        raise RuntimeError("cu_seqlens must have B + 1 entries, kv_lens and block_table B rows")
     return B
 
 
@@ -832,18 +852,17 @@ def rope_append(q, k, v, positions, inv_freq, sections, k_cache, v_cache, block_
     Tv, Hv, Dv, v_ld = _token_rows(v, "v")
     cache = _paged_cache(k_cache, v_cache, block_table, layout)
     B = _sequences(cu_seqlens, kv_lens, block_table)
-    _need(Tk == T and Tv == T and Hk == Hv == cache.n_kv and D == Dk == Dv == cache.head_dim,
-          "q, k, v must have the same tokens and the cache's heads and head dim")
+    if not (Tk == T == Tv and Hk == Hv == cache.n_kv and D == Dk == Dv == cache.head_dim):
+        raise RuntimeError("q, k, v must have the same tokens and the cache's heads and head dim")
     spec = _rope_spec(positions, inv_freq, sections, style, T)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = _like(q)
     else:
-        _cuda_contig(q_out, "q_out", torch.bfloat16)
-        _need(q_out.shape == q.shape, "q_out must have q's shape")
+        _shaped(q_out, "q_out", q.shape, torch.bfloat16)
     if T == 0:
         return q_out
-    _lib.call("gdn_rope_append", _ptr(q), q_ld, _ptr(k), k_ld, _ptr(v), v_ld, _ptr(q_out), ctypes.byref(spec),
-              ctypes.byref(cache), _ptr(cu_seqlens), _ptr(kv_lens), B, T, Hq, _stream())
+    _lib.call("gdn_rope_append", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld, q_out.data_ptr(),
+              ctypes.byref(spec), ctypes.byref(cache), cu_seqlens.data_ptr(), kv_lens.data_ptr(), B, T, Hq, _stream())
     return q_out
 
 
@@ -865,29 +884,27 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
     T, Hq, D, q_ld = _token_rows(q, "q")
     cache = _paged_cache(k_cache, v_cache, block_table, layout)
     B = _sequences(cu_seqlens, kv_lens, block_table)
-    _need(D == cache.head_dim, "q must have the cache's head dim")
+    if D != cache.head_dim:
+        raise RuntimeError("q must have the cache's head dim")
     if max_q is None:
         max_q = int((cu_seqlens[1:] - cu_seqlens[:-1]).max())
     if max_kv is None:
         max_kv = cache.max_pages * cache.page_size
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _like(q)
     else:
-        _cuda_contig(out, "out", torch.bfloat16)
-        _need(out.shape == q.shape, "out must have q's shape")
+        _shaped(out, "out", q.shape, torch.bfloat16)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0:
         return (out, lse) if return_lse else out
     ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
     if workspace is None:
-        if ws_bytes:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    else:
-        _need(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.numel() >= ws_bytes,
-              f"workspace: uint8 CUDA tensor of at least {ws_bytes} bytes required")
-    _lib.call("gdn_paged_attn_fwd", _ptr(q), q_ld, ctypes.byref(cache), _ptr(cu_seqlens), _ptr(kv_lens), _ptr(out),
-              _ptr(lse), B, T, Hq, max_q, max_kv, 1 if causal else 0, window, float(scale), _ptr(workspace),
-              ws_bytes if workspace is not None else 0, _stream())
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    elif not (workspace.is_cuda and workspace.dtype is torch.uint8 and workspace.numel() >= ws_bytes):
+        raise RuntimeError(f"workspace: uint8 CUDA tensor of at least {ws_bytes} bytes required")
+    _lib.call("gdn_paged_attn_fwd", q.data_ptr(), q_ld, ctypes.byref(cache), cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+              out.data_ptr(), _ptr(lse), B, T, Hq, max_q, max_kv, 1 if causal else 0, window, float(scale),
+              workspace.data_ptr(), ws_bytes, _stream())
     return (out, lse) if return_lse else out
 
 
