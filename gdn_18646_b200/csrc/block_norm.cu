@@ -183,8 +183,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) block_norm_fwd_kernel(c
     }
 }
 
-// The rows a backward work item covers: one of `parts` parts of one gate row's rows,
-// so the column sums of an item belong to one gate row.
+// The rows a backward work item covers: every parts-th row of one gate row's rows, so the
+// column sums of an item belong to one gate row.  CTAs side by side take rows side by
+// side (contiguous shares: 122 us instead of 118 at 16384 x 2048, fp32 stream).
 struct BwdPlan {
     int groups;                       // gate rows that are summed over rows (1 when none are)
     int parts;                        // parts per group
@@ -360,7 +361,7 @@ __device__ __forceinline__ void bwd_items(const BlockNormArgs& a, const BwdPlan&
             st.w[i] = mul2(gp[i], gt[i]);
             st.q[i] = 0;
         }
-        rows(st, gp, sum_post, g * group_rows + group_rows * part / plan.parts, g * group_rows + group_rows * (part + 1) / plan.parts);
+        rows(st, gp, sum_post, g * group_rows + part, (g + 1) * group_rows, static_cast<long>(plan.parts));
         if (!row_gate) {
             // read again: they are not kept over the rows
             weight_pairs(a.gamma_post, col, on, gp);
@@ -388,9 +389,9 @@ block_norm_bwd_narrow_kernel(const BlockNormArgs a, const BwdPlan plan, void* dg
     const int sub = threadIdx.x >> 5, col = (threadIdx.x & 31) * 8;
     const bool on = col < a.D, row_gate = dgate_rows != nullptr;
     pdl_launch_dependents();
-    auto rows = [&](BwdRow<F32, true>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1) {
+    auto rows = [&](BwdRow<F32, true>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1, long step) {
         int turn = 0;
-        for (long r = r0 + sub; r < r1; r += kNarrowRows) {
+        for (long r = r0 + sub * step; r < r1; r += kNarrowRows * step) {
             const long at = r * a.D + col;
             uint64_t y[4] = {}, h[4] = {}, dx[4] = {}, dt[4] = {}, gt[4] = {};
             if (on) {
@@ -464,10 +465,12 @@ block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, const BwdRing r
         if (a.dh_out) bulk_load(s + ring.off_dh, static_cast<const uint8_t*>(a.dh_out) + at * HB, e * HB, bar);
         if (row_gate) bulk_load(s + ring.off_gate, a.gate + at, e * 2, bar);
     };
-    auto rows = [&](BwdRow<F32, false>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1) {
-        if (tid == 0)
-            for (long r = r0; r < r1 && r < r0 + ring.stages; ++r) issue(r, used + static_cast<uint32_t>(r - r0));
-        for (long r = r0; r < r1; ++r, ++used) {
+    auto rows = [&](BwdRow<F32, false>& st, const uint64_t (&gp)[4], uint64_t (&sum_post)[4], long r0, long r1, long step) {
+        if (tid == 0) {
+            uint32_t n = used;
+            for (long r = r0; r < r1 && n < used + ring.stages; r += step) issue(r, n++);
+        }
+        for (long r = r0; r < r1; r += step, ++used) {
             const long at = r * a.D + col;
             const uint8_t* s = ring_mem + (used % ring.stages) * ring.bytes;
             // gives up with the error word set; the rows then hold anything, the walk ends as usual
@@ -485,7 +488,7 @@ block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, const BwdRing r
                 }
             }
             st.run(a, y, h, dx, dt, row_gate ? gt : nullptr, gp, sum_post, dgate_rows, dgate_f32, at, on, &red[0][0], turn, [&] {
-                if (tid == 0 && r + ring.stages < r1) issue(r + ring.stages, used + ring.stages);
+                if (tid == 0 && r + ring.stages * step < r1) issue(r + ring.stages * step, used + ring.stages);
             });
         }
     };
