@@ -85,36 +85,60 @@ template <int D, bool INTERLEAVED, bool APPEND>
 __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
     constexpr int UNITS = D / 16;              // lanes per head
     constexpr int HPW = 32 / UNITS;            // heads a warp turns at once
+    constexpr int BATCH = 3;                   // such groups of heads whose loads are in flight together
     const int lane = threadIdx.x & 31, unit = lane % UNITS, sub = lane / UNITS;
-    const long job = static_cast<long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    const int t = static_cast<int>(job / a.splits), split = static_cast<int>(job % a.splits);
+    const uint32_t job = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int t = static_cast<int>(job / a.splits), split = static_cast<int>(job - t * a.splits);
     if (t >= a.T) return;
+    const bool turn = unit * 8 < a.half;
+    // the two 16-byte pieces of this lane's unit: of a rotated unit (pieces p0, p1) and of a copied one
+    const int p0 = (turn && !INTERLEAVED) ? unit * 8 : unit * 16;
+    const int p1 = (turn && !INTERLEAVED) ? a.half + unit * 8 : unit * 16 + 8;
+    const int heads = a.Hq + a.Hk * (APPEND ? 2 : 1), step = a.splits * HPW;
+    const int h0 = split * HPW + sub;
+    uint4 w[BATCH][2];
+    auto load = [&](int h, uint4 (&x)[2]) {
+        const uint16_t* src;
+        if (h < a.Hq)
+            src = a.q + t * a.q_ld + h * D;
+        else if (h < a.Hq + a.Hk)
+            src = a.k + t * a.k_ld + (h - a.Hq) * D;
+        else
+            src = a.v + t * a.v_ld + (h - a.Hq - a.Hk) * D;
+        x[0] = __ldcg(reinterpret_cast<const uint4*>(src + p0));
+        x[1] = __ldcg(reinterpret_cast<const uint4*>(src + p1));
+    };
+    // the first heads' loads are in flight while the token's place and its angles are found
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+        if (h0 + i * step < heads) load(h0 + i * step, w[i]);
 
+    int pos[kMaxAxes] = {};
+    if (turn) {
+#pragma unroll
+        for (int x = 0; x < kMaxAxes; ++x)
+            if (x < a.axes) pos[x] = a.positions[x * a.positions_ld + t];
+    }
     // where this token's key and value go
     long slot = -1;
     if constexpr (APPEND) {
         const int b = sequence_of(a.cu, a.B, t);
         const int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.kv_lens[b];
-        const int pos = len - c1 + t;
-        const int pg = pos >> a.cache.page_shift;
-        bool ok = t >= c0 && t < c1 && c0 >= 0 && len >= 0 && pos >= 0 && pos < len && pg < a.cache.max_pages;
+        const int at = len - c1 + t;
+        const int pg = at >> a.cache.page_shift;
+        bool ok = t >= c0 && t < c1 && c0 >= 0 && len >= 0 && at >= 0 && at < len && pg < a.cache.max_pages;
         if (ok) {
             const int page = a.cache.table[b * a.cache.table_ld + pg];
             ok = page >= 0 && page < a.cache.num_pages;
-            slot = page * a.cache.page_stride + (pos & ((1 << a.cache.page_shift) - 1)) * a.cache.token_stride;
+            slot = page * a.cache.page_stride + (at & ((1 << a.cache.page_shift) - 1)) * a.cache.token_stride;
         }
         if (!ok) {
             slot = -1;
             if (lane == 0 && split == 0) atomicOr(a.err, DERR_PAGED);
         }
     }
-
-    const bool turn = unit * 8 < a.half;
     float sn[8], cs[8];
     if (turn) {
-        int pos[kMaxAxes];
-#pragma unroll
-        for (int x = 0; x < kMaxAxes; ++x) pos[x] = x < a.axes ? a.positions[x * a.positions_ld + t] : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int pair = unit * 8 + i;
@@ -125,61 +149,52 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
             sincos_of(p, __ldg(a.inv_freq + pair), a.sign, sn[i], cs[i]);
         }
     }
-    // the two 16-byte pieces of this lane's unit
-    const int e0 = (turn && !INTERLEAVED) ? unit * 8 : unit * 16;
-    const int e1 = (turn && !INTERLEAVED) ? a.half + unit * 8 : unit * 16 + 8;
-
-    const int heads = a.Hq + a.Hk * (APPEND ? 2 : 1);
-    for (int h = split * HPW + sub; h < heads; h += a.splits * HPW) {
-        const uint16_t* src;
+    auto finish = [&](int h, uint4 (&x)[2]) {
         uint16_t* dst;
-        bool rotate = turn;
         if (h < a.Hq) {
-            src = a.q + t * a.q_ld + h * D;
             dst = a.q_out + (static_cast<long>(t) * a.Hq + h) * D;
-        } else if (h < a.Hq + a.Hk) {
-            const int kh = h - a.Hq;
-            src = a.k + t * a.k_ld + kh * D;
-            if constexpr (APPEND) {
-                if (slot < 0) continue;
-                dst = a.cache.k + slot + kh * a.cache.head_stride;
-            } else {
-                dst = a.k_out + (static_cast<long>(t) * a.Hk + kh) * D;
-            }
+        } else if constexpr (!APPEND) {
+            dst = a.k_out + (static_cast<long>(t) * a.Hk + (h - a.Hq)) * D;
         } else {
-            if (slot < 0) continue;
-            const int vh = h - a.Hq - a.Hk;
-            src = a.v + t * a.v_ld + vh * D;
-            dst = a.cache.v + slot + vh * a.cache.head_stride;
-            rotate = false;
+            if (slot < 0) return;
+            dst = h < a.Hq + a.Hk ? a.cache.k + slot + (h - a.Hq) * a.cache.head_stride
+                                  : a.cache.v + slot + (h - a.Hq - a.Hk) * a.cache.head_stride;
         }
-        uint4 w0 = __ldcg(reinterpret_cast<const uint4*>(src + e0)), w1 = __ldcg(reinterpret_cast<const uint4*>(src + e1));
-        if (rotate) {
+        if (turn && h < a.Hq + a.Hk) {
             float x0[8], x1[8];
-            unpack8(w0, x0);
-            unpack8(w1, x1);
+            unpack8(x[0], x0);
+            unpack8(x[1], x1);
             if constexpr (INTERLEAVED) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = x0[2 * i], q = x0[2 * i + 1], r = x1[2 * i], s = x1[2 * i + 1];
-                    x0[2 * i] = p * cs[i] - q * sn[i];
-                    x0[2 * i + 1] = q * cs[i] + p * sn[i];
-                    x1[2 * i] = r * cs[i + 4] - s * sn[i + 4];
-                    x1[2 * i + 1] = s * cs[i + 4] + r * sn[i + 4];
+                    const float e = x0[2 * i], f = x0[2 * i + 1], g = x1[2 * i], k = x1[2 * i + 1];
+                    x0[2 * i] = e * cs[i] - f * sn[i];
+                    x0[2 * i + 1] = f * cs[i] + e * sn[i];
+                    x1[2 * i] = g * cs[i + 4] - k * sn[i + 4];
+                    x1[2 * i + 1] = k * cs[i + 4] + g * sn[i + 4];
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float p = x0[i], q = x1[i];
-                    x0[i] = p * cs[i] - q * sn[i];
-                    x1[i] = q * cs[i] + p * sn[i];
+                    const float e = x0[i], f = x1[i];
+                    x0[i] = e * cs[i] - f * sn[i];
+                    x1[i] = f * cs[i] + e * sn[i];
                 }
             }
-            w0 = pack8(x0);
-            w1 = pack8(x1);
+            x[0] = pack8(x0);
+            x[1] = pack8(x1);
         }
-        *reinterpret_cast<uint4*>(dst + e0) = w0;
-        *reinterpret_cast<uint4*>(dst + e1) = w1;
+        *reinterpret_cast<uint4*>(dst + p0) = x[0];
+        *reinterpret_cast<uint4*>(dst + p1) = x[1];
+    };
+    for (int h = h0; h < heads; h += BATCH * step) {
+        if (h != h0)
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (h + i * step < heads) load(h + i * step, w[i]);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (h + i * step < heads) finish(h + i * step, w[i]);
     }
 }
 
