@@ -169,6 +169,14 @@ struct Seq {
     __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
         if (q == 0) return 0;
         long long s = static_cast<long long>(q) * a.item_cost;
+        if (q <= 6) {                                           // as they are: the closed form costs as much as six
+            for (int i = 0; i < q; ++i) {
+                int first, count, lo, hi;
+                tiles(a, i, tt, first, count, lo, hi);
+                s += count;
+            }
+            return s;
+        }
         const int full = (kv + kTile - 1) / kTile;
         if (!a.causal) return s + static_cast<long long>(q) * full;
         const int p = kv - n;
@@ -627,7 +635,6 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 if (busy) {
                     const uint32_t s_col = tmem + lanes + buf * kTile;
                     const int j0 = (w.first + j) * kTile;
-                    const bool masked = j0 + kTile > hi_first || j0 < lo_last;
                     float s[kTile];
                     auto load_s = [&]() {
 #pragma unroll
@@ -684,36 +691,30 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     const float mc = m == -INFINITY ? 0.f : m * c;
                     const uint64_t c2 = pack2(c, c), mc2 = pack2(-mc, -mc);
                     uint64_t sum[4] = {0, 0, 0, 0};
-                    auto weights = [&](auto mixed) {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t p[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t p[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float x0, x1;
-                                unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), c2, mc2), x0, x1);
-                                if (decltype(mixed)::value && (i % kPolyOf) < kPolyPairs) {
-                                    exp2_poly2(x0, x1);
-                                } else {
-                                    x0 = ex2_approx(x0);
-                                    x1 = ex2_approx(x1);
-                                }
-                                sum[i & 3] = add2(sum[i & 3], pack2(x0, x1));
-                                p[i] = cvt_bf16x2(x0, x1);
+                        for (int i = 0; i < 16; ++i) {
+                            float x0, x1;
+                            unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), c2, mc2), x0, x1);
+                            if (QT == 2 && (i % kPolyOf) < kPolyPairs) {
+                                exp2_poly2(x0, x1);
+                            } else {
+                                x0 = ex2_approx(x0);
+                                x1 = ex2_approx(x1);
                             }
-                            tmem_st16(s_col + q * 16, p);
-                            if (q == kEarly - 1) {               // the first part of P V may start
-                                tmem_st_wait();
-                                tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(&sh->p_part[buf]);
-                            }
+                            sum[i & 3] = add2(sum[i & 3], pack2(x0, x1));
+                            p[i] = cvt_bf16x2(x0, x1);
                         }
-                    };
-                    if (QT == 2 && !masked)
-                        weights(std::true_type{});
-                    else
-                        weights(std::false_type{});
+                        tmem_st16(s_col + q * 16, p);
+                        if (q == kEarly - 1) {                   // the first part of P V may start
+                            tmem_st_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh->p_part[buf]);
+                        }
+                    }
                     float l0, l1;
                     unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
                     l += l0 + l1;
@@ -731,6 +732,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             if (!warp_wait(&sh->o_full[t], items & 1u, a.err, dead)) break;
             ++items;
             tc_fence_after();
+            if (m == -INFINITY) l = 0.f;                                // saw nothing (the polynomial gives 2^-125 for 2^-inf)
             if (busy) {
                 const bool whole = w.t0 == 0 && w.t1 == w.count;
                 if (whole) {
@@ -815,24 +817,23 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     }
 }
 
-// Joins the parts of the items that pieces cut: block (x, y, z) takes the item that CTA x
-// began and did not finish, rows 32 y .. 32 y + 31 (a lane each, as the parts lie in memory)
-// and 32 V columns (a warp takes V float4).  All loads of a thread are independent of one
-// another but for the first, of the states.  V = 1 spreads the columns of few rows with
-// many parts over blocks; more blocks than that cost more to start than they save (4 us
-// for 4 x as many at one short sequence).
-template <int D, int QT, int V>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+// Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
+// began and did not finish.  A warp takes 32 rows (a lane each, as the parts lie in
+// memory) and V float4 of the columns, SLICES groups of rows to a block.  All loads of a
+// batch are independent of one another; one wave of blocks (each starts with a wait for the states).
+template <int D, int QT, int SLICES, int V>
+__global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
     pdl_wait_prior();
     const int rows = a.part_rows;
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slice = warp % SLICES, colg = (blockIdx.y * (blockDim.x >> 5) + warp) / SLICES;   // its column group
     // the states of this CTA and of the 31 after it in one go
     const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
     const int head = __ldcg(a.part_state + x * 8 + 4);
     int st = x + 1 + lane < ctas ? __ldcg(a.part_state + (x + 1 + lane) * 8) : 0;
     if (mine.y == 0) return;
     const int tok0 = mine.z, toks = mine.w;
-    const int row = blockIdx.y * 32 + lane, r = row & 127;
+    const int row = slice * 32 + lane, r = row & 127;
     const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
     const bool real = tl < a.tile_tokens && tok < toks;
     int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
@@ -852,54 +853,57 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const __grid_const
     // part 0 is CTA x's slot 1, part p the slot 0 of CTA x + p
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (static_cast<long>(x) * 2) * rows + row;
     const float4* po = reinterpret_cast<const float4*>(a.part_o) +
-                       (static_cast<long>(x) * 2 * (D / 4) + (blockIdx.z * 8 + warp) * V) * rows + row;
+                       (static_cast<long>(x) * 2 * (D / 4) + colg * V) * rows + row;
     auto slot = [](int p) { return p == 0 ? 1 : 2 * p; };
+    const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
     // one pass with a running maximum; loads in batches under a predicate (a remainder loop
-    // would wait for each of them)
-    constexpr int N = V == 1 ? 16 : 4;
-    float m = -INFINITY, l = 0.f;
-    float4 o[V];
+    // would wait for each of them), four columns' float4 at a time
+    constexpr int C = V < 4 ? V : 4, N = V == 1 ? 8 : 2;
+#pragma unroll 1
+    for (int c0 = 0; c0 < V; c0 += C) {
+        float m = -INFINITY, l = 0.f;
+        float4 o[C];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < parts; p0 += N) {
-        float2 v[N];
-        float4 u[N][V];
-        float mn = m;
+        for (int i = 0; i < C; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < parts; p0 += N) {
+            float2 v[N];
+            float4 u[N][C];
+            float mn = m;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            v[k] = p0 + k < parts ? __ldcg(ml + slot(p0 + k) * rows) : make_float2(0.f, 0.f);
+            for (int k = 0; k < N; ++k) {
+                v[k] = p0 + k < parts ? __ldcg(ml + slot(p0 + k) * rows) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                u[k][i] = p0 + k < parts ? __ldcg(po + (static_cast<long>(slot(p0 + k)) * (D / 4) + i) * rows)
-                                         : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+                for (int i = 0; i < C; ++i)
+                    u[k][i] = p0 + k < parts ? __ldcg(po + (static_cast<long>(slot(p0 + k)) * (D / 4) + c0 + i) * rows)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
-        for (int k = 0; k < N; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
-        const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
-        m = mn;
-        l *= keep;
+            for (int k = 0; k < N; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
+            const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
+            m = mn;
+            l *= keep;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
-        }
+            for (int i = 0; i < C; ++i) {
+                o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
+            }
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const float w = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
-            l += v[k].y * w;
+            for (int k = 0; k < N; ++k) {
+                const float w = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
+                l += v[k].y * w;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                o[i].x += u[k][i].x * w; o[i].y += u[k][i].y * w; o[i].z += u[k][i].z * w; o[i].w += u[k][i].w * w;
+                for (int i = 0; i < C; ++i) {
+                    o[i].x += u[k][i].x * w; o[i].y += u[k][i].y * w; o[i].z += u[k][i].z * w; o[i].w += u[k][i].w * w;
+                }
             }
         }
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
-    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + (blockIdx.z * 8 + warp) * V;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + colg * V + c0;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        dst[i] = l == 0.f ? make_uint2(0u, 0u)
-                          : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
-    if (a.lse && warp == 0 && blockIdx.z == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+        for (int i = 0; i < C; ++i)
+            dst[i] = l == 0.f ? make_uint2(0u, 0u)
+                              : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
+        if (a.lse && colg == 0 && c0 == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    }
 }
 
 size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
@@ -934,13 +938,16 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    const int rows = min(a.max_q, QT * a.tile_tokens) * a.group, slices = QT == 2 ? 8 : max((rows + 31) / 32, 1);
-    cfg.gridDim = dim3(kMaxCtas, slices, slices == 1 ? D / 32 : 1);
-    cfg.blockDim = dim3(256);
+    // few rows (a decode step): a block per 16 or 8 float4 columns, one each; else all rows of
+    // the item in a block, a quarter of the columns
+    const int slices = QT == 2 ? 8 : (a.part_rows + 31) / 32;
+    constexpr int V = D / 16;
+    cfg.gridDim = dim3(kMaxCtas, slices == 1 ? 2 : QT == 2 ? 2 : 1);
+    cfg.blockDim = dim3(slices == 1 ? D * 4 : 512);
     cfg.stream = st;
-    void (*join)(AttnArgs, int) = paged_attn_join_kernel<D, QT, D / 32>;
+    void (*join)(AttnArgs, int) = paged_attn_join_kernel<D, QT, QT * 4, V>;
     if constexpr (QT == 1)
-        if (slices == 1) join = paged_attn_join_kernel<D, QT, 1>;
+        if (slices == 1) join = paged_attn_join_kernel<D, QT, 1, 1>;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a, static_cast<int>(kMaxCtas));
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
     return launch_status(name);
