@@ -12,7 +12,7 @@
 // (row = token G + g), floor(128 / G) tokens to a tile of 128, so a decode step and a
 // chunk run the same kernel and a key is read once for its whole group.
 //
-// Work.  An item is (sequence, kv head, QT row tiles); its kv tiles are the ones that some
+// Work.  An item is (sequence, kv head, two row tiles); its kv tiles are the ones that some
 // row of it sees.  All kv tiles of all items, with a constant cost per item, form one line
 // that is cut into equal pieces, one per CTA: a long sequence is split over many CTAs and a
 // CTA may take many short ones.  An item cut by a piece's end leaves its o, m, l in the
@@ -25,49 +25,22 @@
 //   S = Q K^T   M 128, N 128 (SS)      -> TMEM, 128 columns per S buffer
 //   P (bf16) overwrites S in TMEM      (rounded to bf16: 2^-9 rms of each weight)
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
-// With two row tiles the tensor core works for one while the softmax of the other runs;
-// with one row tile (at most 128 rows, the decode step) S is double buffered instead.
+// The tensor core works for one row tile while the softmax of the other runs.  Items of
+// at most 64 rows (a decode step) go to paged_attn_rows.cu.
 #include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
-#include "paged.cuh"
+#include "paged_work.cuh"
 #include "tensormap.h"
 
 namespace gdn {
 namespace {
 
-constexpr int kTile = 128;            // positions per kv tile; rows per row tile
-constexpr int kMaxCtas = 148;         // pieces of the work line: one CTA per SM of a B200
-// kv tiles that starting and ending an item is worth, beside the tiles themselves
-__host__ __device__ constexpr int item_cost(int qt) { return qt == 2 ? 2 : 1; }
+constexpr int QT = 2;                 // row tiles of 128 per item
+constexpr int kItemCost = 2;          // kv tiles that starting and ending an item is worth, beside its tiles
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
 constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
-constexpr int kMinPiece = 4;          // shortest piece: splitting finer costs more to join
-
-struct AttnArgs {
-    uint16_t* out;
-    float* lse;
-    const int* cu;
-    const int* kv_lens;
-    const int* table;
-    long table_ld;
-    int num_pages, page_shift;
-    int B, T, Hq, n_kv, group;        // group: query heads per kv head
-    int tile_tokens;                  // floor(128 / group)
-    int max_q, max_kv, causal, window;
-    float scale;
-    int item_cost;
-    unsigned int* err;
-    int* part_state;                  // [ctas][8]: what a CTA left unfinished
-    int part_rows;                    // rows of a part
-    float* part_ml;                   // [ctas][2][part_rows][2]: m, l
-    float* part_o;                    // [ctas][2][D / 4][part_rows][4]
-};
-
-struct alignas(64) AttnMaps {
-    CUtensorMap q, k, v;
-};
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -97,154 +70,7 @@ __device__ __forceinline__ void exp2_poly2(float& x0, float& x1) {
     x1 = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
 }
 
-// sum over i in [0, n) of floor((a i + b) / 128) for a <= 256 (the Euclid-like reduction);
-// after the first reduction every operand is small, so the divisions are 32-bit
-__device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
-    uint32_t m = kTile;
-    long long s = 0;
-    while (n > 0) {
-        const uint32_t qa = a / m, qb = b / m;
-        s += static_cast<long long>(n - 1) * n / 2 * qa + static_cast<long long>(n) * qb;
-        a -= qa * m;
-        b -= qb * m;
-        const uint32_t y = a * n + b;                           // a < 128, n <= 2^24
-        if (y < m) break;
-        n = y / m;
-        b = y - n * m;
-        const uint32_t t = m;
-        m = a;
-        a = t;
-    }
-    return s;
-}
-
-// One lane of the warp, the same one every time.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e != 0;
-}
-// lane 0's value: tells the compiler that it is the same in the whole warp, so that MMA
-// descriptors built from it stay in uniform registers
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-// sdesc_sw128 from its low word
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
-    return static_cast<uint64_t>(kDescHi) << 32 | lo;
-}
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3FFFFu) >> 4) | (lbo_bytes >> 4) << 16; }
-
-// A wait that all lanes of a warp leave alike, also when it gives up.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* dead) {
-    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, dead));
-}
-
-// One sequence as the kernel sees it; tt: tokens per item.
-struct Seq {
-    int c0, n, kv, items;             // first packed token, new tokens, positions, row-tile groups
-    __device__ __forceinline__ void load(const AttnArgs& a, int b, int tt, bool report) {
-        c0 = a.cu[b];
-        const int c1 = a.cu[b + 1];
-        kv = a.kv_lens[b];
-        n = c1 - c0;
-        if (c0 < 0 || c1 > a.T || n < 0 || n > a.max_q || kv < 0 || kv > a.max_kv) {
-            if (report) atomicOr(a.err, DERR_PAGED);
-            c0 = n = kv = 0;
-        }
-        items = (n + tt - 1) / tt;
-    }
-    // positions [lo, hi) that tokens first .. last of the chunk see between them
-    __device__ __forceinline__ void range(const AttnArgs& a, int first, int last, int& lo, int& hi) const {
-        const int p = kv - n;
-        hi = a.causal ? max(0, min(p + last + 1, kv)) : kv;
-        lo = a.window > 0 ? max(0, p + first + 1 - a.window) : 0;
-        if (hi <= lo) lo = hi = 0;
-    }
-    __device__ __forceinline__ void tiles(const AttnArgs& a, int item, int tt, int& first, int& count, int& lo, int& hi) const {
-        range(a, item * tt, min((item + 1) * tt, n) - 1, lo, hi);
-        first = lo / kTile;
-        count = hi > 0 ? (hi + kTile - 1) / kTile - first : 0;
-    }
-    // cost of the items before `q` of one kv head
-    __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
-        if (q == 0) return 0;
-        long long s = static_cast<long long>(q) * a.item_cost;
-        if (q <= 6) {                                           // as they are: the closed form costs as much as six
-            for (int i = 0; i < q; ++i) {
-                int first, count, lo, hi;
-                tiles(a, i, tt, first, count, lo, hi);
-                s += count;
-            }
-            return s;
-        }
-        const int full = (kv + kTile - 1) / kTile;
-        if (!a.causal) return s + static_cast<long long>(q) * full;
-        const int p = kv - n;
-        const int m = min(q, items - 1);
-        const int i0 = p + tt > 0 ? 0 : (-p) / tt;              // first item with p + (i + 1) tt > 0
-        if (i0 < m) s += floor_sum(m - i0, tt, p + (i0 + 1) * tt + kTile - 1);
-        if (q == items) s += full;
-        if (a.window > 0) {
-            const int w = p + 1 - a.window;                     // lo of item i: max(0, w + i tt)
-            const int i1 = w >= 0 ? 0 : (-w + tt - 1) / tt;
-            if (i1 < q) s -= floor_sum(q - i1, tt, w + i1 * tt);
-        }
-        return s;
-    }
-};
-
-// Where a CTA's piece of the work line starts, and its length.
-struct Piece {
-    Seq s;
-    int b, head, item;
-    int skip;                         // units of the first item that belong to earlier CTAs
-    long long units;
-};
-
-// Walks the items of a piece; every role of the CTA does so on its own.
-struct Walk {
-    Seq s;
-    int b, head, item, skip;
-    long long left;
-    int first, count, lo, hi;         // the item's kv tiles and positions
-    int t0, t1;                       // this CTA's part of its tiles: [t0, t1) of [0, count)
-    __device__ __forceinline__ void start(const AttnArgs& a, const Piece& p, int tt) {
-        b = p.b;
-        head = p.head;
-        item = p.item;
-        skip = p.skip;
-        left = p.units;
-        if (left > 0) {
-            s = p.s;
-            set(a, tt);
-        }
-    }
-    __device__ __forceinline__ bool valid() const { return left > 0; }
-    __device__ __forceinline__ void set(const AttnArgs& a, int tt) {
-        s.tiles(a, item, tt, first, count, lo, hi);
-        const long long end = min(static_cast<long long>(count + a.item_cost), skip + left);
-        t0 = max(skip - a.item_cost, 0);
-        t1 = max(static_cast<int>(end) - a.item_cost, 0);
-    }
-    __device__ __forceinline__ void next(const AttnArgs& a, int tt) {
-        left -= count + a.item_cost - skip;
-        skip = 0;
-        if (left <= 0) return;
-        if (++item == s.items) {
-            item = 0;
-            if (++head == a.n_kv) {
-                head = 0;
-                do {
-                    ++b;
-                    s.load(a, b, tt, false);
-                } while (s.items == 0);
-            }
-        }
-        set(a, tt);
-    }
-};
-
-template <int D, int QT>
+template <int D>
 struct Shape {
     static constexpr int HALVES = D / 64;
     static constexpr int Q_BYTES = QT * kTile * D * 2;
@@ -269,90 +95,16 @@ struct Bars {
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_part[2], p_full[2];
     uint64_t o_full[2];
-    uint64_t pv_done;
-    Piece piece;
-    long long scan[16];
-    long long total;
+    PieceScratch scratch;
     uint32_t tmem;
     int abort;
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
 
-// This CTA's piece: a thread sums the costs of its share of the sequences, a scan over the
-// threads finds the sequence in which the piece starts, and all threads together the item in it.
-__device__ __forceinline__ void find_piece(const AttnArgs& a, Bars* sh, int tt) {
-    const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, nw = nt >> 5;
-    if (tid == 0) sh->piece.units = 0;
-    const int each = (a.B + nt - 1) / nt, b0 = tid * each, b1 = min(b0 + each, a.B);
-    long long mine = 0, u = 0;
-    Seq s = {};
-#pragma unroll 4
-    for (int b = b0; b < b1; ++b) {
-        s.load(a, b, tt, blockIdx.x == 0);
-        u = s.cost(a, s.items, tt);
-        mine += u * a.n_kv;
-    }
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) sh->scan[warp] = inc;
-    __syncthreads();
-    long long start = inc - mine, total = 0;
-    for (int w = 0; w < nw; ++w) {
-        const long long v = sh->scan[w];
-        if (w < warp) start += v;
-        total += v;
-    }
-    const long long most = (total + kMinPiece - 1) / kMinPiece;
-    const int pieces = most < gridDim.x ? static_cast<int>(most) : gridDim.x;
-    if (blockIdx.x < pieces) {
-        // total x / pieces without a wide product
-        const long long q = total / pieces;
-        const int r = static_cast<int>(total - q * pieces), x = blockIdx.x;
-        const long long from = q * x + r * x / pieces, to = q * (x + 1) + r * (x + 1) / pieces;
-        if (from >= start && from < start + mine) {
-            int b = b0;
-            if (each > 1) {
-                for (;; ++b) {
-                    s.load(a, b, tt, false);
-                    u = s.cost(a, s.items, tt);
-                    if (from < start + u * a.n_kv) break;
-                    start += u * a.n_kv;
-                }
-            }
-            const long long off = from - start;
-            Piece& p = sh->piece;
-            p.s = s;
-            p.b = b;
-            p.head = static_cast<int>(off / u);
-            p.item = 0;
-            p.skip = static_cast<int>(off - p.head * u);        // within the head, so far
-            p.units = to - from;
-        }
-    }
-    __syncthreads();
-    if (sh->piece.units == 0) return;
-    s = sh->piece.s;
-    const int off = sh->piece.skip;
-    if (s.items == 1) return;
-    __syncthreads();
-    for (int i = tid; i < s.items; i += nt) {
-        const long long c0 = s.cost(a, i, tt);
-        if (c0 <= off && off < s.cost(a, i + 1, tt)) {
-            sh->piece.item = i;
-            sh->piece.skip = off - static_cast<int>(c0);
-        }
-    }
-    __syncthreads();
-}
-
-template <int D, int QT>
-__global__ void __launch_bounds__(Shape<D, QT>::THREADS, 1)
+template <int D>
+__global__ void __launch_bounds__(Shape<D>::THREADS, 1)
 paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
-    using S = Shape<D, QT>;
+    using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Bars* sh = reinterpret_cast<Bars*>(sm + S::OFF_BAR);
@@ -375,7 +127,6 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             mbar_init(&sh->p_full[i], 4);
             mbar_init(&sh->o_full[i], 1);
         }
-        mbar_init(&sh->pv_done, 1);
         sh->abort = 0;
         fence_mbar_init();
         tma_prefetch_desc(&maps.q);
@@ -388,20 +139,16 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     }
     pdl_launch_dependents();
     pdl_wait_prior();                                           // q, the cache and the lengths come from earlier kernels
-    find_piece(a, sh, tt);
+    find_piece(a, &sh->scratch, tt);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh->tmem;
-    const Piece piece = sh->piece;
+    const Piece piece = sh->scratch.piece;
 
     uint32_t q_loads = 0, issued = 0;                           // of the producer
     if (warp == LOAD_WARP) {
-        // ---------------- TMA producer: a lane per (page of the tile, 64-value half)
-        const int page_rows = min(1 << a.page_shift, kTile);
-        const int pages_per_tile = kTile / page_rows;
-        const int units = pages_per_tile * S::HALVES;           // <= 16
-        const int my_page = lane / S::HALVES, my_half = lane % S::HALVES;
+        // ---------------- TMA producer
         int stage = 0;
         uint32_t phase = 0;
         Walk w;
@@ -417,41 +164,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         tma_load_3d(sm + (t * S::HALVES + h) * 16384, &maps.q, &sh->q_full, h * 64, w.head * a.group,
                                     w.s.c0 + w.item * tt + t * a.tile_tokens);
             }
-            const int* row = a.table + w.b * a.table_ld;
-            bool stop = false;
-            for (int j = w.t0; j < w.t1 && !stop; ++j) {
-                const int j0 = (w.first + j) * kTile;
-                // pages of this tile that hold a position somebody sees
-                const int pos = j0 + my_page * page_rows;
-                const bool mine = lane < units && pos + page_rows > w.lo && pos < w.hi;
-                int page = 0;
-                if (mine) {
-                    page = row[pos >> a.page_shift];
-                    if (page < 0 || page >= a.num_pages) {
-                        page = a.num_pages;                     // outside: the copy fills zeros
-                        atomicOr(a.err, DERR_PAGED);
-                    }
-                }
-                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * page_rows * 128;
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (!warp_wait(&sh->empty[stage], phase ^ 1u, a.err, dead)) {
-                        stop = true;
-                        break;
-                    }
-                    if (lane == 0) mbar_arrive_expect_tx(&sh->full[stage], bytes);
-                    __syncwarp();
-                    if (mine)
-                        tma_load_4d(sm + S::OFF_KV + stage * S::STAGE + my_half * 16384 + my_page * page_rows * 128,
-                                    kv ? &maps.v : &maps.k, &sh->full[stage], my_half * 64,
-                                    pos & ((1 << a.page_shift) - 1), w.head, page);
-                    ++issued;
-                    if (++stage == S::STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-            }
-            if (stop) break;
+            if (!load_tiles<D, S::STAGES>(a, maps, w, sm + S::OFF_KV, sh->full, sh->empty, stage, phase, issued, dead)) break;
         }
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer (one lane; the warp together clears unseen value rows)
@@ -583,7 +296,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     tc_fence_after();
                     mma_o(0, done & 1u, vst, j > 0, second_part);
                     commit(&sh->empty[vst]);
-                    commit(&sh->pv_done);
+                    
                     if (j + 1 == n) commit(&sh->o_full[0]);
                     ++done;
                 }
@@ -592,7 +305,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         }
     } else {
         // ---------------- softmax and epilogue: a thread per row
-        const int t = QT == 2 ? warp >> 2 : 0;                  // row tile
+        const int t = warp >> 2;                                // row tile
         const int row = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const int tok = row / a.group, g = row - tok * a.group; // token within the row tile, head within the group
@@ -618,6 +331,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 }
                 continue;
             }
+                  // no token in this row tile
             int lo, hi, dummy, hi_first, lo_last;
             w.s.range(a, rel, rel, lo, hi);
             w.s.range(a, first_tok, first_tok, dummy, hi_first);
@@ -625,15 +339,13 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             float m = -INFINITY, l = 0.f;
             bool stop = false;
             for (int j = w.t0; j < w.t1; ++j) {
-                const int buf = QT == 2 ? t : static_cast<int>(done & 1u);
-                const uint32_t ph = QT == 2 ? (done & 1u) : ((done >> 1) & 1u);
-                if (!warp_wait(&sh->s_full[buf], ph, a.err, dead)) {
+                if (!warp_wait(&sh->s_full[t], done & 1u, a.err, dead)) {
                     stop = true;
                     break;
                 }
                 tc_fence_after();
                 if (busy) {
-                    const uint32_t s_col = tmem + lanes + buf * kTile;
+                    const uint32_t s_col = tmem + lanes + t * kTile;
                     const int j0 = (w.first + j) * kTile;
                     float s[kTile];
                     auto load_s = [&]() {
@@ -669,14 +381,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         const float r = grow ? ex2_approx((m - mx) * c) : 1.f;
                         if (grow) m = mx;
                         l *= r;
-                        // O is at rest: with two row tiles S(j) was issued after P V(j - 1); with one, wait
-                        if constexpr (QT == 1) {
-                            if (!warp_wait(&sh->pv_done, (done - 1) & 1u, a.err, dead)) {
-                                stop = true;
-                                break;
-                            }
-                            tc_fence_after();
-                        }
+                        // O is at rest: S(j) was issued after P V(j - 1)
 #pragma unroll
                         for (int q = 0; q < D / 32; ++q) {
                             float o[32];
@@ -698,7 +403,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         for (int i = 0; i < 16; ++i) {
                             float x0, x1;
                             unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), c2, mc2), x0, x1);
-                            if (QT == 2 && (i % kPolyOf) < kPolyPairs) {
+                            if ((i % kPolyOf) < kPolyPairs) {
                                 exp2_poly2(x0, x1);
                             } else {
                                 x0 = ex2_approx(x0);
@@ -712,7 +417,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                             tmem_st_wait();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(&sh->p_part[buf]);
+                            if (lane == 0) mbar_arrive(&sh->p_part[t]);
                         }
                     }
                     float l0, l1;
@@ -721,11 +426,11 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     tmem_st_wait();
                 } else {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->p_part[buf]);
+                    if (lane == 0) mbar_arrive(&sh->p_part[t]);
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->p_full[buf]);
+                if (lane == 0) mbar_arrive(&sh->p_full[t]);
                 ++done;
             }
             if (stop) break;
@@ -806,9 +511,8 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     }
     tc_fence_before();
     __syncthreads();
-    if (sh->abort && warp == LOAD_WARP) {                       // gave up: let the copies in flight land
-        for (uint32_t i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
-            mbar_wait(&sh->full[i % S::STAGES], (i / S::STAGES) & 1u, a.err);
+    if (sh->abort && warp == LOAD_WARP) {
+        drain_ring(a, sh->full, S::STAGES, issued);
         if (q_loads > 0) mbar_wait(&sh->q_full, (q_loads - 1) & 1u, a.err);
     }
     if (warp == MMA_WARP) {
@@ -819,14 +523,15 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
 
 // Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
 // began and did not finish.  A warp takes 32 rows (a lane each, as the parts lie in
-// memory) and V float4 of the columns, SLICES groups of rows to a block.  All loads of a
-// batch are independent of one another; one wave of blocks (each starts with a wait for the states).
-template <int D, int QT, int SLICES, int V>
+// memory) and a quarter of the columns.  All loads of a batch are independent of one
+// another; one wave of blocks (each starts with a wait for the states).
+template <int D>
 __global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
     pdl_wait_prior();
     const int rows = a.part_rows;
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int slice = warp % SLICES, colg = (blockIdx.y * (blockDim.x >> 5) + warp) / SLICES;   // its column group
+    constexpr int V = D / 16;                                   // float4 of a quarter row
+    const int slice = warp & 7, colg = (blockIdx.y * 16 + warp) >> 3;
     // the states of this CTA and of the 31 after it in one go
     const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
     const int head = __ldcg(a.part_state + x * 8 + 4);
@@ -858,7 +563,7 @@ __global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_co
     const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
     // one pass with a running maximum; loads in batches under a predicate (a remainder loop
     // would wait for each of them), four columns' float4 at a time
-    constexpr int C = V < 4 ? V : 4, N = V == 1 ? 8 : 2;
+    constexpr int C = 4, N = 2;
 #pragma unroll 1
     for (int c0 = 0; c0 < V; c0 += C) {
         float m = -INFINITY, l = 0.f;
@@ -906,30 +611,31 @@ __global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_co
     }
 }
 
-size_t state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * sizeof(int); }
-size_t ml_bytes(int rows) { return static_cast<size_t>(kMaxCtas) * 2 * rows * 2 * sizeof(float); }
-size_t o_bytes(int rows, int D) { return static_cast<size_t>(kMaxCtas) * 2 * rows * D * sizeof(float); }
+// Kernel by the rows (tokens x heads of a group) of the longest chunk: up to 64 the one for
+// few rows, which keeps them in the MMA's narrow dimension; else the one with 128-row tiles
+// (a chunk of 8 tokens of 8 heads over 32768 positions: 45 us there, 97 us here).
+bool few_rows(int max_q, int group) { return static_cast<long>(max_q) * group <= 64; }
 
-// One row tile per item when the longest chunk's rows fit one, else two.
-int row_tiles(int max_q, int group) { return static_cast<long>(max_q) <= 128 / group ? 1 : 2; }
-// Rows of an unfinished item's part: both row tiles, or the rows that the longest chunk has
-// (compact, so that the parts of a decode step lie close together).
-int part_rows(int max_q, int group) { return row_tiles(max_q, group) == 2 ? 256 : max((max_q * group + 7) / 8 * 8, 8); }
+// Rows of an unfinished item's part.
+int part_rows(int max_q, int group) {
+    const int rows = (max_q > 1 ? max_q : 1) * group;
+    return !few_rows(max_q, group) ? QT * 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
 
-template <int D, int QT>
+template <int D>
 int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
-    using S = Shape<D, QT>;
+    using S = Shape<D>;
     const char* name = "gdn_paged_attn_fwd";
     static std::once_flag once[64];                             // once per device
     static cudaError_t attr[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(GDN_ERR_CUDA, "%s: no current device", name);
     std::call_once(once[dev], [dev] {
-        attr[dev] = cudaFuncSetAttribute(paged_attn_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        attr[dev] = cudaFuncSetAttribute(paged_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     });
     if (attr[dev] != cudaSuccess)
         return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr[dev]));
-    paged_attn_kernel<D, QT><<<kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
+    paged_attn_kernel<D><<<kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
     int rc = launch_status(name);
     if (rc != GDN_OK) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -938,17 +644,10 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    // few rows (a decode step): a block per 16 or 8 float4 columns, one each; else all rows of
-    // the item in a block, a quarter of the columns
-    const int slices = QT == 2 ? 8 : (a.part_rows + 31) / 32;
-    constexpr int V = D / 16;
-    cfg.gridDim = dim3(kMaxCtas, slices == 1 ? 2 : QT == 2 ? 2 : 1);
-    cfg.blockDim = dim3(slices == 1 ? D * 4 : 512);
+    cfg.gridDim = dim3(kMaxCtas, 2);
+    cfg.blockDim = dim3(512);
     cfg.stream = st;
-    void (*join)(AttnArgs, int) = paged_attn_join_kernel<D, QT, QT * 4, V>;
-    if constexpr (QT == 1)
-        if (slices == 1) join = paged_attn_join_kernel<D, QT, 1, 1>;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a, static_cast<int>(kMaxCtas));
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, a, static_cast<int>(kMaxCtas));
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
     return launch_status(name);
 }
@@ -964,7 +663,7 @@ extern "C" size_t gdn_paged_attn_workspace_bytes(int B, int Ttot, int Hq, int n_
         (head_dim != 64 && head_dim != 128))
         return 0;
     const int rows = part_rows(max_q, Hq / n_kv);
-    return state_bytes() + ml_bytes(rows) + o_bytes(rows, head_dim);
+    return part_state_bytes() + part_ml_bytes(rows) + part_o_bytes(rows, head_dim);
 }
 
 extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cache* cache, const int* cu_seqlens,
@@ -1012,20 +711,20 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.Hq = Hq;
     a.n_kv = pv.n_kv;
     a.group = Hq / pv.n_kv;
-    a.tile_tokens = kTile / a.group;
+    const bool few = few_rows(max_q, a.group);
+    a.part_rows = part_rows(max_q, a.group);
+    a.tile_tokens = (few ? a.part_rows : 128) / a.group;
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.causal = causal != 0;
     a.window = window;
     a.scale = scale == 0.f ? 1.f / sqrtf(static_cast<float>(D)) : scale;
     a.err = device_error_word();
-    const int qt = row_tiles(max_q, a.group);
-    a.item_cost = item_cost(qt);
-    a.part_rows = part_rows(max_q, a.group);
+    a.item_cost = few ? 1 : kItemCost;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_state = reinterpret_cast<int*>(ws);
-    a.part_ml = reinterpret_cast<float*>(ws + state_bytes());
-    a.part_o = reinterpret_cast<float*>(ws + state_bytes() + ml_bytes(a.part_rows));
+    a.part_ml = reinterpret_cast<float*>(ws + part_state_bytes());
+    a.part_o = reinterpret_cast<float*>(ws + part_state_bytes() + part_ml_bytes(a.part_rows));
 
     AttnMaps maps;
     {
@@ -1045,6 +744,6 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
         if ((st = make_map_bf16(&maps.v, pv.v, 4, dims, strides, box, true)) != GDN_OK) return st;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (D == 64) return qt == 1 ? launch<64, 1>(maps, a, s) : launch<64, 2>(maps, a, s);
-    return qt == 1 ? launch<128, 1>(maps, a, s) : launch<128, 2>(maps, a, s);
+    if (few) return launch_attn_rows(maps, a, D, s);
+    return D == 64 ? launch<64>(maps, a, s) : launch<128>(maps, a, s);
 }

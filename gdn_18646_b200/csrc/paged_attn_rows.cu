@@ -1,0 +1,525 @@
+// paged_attn_rows.cu -- paged attention where an item has few rows (a decode step, a few
+// drafted tokens: tokens x query heads of a kv head <= 64), on tcgen05.
+//
+// The mathematics, the rows and the line of work are those of paged_attn.cu.  Here the
+// keys stand in the MMA's wide dimension and the rows in its narrow one:
+//   S^T = K Q^T      M 128 positions, N rows (16, 32 or 64), SS    -> TMEM, lane = position
+//   P^T (bf16)       thread = position, written to shared memory as the next B operand
+//   O^T += V^T P^T   M = D, N rows, SS (V as it lies, MN-major)    -> TMEM, lane = value index
+// so a tile of 128 keys costs N/128 of the tensor work of a 128-row tile, and its softmax
+// 128 threads x N exponentials instead of one warp x 128 a row (a tile took 2050 cycles that
+// way, which bound the kernel as soon as the clock fell; HBM delivers one in 2800).  The running
+// maximum is the same for all threads; only when some weight would pass 2^8 do they
+// reduce a new one and rescale.  The sums l stay per thread until the item ends.
+//
+// Bound by HBM: K and V are read once, 32 KB (D 128) per ring stage.
+#include <mutex>
+
+#include "common.cuh"
+#include "paged_work.cuh"
+
+namespace gdn {
+namespace {
+
+constexpr int kRowsThreads = 192;     // 4 softmax warps, MMA, load
+
+template <int D, int N>
+struct RowsShape {
+    static constexpr int HALVES = D / 64;
+    static constexpr int STAGE = kTile * D * 2;
+    static constexpr int Q_BYTES = HALVES * N * 128;            // one of two buffers
+    static constexpr int P_BYTES = 2 * N * 128;                 // 128 positions as two halves; one of two buffers
+    // D 64: the MMA (M 128) reads 16 KB past a V tile for result lanes that nobody uses
+    static constexpr int AFTER = 2 * Q_BYTES + 2 * P_BYTES + 3072 > 16384 ? 2 * Q_BYTES + 2 * P_BYTES + 3072 : 16384;
+    static constexpr int FIT = (232448 - 1024 - AFTER) / STAGE;
+    static constexpr int STAGES = FIT < 12 ? FIT : 12;
+    static constexpr int OFF_Q = STAGES * STAGE;
+    static constexpr int OFF_P = OFF_Q + 2 * Q_BYTES;
+    static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
+    static constexpr int SMEM = 1024 + OFF_Q + AFTER;
+    static constexpr int COLS = N == 16 ? 64 : N == 32 ? 128 : 256;     // TMEM: two S buffers, O
+    static constexpr int T_O = 2 * N;
+    static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct RowsBars {
+    uint64_t full[16], empty[16];
+    uint64_t q_full[2], q_empty[2];
+    uint64_t s_full[2], p_full[2];
+    uint64_t o_full, pv_done;
+    PieceScratch scratch;
+    float red[4][64];                 // per warp and row: tile maxima, then sums
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(RowsBars) <= 3072, "barrier block");
+
+// whether any of the 128 softmax threads says so
+__device__ __forceinline__ bool any_of_128(bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(x))
+        : "memory");
+    return r != 0;
+}
+
+// 16 columns of the thread's lane; the caller waits
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int D, int N>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+    using S = RowsShape<D, N>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    RowsBars* sh = reinterpret_cast<RowsBars*>(sm + S::OFF_BAR);
+    volatile int* dead = &sh->abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int MMA_WARP = 4, LOAD_WARP = 5;
+    const int tt = a.tile_tokens, cta = blockIdx.x;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&sh->full[i], 1);
+            mbar_init(&sh->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->q_full[i], 1);
+            mbar_init(&sh->q_empty[i], 1);
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_full[i], 4);
+        }
+        mbar_init(&sh->o_full, 1);
+        mbar_init(&sh->pv_done, 1);
+        sh->abort = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc(&sh->tmem, S::COLS);
+        tmem_relinquish();
+    }
+    pdl_launch_dependents();
+    pdl_wait_prior();                                           // q, the cache and the lengths come from earlier kernels
+    find_piece(a, &sh->scratch, tt);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem;
+    const Piece piece = sh->scratch.piece;
+
+    uint32_t q_loads = 0, issued = 0;                           // of the producer
+    int stage = 0;                                              // the kv ring, as the producer or the MMA warp walks it
+    uint32_t phase = 0;
+    auto step = [&]() {
+        if (++stage == S::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    };
+    if (warp == LOAD_WARP) {
+        // ---------------- TMA producer
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            if (w.t0 >= w.t1) continue;
+            const int qb = q_loads & 1;
+            if (!warp_wait(&sh->q_empty[qb], ((q_loads >> 1) & 1u) ^ 1u, a.err, dead)) break;
+            ++q_loads;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sh->q_full[qb], S::HALVES * tt * a.group * 128);
+                for (int h = 0; h < S::HALVES; ++h)
+                    tma_load_3d(sm + S::OFF_Q + qb * S::Q_BYTES + h * N * 128, &maps.q, &sh->q_full[qb], h * 64,
+                                w.head * a.group, w.s.c0 + w.item * tt);
+            }
+            if (!load_tiles<D, S::STAGES>(a, maps, w, sm, sh->full, sh->empty, stage, phase, issued, dead)) break;
+        }
+    } else if (warp == MMA_WARP) {
+        // ---------------- MMA issuer (one lane; the warp together clears unseen value rows)
+        constexpr uint32_t id_s = idesc_bf16(128, N, false, false);
+        constexpr uint32_t id_o = idesc_bf16(128, N, true, false);
+        const uint32_t k_lo = desc_lo(smem_u32(sm), 16), v_lo = desc_lo(smem_u32(sm), 16384);
+        const uint32_t q_lo = desc_lo(smem_u32(sm) + S::OFF_Q, 16), p_lo = desc_lo(smem_u32(sm) + S::OFF_P, 16);
+        uint32_t items = 0, done = 0;                           // done: kv tiles finished so far
+        auto mma_s = [&](uint32_t qb, uint32_t buf, int st) {   // S^T[buf] = K Q^T
+            const uint32_t k = uniform(k_lo + st * (S::STAGE >> 4)), q = uniform(q_lo + qb * (S::Q_BYTES >> 4));
+            const uint32_t d = uniform(tmem + buf * N);
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_bf16_ss(d, desc_of(k + (kk >> 2) * 1024 + (kk & 3) * 2), desc_of(q + (kk >> 2) * (N * 8) + (kk & 3) * 2),
+                                 id_s, kk > 0);
+                umma_commit(&sh->s_full[buf]);
+            }
+        };
+        auto mma_o = [&](uint32_t buf, int st, bool add) {      // O^T (+)= V^T P^T[buf]
+            const uint32_t v = uniform(v_lo + st * (S::STAGE >> 4)), p = uniform(p_lo + buf * (S::P_BYTES >> 4));
+            const uint32_t d = uniform(tmem + S::T_O), acc = uniform(add);
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kTile / 16; ++kk)
+                    umma_bf16_ss(d, desc_of(v + kk * 128), desc_of(p + (kk >> 2) * (N * 8) + (kk & 3) * 2), id_o,
+                                 kk > 0 ? 1u : acc);
+            }
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (elect_one()) umma_commit(bar);
+        };
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            if (w.t0 >= w.t1) continue;
+            const uint32_t qb = items & 1;
+            if (!warp_wait(&sh->q_full[qb], (items >> 1) & 1u, a.err, dead)) break;
+            ++items;
+            const int n = w.t1 - w.t0;
+            if (!warp_wait(&sh->full[stage], phase, a.err, dead)) break;
+            tc_fence_after();
+            mma_s(qb, done & 1u, stage);
+            commit(&sh->empty[stage]);
+            if (n == 1) commit(&sh->q_empty[qb]);
+            step();
+            bool stop = false;
+            for (int j = 0; j < n; ++j) {
+                const int vst = stage;
+                const uint32_t vph = phase;
+                step();
+                if (j + 1 < n) {
+                    if (!warp_wait(&sh->full[stage], phase, a.err, dead)) { stop = true; break; }
+                    tc_fence_after();
+                    mma_s(qb, (done + 1) & 1u, stage);
+                    commit(&sh->empty[stage]);
+                    if (j + 2 == n) commit(&sh->q_empty[qb]);
+                    step();
+                }
+                if (!warp_wait(&sh->full[vst], vph, a.err, dead)) { stop = true; break; }
+                clear_rows<D>(w, w.t0 + j, sm + vst * S::STAGE);
+                if (!warp_wait(&sh->p_full[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
+                tc_fence_after();
+                mma_o(done & 1u, vst, j > 0);
+                commit(&sh->empty[vst]);
+                commit(&sh->pv_done);
+                if (j + 1 == n) commit(&sh->o_full);
+                ++done;
+            }
+            if (stop) break;
+        }
+    } else {
+        // ---------------- softmax and epilogue: thread = position of the tile, then value index.
+        // No early way out of a tile: a wait that gave up returns, and all warps keep meeting at
+        // the barriers until their walk ends.
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        const float c = a.scale * 1.4426950408889634f;
+        uint8_t* const p_base = sm + S::OFF_P + (tid >> 6) * (N * 128);
+        uint32_t done = 0, items = 0;
+        if (tid == 0)
+            for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
+        Walk w;
+        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+            const int toks = min(tt, w.s.n - w.item * tt), nr = toks * a.group;     // rows of the item
+            const long at0 = static_cast<long>(w.s.c0 + w.item * tt) * a.Hq + w.head * a.group;
+            auto row_at = [&](int r) {                          // (token, head) row of the output
+                const int tok = r / a.group;
+                return at0 + static_cast<long>(tok) * a.Hq + (r - tok * a.group);
+            };
+            if (w.t0 >= w.t1) {
+                if (w.count == 0) {                             // sees nothing
+                    for (int r = 0; r < nr; ++r) {
+                        const long at = row_at(r);
+                        if (tid < D) a.out[at * D + tid] = 0;
+                        if (a.lse && tid == 0) a.lse[at] = -INFINITY;
+                    }
+                }
+                continue;
+            }
+            int lo0, hi0, lo1, hi1;                             // what the first and the last token see
+            w.s.range(a, w.item * tt, w.item * tt, lo0, hi0);
+            w.s.range(a, w.item * tt + toks - 1, w.item * tt + toks - 1, lo1, hi1);
+            float m[N], l[N];
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                m[r] = -INFINITY;
+                l[r] = 0.f;
+            }
+            for (int j = w.t0; j < w.t1; ++j, ++done) {
+                const uint32_t buf = done & 1u;
+                const int j0 = (w.first + j) * kTile, pos = j0 + tid;
+                float s[N];
+                warp_wait(&sh->s_full[buf], (done >> 1) & 1u, a.err, dead);
+                tc_fence_after();
+#pragma unroll
+                for (int q = 0; q < N; q += 16) tmem_ld16(tmem + lanes + buf * N + q, s + q);
+                tmem_ld_wait();
+                if (j0 + kTile > hi0 || j0 < lo1) {
+                    int g = 0, tok = 0, lo, hi;
+                    w.s.range(a, w.item * tt, w.item * tt, lo, hi);
+#pragma unroll
+                    for (int r = 0; r < N; ++r) {
+                        if (pos < lo || pos >= hi) s[r] = -INFINITY;
+                        if (++g == a.group) {
+                            g = 0;
+                            ++tok;
+                            w.s.range(a, w.item * tt + tok, w.item * tt + tok, lo, hi);
+                        }
+                    }
+                }
+                bool grow = false;                              // m = -inf: true for any finite s
+#pragma unroll
+                for (int r = 0; r < N; ++r)
+                    if (r < nr) grow |= (s[r] - m[r]) * c > 8.f;
+                if (any_of_128(grow)) {
+#pragma unroll
+                    for (int r = 0; r < N; ++r) {
+                        if (r >= nr) break;
+                        float x = s[r];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        if (lane == 0) sh->red[warp][r] = x;
+                    }
+                    named_bar(1, 128);
+                    const bool have_o = j > w.t0;
+                    if (have_o) {                               // O once P V(j - 1) is in it
+                        warp_wait(&sh->pv_done, (done - 1) & 1u, a.err, dead);
+                        tc_fence_after();
+                    }
+#pragma unroll
+                    for (int q = 0; q < N; q += 16) {
+                        float f[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = q + i;
+                            f[i] = 1.f;
+                            if (r < nr) {
+                                const float x = fmaxf(fmaxf(sh->red[0][r], sh->red[1][r]), fmaxf(sh->red[2][r], sh->red[3][r]));
+                                if (x > m[r]) {
+                                    f[i] = ex2_approx((m[r] - x) * c);
+                                    m[r] = x;
+                                    l[r] *= f[i];
+                                }
+                            }
+                        }
+                        if (have_o) {
+                            float o[16];
+                            uint32_t u[16];
+                            tmem_ld16(tmem + lanes + S::T_O + q, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f[i]);
+                            tmem_st16(tmem + lanes + S::T_O + q, u);
+                        }
+                    }
+                    if (have_o) tmem_st_wait();
+                }
+                uint8_t* const pb = p_base + buf * S::P_BYTES;
+#pragma unroll
+                for (int r = 0; r < N; ++r) {
+                    if (r >= nr) break;
+                    const float p = ex2_approx(fmaf(s[r], c, m[r] == -INFINITY ? 0.f : -m[r] * c));
+                    l[r] += p;
+                    *reinterpret_cast<uint16_t*>(pb + sw128_off(r, tid & 63)) = f32_to_bf16_bits(p);
+                }
+                fence_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[buf]);
+            }
+            // the sums of the threads, in order
+            named_bar(1, 128);
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                if (r >= nr) break;
+                float x = l[r];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                if (lane == 0) sh->red[warp][r] = x;
+            }
+            named_bar(1, 128);
+            warp_wait(&sh->o_full, items & 1u, a.err, dead);
+            ++items;
+            tc_fence_after();
+            const bool whole = w.t0 == 0 && w.t1 == w.count;
+            const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * a.part_rows;
+            int g = 0;
+            long at = at0;
+#pragma unroll
+            for (int q = 0; q < N; q += 16) {
+                if (q >= nr) break;
+                float o[16];
+                tmem_ld16(tmem + lanes + S::T_O + q, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = q + i;
+                    if (r >= nr) break;
+                    const float sum = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
+                    if (whole) {
+                        if (tid < D) a.out[at * D + tid] = f32_to_bf16_bits(sum == 0.f ? 0.f : o[i] * (1.f / sum));
+                        if (a.lse && tid == r) a.lse[at] = sum == 0.f ? -INFINITY : m[r] * a.scale + logf(sum);
+                    } else {
+                        if (tid < D) a.part_o[(slot + r) * D + tid] = o[i];
+                        if (tid == r) {
+                            a.part_ml[(slot + r) * 2] = m[r];
+                            a.part_ml[(slot + r) * 2 + 1] = sum;
+                        }
+                    }
+                    ++at;
+                    if (++g == a.group) {
+                        g = 0;
+                        at += a.Hq - a.group;
+                    }
+                }
+            }
+            tc_fence_before();
+            if (tid == 0 && !whole) {
+                int* ps = a.part_state + cta * 8;
+                if (w.t0 == 0) {
+                    ps[1] = 1;
+                    ps[2] = w.s.c0 + w.item * tt;                // first token
+                    ps[3] = toks;
+                    ps[4] = w.head;
+                } else {
+                    ps[0] = w.t1 == w.count ? 2 : 1;             // 2: the item's last part
+                }
+            }
+            named_bar(1, 128);                                  // red is read before the next item's maxima
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (sh->abort && warp == LOAD_WARP) {
+        drain_ring(a, sh->full, S::STAGES, issued);
+        for (uint32_t i = q_loads > 2 ? q_loads - 2 : 0; i < q_loads; ++i) mbar_wait(&sh->q_full[i & 1], (i >> 1) & 1u, a.err);
+    }
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::COLS);
+    }
+}
+
+// Joins the parts of the items that pieces cut: block x takes the item that CTA x began and
+// did not finish, a warp per row, the lanes along its values.
+template <int D>
+__global__ void __launch_bounds__(512) paged_attn_rows_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    pdl_wait_prior();
+    constexpr int V = D / 32, BATCH = 16;
+    const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the states of this CTA and of the 31 after it in one go
+    const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
+    const int head = __ldcg(a.part_state + x * 8 + 4);
+    int st = x + 1 + lane < ctas ? __ldcg(a.part_state + (x + 1 + lane) * 8) : 0;
+    if (mine.y == 0) return;
+    int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
+    for (int at = x + 1;;) {
+        const uint32_t end = __ballot_sync(0xffffffffu, st != 1);
+        if (end) {
+            const int k = __ffs(end) - 1;
+            parts += k + (__shfl_sync(0xffffffffu, st, k) == 2 ? 1 : 0);
+            break;
+        }
+        parts += 32;
+        at += 32;
+        st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
+    }
+    const float c = a.scale * 1.4426950408889634f;
+    for (int r = warp; r < mine.w * a.group; r += 16) {
+        // part 0 is CTA x's slot 1, part p the slot 0 of CTA x + p
+        auto row = [&](int p) { return (static_cast<long>(x) * 2 + (p == 0 ? 1 : 2 * p)) * a.part_rows + r; };
+        float m = -INFINITY, l = 0.f, o[V] = {};
+        for (int p0 = 0; p0 < parts; p0 += BATCH) {             // loads of a batch under a predicate, all in flight
+            float2 v[BATCH];
+            float u[BATCH][V];
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                v[k] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[k][i] = 0.f;
+                if (p0 + k < parts) {
+                    v[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + row(p0 + k));
+                    const float* src = a.part_o + row(p0 + k) * D + lane * V;
+                    if constexpr (V == 4) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
+                        u[k][0] = f.x; u[k][1] = f.y; u[k][2] = f.z; u[k][3] = f.w;
+                    } else {
+                        const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
+                        u[k][0] = f.x; u[k][1] = f.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
+            const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
+            m = mn;
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] *= keep;
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const float f = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
+                l += v[k].y * f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] += u[k][i] * f;
+            }
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int tok = r / a.group;
+        const long at = static_cast<long>(mine.z + tok) * a.Hq + head * a.group + (r - tok * a.group);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * V);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) dst[i] = l == 0.f ? 0u : cvt_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
+        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    }
+}
+
+template <int D, int N>
+int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
+    using S = RowsShape<D, N>;
+    const char* name = "gdn_paged_attn_fwd";
+    static std::once_flag once[64];                             // once per device
+    static cudaError_t attr[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(GDN_ERR_CUDA, "%s: no current device", name);
+    std::call_once(once[dev], [dev] {
+        attr[dev] = cudaFuncSetAttribute(paged_attn_rows_kernel<D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    });
+    if (attr[dev] != cudaSuccess)
+        return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr[dev]));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = launch_overlap() ? 1 : 0;
+    cfg.stream = st;
+    cfg.gridDim = dim3(kMaxCtas);
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_rows_kernel<D, N>, maps, a);
+    if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
+    cfg.numAttrs = 1;                                           // starts while the first kernel ends
+    cfg.blockDim = dim3(512);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_attn_rows_join_kernel<D>, a, static_cast<int>(kMaxCtas));
+    if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
+    return launch_status(name);
+}
+
+}  // namespace
+
+int launch_attn_rows(const AttnMaps& maps, const AttnArgs& a, int D, cudaStream_t st) {
+    if (D == 64) return a.part_rows == 16 ? launch<64, 16>(maps, a, st) : a.part_rows == 32 ? launch<64, 32>(maps, a, st) : launch<64, 64>(maps, a, st);
+    return a.part_rows == 16 ? launch<128, 16>(maps, a, st) : a.part_rows == 32 ? launch<128, 32>(maps, a, st) : launch<128, 64>(maps, a, st);
+}
+
+}  // namespace gdn
