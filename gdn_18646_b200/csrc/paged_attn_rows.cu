@@ -262,17 +262,14 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                 for (int q = 0; q < N; q += 16) tmem_ld16(tmem + lanes + buf * N + q, s + q);
                 tmem_ld_wait();
                 if (j0 + kTile > hi0 || j0 < lo1) {
-                    int g = 0, tok = 0, lo, hi;
-                    w.s.range(a, w.item * tt, w.item * tt, lo, hi);
+                    // the token that stands at this position, and the rows from it up to its window's end
+                    const int tok = pos - (w.s.kv - w.s.n + w.item * tt);
+                    int from = a.causal ? min(max(tok, 0) * a.group, N) : 0, to = N;
+                    if (a.window > 0) to = min(max(tok + a.window, 0), N) * a.group;
+                    if (pos >= w.s.kv) from = N;
 #pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        if (pos < lo || pos >= hi) s[r] = -INFINITY;
-                        if (++g == a.group) {
-                            g = 0;
-                            ++tok;
-                            w.s.range(a, w.item * tt + tok, w.item * tt + tok, lo, hi);
-                        }
-                    }
+                    for (int r = 0; r < N; ++r)
+                        if (r < from || r >= to) s[r] = -INFINITY;
                 }
                 bool grow = false;                              // m = -inf: true for any finite s
 #pragma unroll

@@ -219,9 +219,11 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
     const long long most = (total + kMinPiece - 1) / kMinPiece;
     const int pieces = most < gridDim.x ? static_cast<int>(most) : gridDim.x;
     if (blockIdx.x < pieces) {
-        // total x / pieces without a wide product
-        const long long q = total / pieces;
-        const int r = static_cast<int>(total - q * pieces), x = blockIdx.x;
+        // total x / pieces without a wide product; the quotient in two short divisions (total < 2^48)
+        const uint32_t top = static_cast<uint32_t>(total >> 24), q1 = top / pieces;
+        const uint32_t low = (top - q1 * pieces) << 24 | static_cast<uint32_t>(total & 0xffffff), q0 = low / pieces;
+        const long long q = static_cast<long long>(q1) << 24 | q0;
+        const int r = static_cast<int>(low - q0 * pieces), x = blockIdx.x;
         const long long from = q * x + r * x / pieces, to = q * (x + 1) + r * (x + 1) / pieces;
         if (from >= start && from < start + mine) {
             int b = b0;
@@ -233,13 +235,15 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
                     start += u * a.n_kv;
                 }
             }
-            const long long off = from - start;
+            long long off = from - start;
+            int head = 0;
+            for (; off >= u; off -= u) ++head;
             Piece& p = sh->piece;
             p.s = s;
             p.b = b;
-            p.head = static_cast<int>(off / u);
+            p.head = head;
             p.item = 0;
-            p.skip = static_cast<int>(off - p.head * u);        // within the head, so far
+            p.skip = static_cast<int>(off);                     // within the head, so far
             p.units = to - from;
         }
     }
