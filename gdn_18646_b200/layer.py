@@ -111,13 +111,14 @@ class GDNLayer:
         return q, k, v, z, ab
 
     @torch.no_grad()
-    def prefill(self, x: torch.Tensor, state: dict | None = None, trace: dict | None = None):
-        """x [B,T,D] bf16 -> (y [B,T,D] bf16, state after the last token).
+    def prefill(self, x: torch.Tensor, state: dict | None = None, trace: dict | None = None, *, normed: bool = False):
+        """x [B,T,D] bf16 -> (y [B,T,D] bf16, state after the last token).  ``normed``: x has
+        been through the layer's input norm already (a stack's ``block_norm`` does it).
         ``trace``: a dict that receives the intermediate tensors (xn, q, k, v, z,
         a, b [B,Hv,T], o [B,T,Hv,dv], y_norm) for stage-by-stage checks."""
         c, w = self.cfg, self.w
         B, T, D = x.shape
-        xn = ops.rmsnorm(x.reshape(B * T, D), w["norm_gamma"], c.eps).reshape(B, T, D)
+        xn = x if normed else ops.rmsnorm(x.reshape(B * T, D), w["norm_gamma"], c.eps).reshape(B, T, D)
         new_state = self.init_state(B, x.device, fill=torch.empty)   # written by the projections and prefill
         q, k, v, z, ab = self._project(xn, state, new_state)
         a, b = ab[..., :c.n_v], ab[..., c.n_v:2 * c.n_v]          # [B, T, Hv] token rows, read in place
@@ -133,10 +134,11 @@ class GDNLayer:
         return out, new_state
 
     @torch.no_grad()
-    def decode(self, x: torch.Tensor, state: dict, out_state: dict | None = None):
+    def decode(self, x: torch.Tensor, state: dict, out_state: dict | None = None, *, normed: bool = False):
         """One token: x [B,1,D] bf16 -> (y [B,1,D] bf16, state).  The recurrent
         state is updated in place; conv histories go to ``out_state`` (fresh
         buffers by default; ``out_state=state`` updates them in place too).
+        ``normed``: x has been through the layer's input norm already.
 
         Three launches: RMSNorm + q|k|v (conv4, SiLU) + z + a + b as one
         weight-streaming GEMV over the cached conv history (gdn_decode_proj_fwd),
@@ -159,7 +161,7 @@ class GDNLayer:
             dict(W=w["W_z"]),
             dict(W=w["W_ab"][:c.n_v]),
             dict(W=w["W_ab"][c.n_v:]),
-        ], norm_gamma=w["norm_gamma"], eps=c.eps)
+        ], norm_gamma=None if normed else w["norm_gamma"], eps=c.eps)
         y = ops.decode_step_gated(q.view(B, c.n_qk, c.dk), k.view(B, c.n_qk, c.dk), v.view(B, c.n_v, c.dv), a, b,
                                   w["A_log"], w["dt_bias"], state["recurrent"], z.view(B, c.n_v, c.dv),
                                   w["onorm_gamma"], c.eps, scale=self.scale, state_out=out_state["recurrent"],
