@@ -27,6 +27,7 @@
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // The tensor core works for one row tile while the softmax of the other runs.  Items of
 // at most 64 rows (a decode step) go to paged_attn_rows.cu.
+#include <cstddef>
 #include <mutex>
 #include <type_traits>
 
@@ -38,10 +39,14 @@ namespace gdn {
 namespace {
 
 constexpr int QT = 2;                 // row tiles of 128 per item
-constexpr int kItemCost = 2;          // kv tiles that starting and ending an item is worth, beside its tiles
+constexpr int kItemCost = 3;          // kv tiles that starting and ending an item is worth, beside its tiles
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
 constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
 
+// umma_commit to a barrier given by its shared-memory address
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -167,141 +172,106 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             if (!load_tiles<D, S::STAGES>(a, maps, w, sm + S::OFF_KV, sh->full, sh->empty, stage, phase, issued, dead)) break;
         }
     } else if (warp == MMA_WARP) {
-        // ---------------- MMA issuer (one lane; the warp together clears unseen value rows)
+        // ---------------- MMA issuer (one lane; the warp together clears unseen value rows).
+        // The tensor core takes about one MMA in 64 cycles and queues few, so what this warp does
+        // between MMAs is time lost: one shuffle a tile makes the stages uniform (descriptors then
+        // stay in uniform registers), barriers go by shared-memory addresses.
         constexpr uint32_t id_s = idesc_bf16(128, kTile, false, false);
         constexpr uint32_t id_o = idesc_bf16(128, D, false, true);
-        int stage = 0, items = 0;
-        uint32_t phase = 0;
-        uint32_t done = 0;                                      // kv tiles finished so far
+        const uint32_t sm0 = uniform(smem_u32(sm)), tm = uniform(tmem), bars = smem_u32(sh);
+        const uint32_t q_lo = desc_lo(sm0, 16), k_lo = desc_lo(sm0 + S::OFF_KV, 16), v_lo = desc_lo(sm0 + S::OFF_KV, 16384);
+        const uint32_t full = bars + offsetof(Bars, full), empty = bars + offsetof(Bars, empty);
+        const uint32_t s_full = bars + offsetof(Bars, s_full), p_part = bars + offsetof(Bars, p_part);
+        const uint32_t p_full = bars + offsetof(Bars, p_full), o_full = bars + offsetof(Bars, o_full);
+        const uint32_t q_full = bars + offsetof(Bars, q_full), q_empty = bars + offsetof(Bars, q_empty);
+        uint32_t stage = 0, phase = 0, items = 0, done = 0;     // done: kv tiles finished so far
         auto step = [&]() {
             if (++stage == S::STAGES) {
                 stage = 0;
                 phase ^= 1u;
             }
         };
-        const uint32_t q_lo = desc_lo(smem_u32(sm), 16);
-        const uint32_t k_lo = desc_lo(smem_u32(sm) + S::OFF_KV, 16), v_lo = desc_lo(smem_u32(sm) + S::OFF_KV, 16384);
-        auto mma_s = [&](int t, int buf, int st) {              // S[buf] = Q[t] K^T
-            const uint32_t q = uniform(q_lo + t * (S::HALVES * 1024)), k = uniform(k_lo + st * (S::STAGE >> 4));
-            const uint32_t d = uniform(tmem + buf * kTile);
-            if (elect_one()) {
+        // inside an elected lane's branch: S[t] = Q[t] K^T;  O[t] (+)= P[t] V over k-steps k0 .. k1 - 1
+        auto mma_s = [&](int t, uint32_t st) {
+            const uint32_t q = q_lo + t * (S::HALVES * 1024), k = k_lo + st * (S::STAGE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t o = (kk >> 2) * 1024 + (kk & 3) * 2;
-                    umma_bf16_ss(d, desc_of(q + o), desc_of(k + o), id_s, kk > 0);
-                }
-                umma_commit(&sh->s_full[buf]);
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t o = (kk >> 2) * 1024 + (kk & 3) * 2;
+                umma_bf16_ss(tm + t * kTile, desc_of(q + o), desc_of(k + o), id_s, kk > 0);
             }
+            commit_to(s_full + t * 8);
         };
-        auto mma_o = [&](int t, int buf, int st, bool add, auto part) {   // O[t] (+)= P[buf] V, first or second part
-            const uint32_t v = uniform(v_lo + st * (S::STAGE >> 4));
-            const uint32_t d = uniform(tmem + S::T_O + t * S::O_COLS), pm = uniform(tmem + buf * kTile);
-            const uint32_t acc = uniform(add);
-            if (elect_one()) {
-                constexpr int k0 = decltype(part)::value == 0 ? 0 : kEarly * 2, k1 = decltype(part)::value == 0 ? kEarly * 2 : kTile / 16;
+        auto mma_o = [&](int t, uint32_t st, uint32_t add, auto k0, auto k1) {
+            const uint32_t v = v_lo + st * (S::STAGE >> 4);
 #pragma unroll
-                for (int kk = k0; kk < k1; ++kk)
-                    umma_bf16_ts(d, pm + kk * 8, desc_of(v + kk * 128), id_o, kk > 0 ? 1u : acc);
-            }
+            for (int kk = decltype(k0)::value; kk < decltype(k1)::value; ++kk)
+                umma_bf16_ts(tm + S::T_O + t * S::O_COLS, tm + t * kTile + kk * 8, desc_of(v + kk * 128), id_o, kk > 0 ? 1u : add);
         };
-        constexpr std::integral_constant<int, 0> first_part{};
-        constexpr std::integral_constant<int, 1> second_part{};
-        auto commit = [&](uint64_t* bar) {
-            if (elect_one()) umma_commit(bar);
-        };
-        // zero the value rows that no row of the item sees: a weight of 0 times what the cache
-        // holds there (NaN included) has to be 0
-        auto clear_rows = [&](const Walk& w, int j, int st) {
-            const int j0 = (w.first + j) * kTile;
-            if (j0 >= w.lo && j0 + kTile <= w.hi) return;
-            uint8_t* v = sm + S::OFF_KV + st * S::STAGE;
-            const int below = max(0, w.lo - j0), above = min(kTile, w.hi - j0);
-            for (int c = lane; c < kTile * 8 * S::HALVES; c += 32) {
-                const int r = (c >> 3) & (kTile - 1);
-                if (r < below || r >= above) *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
-            __syncwarp();
-        };
+        constexpr std::integral_constant<int, 0> k_first{};
+        constexpr std::integral_constant<int, kEarly * 2> k_early{};
+        constexpr std::integral_constant<int, kTile / 16> k_last{};
         Walk w;
         for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
             if (w.t0 >= w.t1) continue;
-            if (!warp_wait(&sh->q_full, static_cast<uint32_t>(items & 1), a.err, dead)) break;
-            ++items;
             const int n = w.t1 - w.t0;
-            if (!warp_wait(&sh->full[stage], phase, a.err, dead)) break;
+            // only the item's first and last tile hold positions that no row of it sees
+            const int clear_lo = (w.first + w.t0) * kTile < w.lo ? 0 : -1;
+            const int clear_hi = (w.first + w.t1) * kTile > w.hi ? n - 1 : -1;
+            wait_at(q_full, items & 1u, a.err, dead);
+            ++items;
+            wait_at(full + stage * 8, phase, a.err, dead);
             tc_fence_after();
-            bool stop = false;
-            if constexpr (QT == 2) {
-                mma_s(0, 0, stage);
-                mma_s(1, 1, stage);
-                commit(&sh->empty[stage]);
-                if (n == 1) commit(&sh->q_empty);
-                step();
-                for (int j = 0; j < n; ++j) {
-                    const int vst = stage;
-                    if (!warp_wait(&sh->full[vst], phase, a.err, dead)) { stop = true; break; }
-                    step();
-                    clear_rows(w, w.t0 + j, vst);
-                    const bool more = j + 1 < n;
-                    const int kst = stage;
-                    const uint32_t kph = phase;
-                    if (more) step();
-                    for (int t = 0; t < 2; ++t) {
-                        if (!warp_wait(&sh->p_part[t], done & 1u, a.err, dead)) { stop = true; break; }
-                        tc_fence_after();
-                        mma_o(t, t, vst, j > 0, first_part);
-                        if (!warp_wait(&sh->p_full[t], done & 1u, a.err, dead)) { stop = true; break; }
-                        tc_fence_after();
-                        mma_o(t, t, vst, j > 0, second_part);
-                        if (t == 1) commit(&sh->empty[vst]);
-                        if (more) {
-                            if (t == 0 && !warp_wait(&sh->full[kst], kph, a.err, dead)) { stop = true; break; }
-                            tc_fence_after();
-                            mma_s(t, t, kst);
-                            if (t == 1) {
-                                commit(&sh->empty[kst]);
-                                if (j + 2 == n) commit(&sh->q_empty);
-                            }
-                        } else {
-                            commit(&sh->o_full[t]);
-                        }
-                    }
-                    if (stop) break;
-                    ++done;
-                }
-            } else {
-                mma_s(0, done & 1u, stage);
-                commit(&sh->empty[stage]);
-                if (n == 1) commit(&sh->q_empty);
-                step();
-                for (int j = 0; j < n; ++j) {
-                    const int vst = stage;
-                    const uint32_t vph = phase;
-                    step();
-                    if (j + 1 < n) {
-                        if (!warp_wait(&sh->full[stage], phase, a.err, dead)) { stop = true; break; }
-                        tc_fence_after();
-                        mma_s(0, (done + 1) & 1u, stage);
-                        commit(&sh->empty[stage]);
-                        if (j + 2 == n) commit(&sh->q_empty);
-                        step();
-                    }
-                    if (!warp_wait(&sh->full[vst], vph, a.err, dead)) { stop = true; break; }
-                    clear_rows(w, w.t0 + j, vst);
-                    if (!warp_wait(&sh->p_part[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
-                    tc_fence_after();
-                    mma_o(0, done & 1u, vst, j > 0, first_part);
-                    if (!warp_wait(&sh->p_full[done & 1u], (done >> 1) & 1u, a.err, dead)) { stop = true; break; }
-                    tc_fence_after();
-                    mma_o(0, done & 1u, vst, j > 0, second_part);
-                    commit(&sh->empty[vst]);
-                    
-                    if (j + 1 == n) commit(&sh->o_full[0]);
-                    ++done;
+            {
+                const uint32_t k = uniform(stage);
+                if (elect_one()) {
+                    mma_s(0, k);
+                    mma_s(1, k);
+                    commit_to(empty + k * 8);
+                    if (n == 1) commit_to(q_empty);
                 }
             }
-            if (stop) break;
+            step();
+            for (int j = 0; j < n; ++j) {
+                const uint32_t vst = stage, vph = phase;
+                step();
+                const uint32_t kst = stage, kph = phase;
+                const bool more = j + 1 < n;
+                if (more) step();
+                const uint32_t both = uniform(vst | kst << 8 | (j > 0 ? 1u << 16 : 0u));
+                const uint32_t v = both & 0xff, k = (both >> 8) & 0xff, add = both >> 16, ph = done & 1u;
+                wait_at(full + vst * 8, vph, a.err, dead);
+                if (j == clear_lo || j == clear_hi) clear_rows<D>(w, w.t0 + j, sm + S::OFF_KV + vst * S::STAGE);
+                wait_at(p_part, ph, a.err, dead);
+                tc_fence_after();
+                if (elect_one()) mma_o(0, v, add, k_first, k_early);
+                wait_at(p_full, ph, a.err, dead);
+                tc_fence_after();
+                if (more) wait_at(full + kst * 8, kph, a.err, dead);
+                if (elect_one()) {
+                    mma_o(0, v, add, k_early, k_last);
+                    if (more)
+                        mma_s(0, k);
+                    else
+                        commit_to(o_full);
+                }
+                wait_at(p_part + 8, ph, a.err, dead);
+                tc_fence_after();
+                if (elect_one()) mma_o(1, v, add, k_first, k_early);
+                wait_at(p_full + 8, ph, a.err, dead);
+                tc_fence_after();
+                if (elect_one()) {
+                    mma_o(1, v, add, k_early, k_last);
+                    commit_to(empty + v * 8);
+                    if (more) {
+                        mma_s(1, k);
+                        commit_to(empty + k * 8);
+                        if (j + 2 == n) commit_to(q_empty);
+                    } else {
+                        commit_to(o_full + 8);
+                    }
+                }
+                ++done;
+            }
         }
     } else {
         // ---------------- softmax and epilogue: a thread per row
@@ -311,6 +281,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         const int tok = row / a.group, g = row - tok * a.group; // token within the row tile, head within the group
         const float c = a.scale * 1.4426950408889634f;
         const uint32_t o_col = tmem + lanes + S::T_O + t * S::O_COLS;
+        const uint32_t s_full = smem_u32(&sh->s_full[t]), o_full = smem_u32(&sh->o_full[t]);
         uint32_t done = 0, items = 0;
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
@@ -331,18 +302,13 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 }
                 continue;
             }
-                  // no token in this row tile
             int lo, hi, dummy, hi_first, lo_last;
             w.s.range(a, rel, rel, lo, hi);
             w.s.range(a, first_tok, first_tok, dummy, hi_first);
             w.s.range(a, last_tok, last_tok, lo_last, dummy);
             float m = -INFINITY, l = 0.f;
-            bool stop = false;
             for (int j = w.t0; j < w.t1; ++j) {
-                if (!warp_wait(&sh->s_full[t], done & 1u, a.err, dead)) {
-                    stop = true;
-                    break;
-                }
+                wait_at(s_full, done & 1u, a.err, dead);
                 tc_fence_after();
                 if (busy) {
                     const uint32_t s_col = tmem + lanes + t * kTile;
@@ -352,17 +318,15 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
 #pragma unroll
                         for (int q = 0; q < 4; ++q) tmem_ld32(s_col + q * 32, reinterpret_cast<float(&)[32]>(s[q * 32]));
                         tmem_ld_wait();
-                        if (j0 + kTile > hi_first) {
-                            const int end = hi - j0;
+                        if (j0 + kTile > hi_first || j0 < lo_last) {     // bits of the positions this row sees
 #pragma unroll
-                            for (int i = 0; i < kTile; ++i)
-                                if (i >= end) s[i] = -INFINITY;
-                        }
-                        if (j0 < lo_last) {
-                            const int begin = lo - j0;
+                            for (int q = 0; q < 4; ++q) {
+                                const int e = min(max(hi - j0 - q * 32, 0), 32), b = min(max(lo - j0 - q * 32, 0), 32);
+                                const uint32_t bits = (e == 32 ? ~0u : (1u << e) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
 #pragma unroll
-                            for (int i = 0; i < kTile; ++i)
-                                if (i < begin) s[i] = -INFINITY;
+                                for (int i = 0; i < 32; ++i)
+                                    if (!(bits & (1u << i))) s[q * 32 + i] = -INFINITY;
+                            }
                         }
                     };
                     load_s();
@@ -433,8 +397,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 if (lane == 0) mbar_arrive(&sh->p_full[t]);
                 ++done;
             }
-            if (stop) break;
-            if (!warp_wait(&sh->o_full[t], items & 1u, a.err, dead)) break;
+            wait_at(o_full, items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
             if (m == -INFINITY) l = 0.f;                                // saw nothing (the polynomial gives 2^-125 for 2^-inf)

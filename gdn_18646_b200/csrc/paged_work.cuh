@@ -72,6 +72,37 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3FFFFu) >> 4) | (lbo_bytes >> 4) << 16; }
 
+// A wait at a barrier given by its shared-memory address, for warps whose every step counts: it
+// ends with the warp together and says nothing when it gave up (the error word and *dead are
+// set then, all later waits return at once, and the warp runs on to its end over garbage).
+static __device__ __noinline__ void wait_slowly(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    const long long t0 = clock64(), budget = wait_budget();
+    uint32_t ok = 0;
+    while (!ok) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok || *dead) return;
+        if (clock64() - t0 > budget) {
+            if (err) atomicOr(err, DERR_TIMEOUT);
+            *dead = 1;
+            return;
+        }
+    }
+}
+__device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (!ok) wait_slowly(bar, parity, err, dead);
+    __syncwarp();
+}
+
 // A wait that all lanes of a warp leave alike, also when it gives up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* dead) {
     return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, dead));

@@ -899,7 +899,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
         return (out, lse) if return_lse else out
     ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
     if workspace is None:
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(ws_bytes // 2)
     elif not (workspace.is_cuda and workspace.dtype is torch.uint8 and workspace.numel() >= ws_bytes):
         raise RuntimeError(f"workspace: uint8 CUDA tensor of at least {ws_bytes} bytes required")
     _lib.call("gdn_paged_attn_fwd", q.data_ptr(), q_ld, ctypes.byref(cache), cu_seqlens.data_ptr(), kv_lens.data_ptr(),
