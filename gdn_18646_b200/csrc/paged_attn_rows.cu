@@ -30,12 +30,15 @@ struct RowsShape {
     static constexpr int Q_BYTES = HALVES * N * 128;            // one of two buffers
     static constexpr int P_BYTES = 2 * N * 128;                 // 128 positions as two halves; one of two buffers
     // D 64: the MMA (M 128) reads 16 KB past a V tile for result lanes that nobody uses
-    static constexpr int AFTER = 2 * Q_BYTES + 2 * P_BYTES + 3072 > 16384 ? 2 * Q_BYTES + 2 * P_BYTES + 3072 : 16384;
+    static constexpr int L_BYTES = N * 128 * 4;                 // every thread's part of the rows' sums
+    static constexpr int USED = 2 * Q_BYTES + 2 * P_BYTES + L_BYTES + 3072;
+    static constexpr int AFTER = USED > 16384 ? USED : 16384;
     static constexpr int FIT = (232448 - 1024 - AFTER) / STAGE;
     static constexpr int STAGES = FIT < 12 ? FIT : 12;
     static constexpr int OFF_Q = STAGES * STAGE;
     static constexpr int OFF_P = OFF_Q + 2 * Q_BYTES;
-    static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
+    static constexpr int OFF_L = OFF_P + 2 * P_BYTES;
+    static constexpr int OFF_BAR = OFF_L + L_BYTES;
     static constexpr int SMEM = 1024 + OFF_Q + AFTER;
     static constexpr int COLS = N == 16 ? 64 : N == 32 ? 128 : 256;     // TMEM: two S buffers, O
     static constexpr int T_O = 2 * N;
@@ -48,6 +51,7 @@ struct RowsBars {
     uint64_t s_full[2], p_full[2];
     uint64_t o_full, pv_done;
     PieceScratch scratch;
+    float m[64], f[64];               // per row: reference maximum, factor of a rescale
     float red[4][64];                 // per warp and row: tile maxima, then sums
     uint32_t tmem;
     int abort;
@@ -65,16 +69,43 @@ __device__ __forceinline__ bool any_of_128(bool x) {
     return r != 0;
 }
 
-// 16 columns of the thread's lane; the caller waits
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+// 8 columns of the thread's lane
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+    tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+                 "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
+// Eight rows' maxima (or sums) over the warp's lanes: halves of the rows go to halves of the
+// lanes, so lanes 4 i .. 4 i + 3 end with row i's.
+template <bool MAX>
+__device__ __forceinline__ float reduce8(float (&v)[8]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 4, o = 16; n >= 1; n >>= 1, o >>= 1) {
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            const float got = __shfl_xor_sync(0xffffffffu, send, o);
+            v[i] = MAX ? fmaxf(keep, got) : keep + got;
+        }
+    }
+#pragma unroll
+    for (int o = 2; o >= 1; o >>= 1) {
+        const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
+        v[0] = MAX ? fmaxf(v[0], got) : v[0] + got;
+    }
+    return v[0];
 }
 
 template <int D, int N>
@@ -217,14 +248,19 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         }
     } else {
         // ---------------- softmax and epilogue: thread = position of the tile, then value index.
-        // No early way out of a tile: a wait that gave up returns, and all warps keep meeting at
-        // the barriers until their walk ends.
+        // Eight rows at a time in loops that are not unrolled: with all rows unrolled the code did
+        // not stay in the instruction cache, and an item of one tile took 11 us (N 16) to 24 us
+        // (N 64).  No early way out of a tile: a wait that gave up returns, and all warps keep
+        // meeting at the barriers until their walk ends.
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         const float c = a.scale * 1.4426950408889634f;
         uint8_t* const p_base = sm + S::OFF_P + (tid >> 6) * (N * 128);
+        float* const l = reinterpret_cast<float*>(sm + S::OFF_L) + tid;                 // l[row * 128]
         uint32_t done = 0, items = 0;
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
+        if (tid < 64) sh->m[tid] = -INFINITY;
+        named_bar(1, 128);
         Walk w;
         for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
             const int toks = min(tt, w.s.n - w.item * tt), nr = toks * a.group;     // rows of the item
@@ -246,85 +282,85 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             int lo0, hi0, lo1, hi1;                             // what the first and the last token see
             w.s.range(a, w.item * tt, w.item * tt, lo0, hi0);
             w.s.range(a, w.item * tt + toks - 1, w.item * tt + toks - 1, lo1, hi1);
-            float m[N], l[N];
-#pragma unroll
-            for (int r = 0; r < N; ++r) {
-                m[r] = -INFINITY;
-                l[r] = 0.f;
-            }
+#pragma unroll 1
+            for (int r = 0; r < nr; ++r) l[r * 128] = 0.f;
+#pragma unroll 1
             for (int j = w.t0; j < w.t1; ++j, ++done) {
-                const uint32_t buf = done & 1u;
+                const uint32_t buf = done & 1u, s_col = tmem + lanes + buf * N;
                 const int j0 = (w.first + j) * kTile, pos = j0 + tid;
-                float s[N];
-                warp_wait(&sh->s_full[buf], (done >> 1) & 1u, a.err, dead);
-                tc_fence_after();
-#pragma unroll
-                for (int q = 0; q < N; q += 16) tmem_ld16(tmem + lanes + buf * N + q, s + q);
-                tmem_ld_wait();
+                // rows [from, to) see this position: those of the token that stands here and of the
+                // tokens after it, up to the window's end
+                int from = 0, to = N;
                 if (j0 + kTile > hi0 || j0 < lo1) {
-                    // the token that stands at this position, and the rows from it up to its window's end
                     const int tok = pos - (w.s.kv - w.s.n + w.item * tt);
-                    int from = a.causal ? min(max(tok, 0) * a.group, N) : 0, to = N;
+                    if (a.causal) from = min(max(tok, 0) * a.group, N);
                     if (a.window > 0) to = min(max(tok + a.window, 0), N) * a.group;
                     if (pos >= w.s.kv) from = N;
-#pragma unroll
-                    for (int r = 0; r < N; ++r)
-                        if (r < from || r >= to) s[r] = -INFINITY;
                 }
+                float s[8];
+                auto load = [&](int q) {
+                    tmem_ld8(s_col + q, s);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (q + i < from || q + i >= to) s[i] = -INFINITY;
+                };
+                wait_at(smem_u32(&sh->s_full[buf]), (done >> 1) & 1u, a.err, dead);
+                tc_fence_after();
                 bool grow = false;                              // m = -inf: true for any finite s
+#pragma unroll 1
+                for (int q = 0; q < nr; q += 8) {
+                    load(q);
 #pragma unroll
-                for (int r = 0; r < N; ++r)
-                    if (r < nr) grow |= (s[r] - m[r]) * c > 8.f;
+                    for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[i] - sh->m[q + i]) * c > 8.f;
+                }
                 if (any_of_128(grow)) {
+#pragma unroll 1
+                    for (int q = 0; q < nr; q += 8) {
+                        if (nr > 8) load(q);
+                        float x[8];
 #pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        if (r >= nr) break;
-                        float x = s[r];
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                        if (lane == 0) sh->red[warp][r] = x;
+                        for (int i = 0; i < 8; ++i) x[i] = s[i];
+                        const float top = reduce8<true>(x);
+                        if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = top;
                     }
                     named_bar(1, 128);
-                    const bool have_o = j > w.t0;
-                    if (have_o) {                               // O once P V(j - 1) is in it
-                        warp_wait(&sh->pv_done, (done - 1) & 1u, a.err, dead);
+                    if (tid < nr) {
+                        const float x = fmaxf(fmaxf(sh->red[0][tid], sh->red[1][tid]), fmaxf(sh->red[2][tid], sh->red[3][tid]));
+                        const float m = sh->m[tid];
+                        sh->f[tid] = x > m ? ex2_approx((m - x) * c) : 1.f;
+                        if (x > m) sh->m[tid] = x;
+                    }
+                    named_bar(1, 128);
+                    if (j > w.t0) {                             // O once P V(j - 1) is in it
+                        wait_at(smem_u32(&sh->pv_done), (done - 1) & 1u, a.err, dead);
                         tc_fence_after();
-                    }
+#pragma unroll 1
+                        for (int q = 0; q < nr; q += 8) {
+                            float o[8];
+                            tmem_ld8(tmem + lanes + S::T_O + q, o);
 #pragma unroll
-                    for (int q = 0; q < N; q += 16) {
-                        float f[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int r = q + i;
-                            f[i] = 1.f;
-                            if (r < nr) {
-                                const float x = fmaxf(fmaxf(sh->red[0][r], sh->red[1][r]), fmaxf(sh->red[2][r], sh->red[3][r]));
-                                if (x > m[r]) {
-                                    f[i] = ex2_approx((m[r] - x) * c);
-                                    m[r] = x;
-                                    l[r] *= f[i];
-                                }
+                            for (int i = 0; i < 8; ++i) {
+                                const float f = q + i < nr ? sh->f[q + i] : 1.f;
+                                o[i] *= f;
+                                if (q + i < nr) l[(q + i) * 128] *= f;
                             }
+                            tmem_st8(tmem + lanes + S::T_O + q, o);
                         }
-                        if (have_o) {
-                            float o[16];
-                            uint32_t u[16];
-                            tmem_ld16(tmem + lanes + S::T_O + q, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f[i]);
-                            tmem_st16(tmem + lanes + S::T_O + q, u);
-                        }
+                        tmem_st_wait();
                     }
-                    if (have_o) tmem_st_wait();
                 }
                 uint8_t* const pb = p_base + buf * S::P_BYTES;
+                // rows past the item's go with the last eight (their columns go nowhere)
+#pragma unroll 1
+                for (int q = 0; q < nr; q += 8) {
+                    if (nr > 8) load(q);
 #pragma unroll
-                for (int r = 0; r < N; ++r) {
-                    if (r >= nr) break;
-                    const float p = ex2_approx(fmaf(s[r], c, m[r] == -INFINITY ? 0.f : -m[r] * c));
-                    l[r] += p;
-                    *reinterpret_cast<uint16_t*>(pb + sw128_off(r, tid & 63)) = f32_to_bf16_bits(p);
+                    for (int i = 0; i < 8; ++i) {
+                        const float m = sh->m[q + i];
+                        const float p = ex2_approx(fmaf(s[i], c, m == -INFINITY ? 0.f : -m * c));
+                        if (q + i < nr) l[(q + i) * 128] += p;
+                        *reinterpret_cast<uint16_t*>(pb + sw128_off(q + i, tid & 63)) = f32_to_bf16_bits(p);
+                    }
                 }
                 fence_async_smem();
                 tc_fence_before();
@@ -332,52 +368,52 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                 if (lane == 0) mbar_arrive(&sh->p_full[buf]);
             }
             // the sums of the threads, in order
-            named_bar(1, 128);
+#pragma unroll 1
+            for (int q = 0; q < nr; q += 8) {
+                float x[8];
 #pragma unroll
-            for (int r = 0; r < N; ++r) {
-                if (r >= nr) break;
-                float x = l[r];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                if (lane == 0) sh->red[warp][r] = x;
+                for (int i = 0; i < 8; ++i) x[i] = q + i < nr ? l[(q + i) * 128] : 0.f;
+                const float sum = reduce8<false>(x);
+                if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = sum;
             }
             named_bar(1, 128);
-            warp_wait(&sh->o_full, items & 1u, a.err, dead);
+            wait_at(smem_u32(&sh->o_full), items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
             const bool whole = w.t0 == 0 && w.t1 == w.count;
             const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * a.part_rows;
-            int g = 0;
-            long at = at0;
+#pragma unroll 1
+            for (int q = 0; q < nr; q += 8) {
+                float o[8];
+                tmem_ld8(tmem + lanes + S::T_O + q, o);
+                int tok = q / a.group, g = q - tok * a.group;
+                if (tid < D)
 #pragma unroll
-            for (int q = 0; q < N; q += 16) {
-                if (q >= nr) break;
-                float o[16];
-                tmem_ld16(tmem + lanes + S::T_O + q, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = q + i;
-                    if (r >= nr) break;
-                    const float sum = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
-                    if (whole) {
-                        if (tid < D) a.out[at * D + tid] = f32_to_bf16_bits(sum == 0.f ? 0.f : o[i] * (1.f / sum));
-                        if (a.lse && tid == r) a.lse[at] = sum == 0.f ? -INFINITY : m[r] * a.scale + logf(sum);
-                    } else {
-                        if (tid < D) a.part_o[(slot + r) * D + tid] = o[i];
-                        if (tid == r) {
-                            a.part_ml[(slot + r) * 2] = m[r];
-                            a.part_ml[(slot + r) * 2 + 1] = sum;
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = q + i;
+                        const float sum = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
+                        if (r < nr) {
+                            if (whole)
+                                a.out[(at0 + static_cast<long>(tok) * a.Hq + g) * D + tid] =
+                                    f32_to_bf16_bits(sum == 0.f ? 0.f : __fdividef(o[i], sum));
+                            else
+                                a.part_o[(slot + r) * D + tid] = o[i];
+                        }
+                        if (++g == a.group) {
+                            g = 0;
+                            ++tok;
                         }
                     }
-                    ++at;
-                    if (++g == a.group) {
-                        g = 0;
-                        at += a.Hq - a.group;
-                    }
-                }
             }
             tc_fence_before();
+            if (tid < nr) {
+                const float sum = (sh->red[0][tid] + sh->red[1][tid]) + (sh->red[2][tid] + sh->red[3][tid]), m = sh->m[tid];
+                if (!whole)
+                    *reinterpret_cast<float2*>(a.part_ml + (slot + tid) * 2) = make_float2(m, sum);
+                else if (a.lse)
+                    a.lse[row_at(tid)] = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
+            }
+            if (tid < 64) sh->m[tid] = -INFINITY;               // for the next item
             if (tid == 0 && !whole) {
                 int* ps = a.part_state + cta * 8;
                 if (w.t0 == 0) {
@@ -389,7 +425,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                     ps[0] = w.t1 == w.count ? 2 : 1;             // 2: the item's last part
                 }
             }
-            named_bar(1, 128);                                  // red is read before the next item's maxima
+            named_bar(1, 128);
         }
     }
     tc_fence_before();
