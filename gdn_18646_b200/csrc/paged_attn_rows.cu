@@ -30,15 +30,13 @@ struct RowsShape {
     static constexpr int Q_BYTES = HALVES * N * 128;            // one of two buffers
     static constexpr int P_BYTES = 2 * N * 128;                 // 128 positions as two halves; one of two buffers
     // D 64: the MMA (M 128) reads 16 KB past a V tile for result lanes that nobody uses
-    static constexpr int L_BYTES = N * 128 * 4;                 // every thread's part of the rows' sums
-    static constexpr int USED = 2 * Q_BYTES + 2 * P_BYTES + L_BYTES + 3072;
+    static constexpr int USED = 2 * Q_BYTES + 2 * P_BYTES + 3072;
     static constexpr int AFTER = USED > 16384 ? USED : 16384;
     static constexpr int FIT = (232448 - 1024 - AFTER) / STAGE;
     static constexpr int STAGES = FIT < 12 ? FIT : 12;
     static constexpr int OFF_Q = STAGES * STAGE;
     static constexpr int OFF_P = OFF_Q + 2 * Q_BYTES;
-    static constexpr int OFF_L = OFF_P + 2 * P_BYTES;
-    static constexpr int OFF_BAR = OFF_L + L_BYTES;
+    static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
     static constexpr int SMEM = 1024 + OFF_Q + AFTER;
     static constexpr int COLS = N == 16 ? 64 : N == 32 ? 128 : 256;     // TMEM: two S buffers, O
     static constexpr int T_O = 2 * N;
@@ -84,6 +82,23 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
                  "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
                  "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
                  : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float (&v)[N]) {
+    if constexpr (N == 16) {
+        uint32_t r[16];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 32; ++i) tmem_ld32(taddr + i * 32, reinterpret_cast<float(&)[32]>(v[i * 32]));
+    }
+    tmem_ld_wait();
 }
 // Eight rows' maxima (or sums) over the warp's lanes: halves of the rows go to halves of the
 // lanes, so lanes 4 i .. 4 i + 3 end with row i's.
@@ -248,14 +263,14 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         }
     } else {
         // ---------------- softmax and epilogue: thread = position of the tile, then value index.
-        // Eight rows at a time in loops that are not unrolled: with all rows unrolled the code did
-        // not stay in the instruction cache, and an item of one tile took 11 us (N 16) to 24 us
-        // (N 64).  No early way out of a tile: a wait that gave up returns, and all warps keep
+        // What a tile always does is unrolled over the rows; the new maximum, the rescale and the
+        // end of an item are loops over eight rows, because with those unrolled the code did not
+        // stay in the instruction cache (an item of one tile took 11 us at N 16, 24 us at N 64).
+        // No early way out of a tile: a wait that gave up returns, and all warps keep
         // meeting at the barriers until their walk ends.
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         const float c = a.scale * 1.4426950408889634f;
         uint8_t* const p_base = sm + S::OFF_P + (tid >> 6) * (N * 128);
-        float* const l = reinterpret_cast<float*>(sm + S::OFF_L) + tid;                 // l[row * 128]
         uint32_t done = 0, items = 0;
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
@@ -282,8 +297,9 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             int lo0, hi0, lo1, hi1;                             // what the first and the last token see
             w.s.range(a, w.item * tt, w.item * tt, lo0, hi0);
             w.s.range(a, w.item * tt + toks - 1, w.item * tt + toks - 1, lo1, hi1);
-#pragma unroll 1
-            for (int r = 0; r < nr; ++r) l[r * 128] = 0.f;
+            float l[N];                                         // this thread's part of the rows' sums
+#pragma unroll
+            for (int r = 0; r < N; ++r) l[r] = 0.f;
 #pragma unroll 1
             for (int j = w.t0; j < w.t1; ++j, ++done) {
                 const uint32_t buf = done & 1u, s_col = tmem + lanes + buf * N;
@@ -297,29 +313,30 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                     if (a.window > 0) to = min(max(tok + a.window, 0), N) * a.group;
                     if (pos >= w.s.kv) from = N;
                 }
-                float s[8];
-                auto load = [&](int q) {
-                    tmem_ld8(s_col + q, s);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (q + i < from || q + i >= to) s[i] = -INFINITY;
-                };
                 wait_at(smem_u32(&sh->s_full[buf]), (done >> 1) & 1u, a.err, dead);
                 tc_fence_after();
-                bool grow = false;                              // m = -inf: true for any finite s
-#pragma unroll 1
-                for (int q = 0; q < nr; q += 8) {
-                    load(q);
+                float s[N];
+                tmem_ld_rows<N>(s_col, s);
+                if (from > 0 || to < N) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[i] - sh->m[q + i]) * c > 8.f;
+                    for (int r = 0; r < N; ++r)
+                        if (r < from || r >= to) s[r] = -INFINITY;
+                }
+                bool grow = false;                              // m = -inf: true for any finite s
+#pragma unroll
+                for (int q = 0; q < N; q += 8) {
+                    if (q >= nr) break;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[q + i] - sh->m[q + i]) * c > 8.f;
                 }
                 if (any_of_128(grow)) {
 #pragma unroll 1
                     for (int q = 0; q < nr; q += 8) {
-                        if (nr > 8) load(q);
                         float x[8];
+                        tmem_ld8(s_col + q, x);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = s[i];
+                        for (int i = 0; i < 8; ++i)
+                            if (q + i < from || q + i >= to) x[i] = -INFINITY;
                         const float top = reduce8<true>(x);
                         if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = top;
                     }
@@ -339,26 +356,25 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                             float o[8];
                             tmem_ld8(tmem + lanes + S::T_O + q, o);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float f = q + i < nr ? sh->f[q + i] : 1.f;
-                                o[i] *= f;
-                                if (q + i < nr) l[(q + i) * 128] *= f;
-                            }
+                            for (int i = 0; i < 8; ++i) o[i] *= q + i < nr ? sh->f[q + i] : 1.f;
                             tmem_st8(tmem + lanes + S::T_O + q, o);
                         }
                         tmem_st_wait();
+#pragma unroll
+                        for (int r = 0; r < N; ++r)
+                            if (r < nr) l[r] *= sh->f[r];
                     }
                 }
                 uint8_t* const pb = p_base + buf * S::P_BYTES;
                 // rows past the item's go with the last eight (their columns go nowhere)
-#pragma unroll 1
-                for (int q = 0; q < nr; q += 8) {
-                    if (nr > 8) load(q);
+#pragma unroll
+                for (int q = 0; q < N; q += 8) {
+                    if (q >= nr) break;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float m = sh->m[q + i];
-                        const float p = ex2_approx(fmaf(s[i], c, m == -INFINITY ? 0.f : -m * c));
-                        if (q + i < nr) l[(q + i) * 128] += p;
+                        const float p = ex2_approx(fmaf(s[q + i], c, m == -INFINITY ? 0.f : -m * c));
+                        l[q + i] += p;
                         *reinterpret_cast<uint16_t*>(pb + sw128_off(q + i, tid & 63)) = f32_to_bf16_bits(p);
                     }
                 }
@@ -368,11 +384,12 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                 if (lane == 0) mbar_arrive(&sh->p_full[buf]);
             }
             // the sums of the threads, in order
-#pragma unroll 1
-            for (int q = 0; q < nr; q += 8) {
+#pragma unroll
+            for (int q = 0; q < N; q += 8) {
+                if (q >= nr) break;
                 float x[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = q + i < nr ? l[(q + i) * 128] : 0.f;
+                for (int i = 0; i < 8; ++i) x[i] = l[q + i];
                 const float sum = reduce8<false>(x);
                 if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = sum;
             }
