@@ -26,7 +26,7 @@
 //   P (bf16) overwrites S in TMEM      (rounded to bf16: 2^-9 rms of each weight)
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // The tensor core works for one row tile while the softmax of the other runs.  Items of
-// at most 64 rows (a decode step) go to paged_attn_rows.cu.
+// at most 32 rows (a decode step) go to paged_attn_rows.cu.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -40,6 +40,7 @@ namespace {
 
 constexpr int QT = 2;                 // row tiles of 128 per item
 constexpr int kItemCost = 3;          // kv tiles that starting and ending an item is worth, beside its tiles
+constexpr int kWholeTiles = 8;        // items of so many kv tiles are not cut when there are few
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
 constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
 
@@ -574,15 +575,24 @@ __global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_co
     }
 }
 
-// Kernel by the rows (tokens x heads of a group) of the longest chunk: up to 64 the one for
-// few rows, which keeps them in the MMA's narrow dimension; else the one with 128-row tiles
-// (a chunk of 8 tokens of 8 heads over 32768 positions: 45 us there, 97 us here).
-bool few_rows(int max_q, int group) { return static_cast<long>(max_q) * group <= 64; }
+// Kernel by the rows (tokens x heads of a group) of the longest chunk: up to 32 the one for
+// few rows, which keeps them in the MMA's narrow dimension, else the one with 128-row tiles.
+// Both sides, us: 25 rows (16 x 5 tokens over 4096, head dim 64) 51 / 61; 40 rows (5 tokens over
+// 32768) 58 / 62; 64 rows (4 tokens x 16 heads over 4096) 64 / 50, (8 x 8 over 32768) 72 / 62.
+bool few_rows(int max_q, int group) { return static_cast<long>(max_q > 1 ? max_q : 1) * group <= 32; }
 
 // Rows of an unfinished item's part.
 int part_rows(int max_q, int group) {
-    const int rows = (max_q > 1 ? max_q : 1) * group;
-    return !few_rows(max_q, group) ? QT * 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    return !few_rows(max_q, group) ? QT * 128 : max_q * group <= 16 && group <= 16 ? 16 : 32;
+}
+
+// CTAs for a call whose items are few and short enough to be left whole, one per item, so
+// that no second launch has to join parts; 0: the work is cut.  Both sides on the device, us,
+// whole / cut: 1 token over 1000 positions 13.0 / 13.2 (and 3 less on the host), 8 x 1 over 1000
+// 13.1 / 14.8, 100 over 1000 24.5 / 29.7, 1 over 2000 19.2 / 12.7, 100 over 2000 38 / 33.
+int whole_items(int B, int T, int n_kv, int item_tokens, int max_kv) {
+    const long most = static_cast<long>(n_kv) * (static_cast<long>(B) + T / item_tokens);
+    return most <= kMaxCtas && max_kv <= kWholeTiles * kTile ? static_cast<int>(most) : 0;
 }
 
 template <int D>
@@ -598,9 +608,9 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     });
     if (attr[dev] != cudaSuccess)
         return fail(GDN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(attr[dev]));
-    paged_attn_kernel<D><<<kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
+    paged_attn_kernel<D><<<a.whole ? a.whole : kMaxCtas, S::THREADS, S::SMEM, st>>>(maps, a);
     int rc = launch_status(name);
-    if (rc != GDN_OK) return rc;
+    if (rc != GDN_OK || a.whole) return rc;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -676,7 +686,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.group = Hq / pv.n_kv;
     const bool few = few_rows(max_q, a.group);
     a.part_rows = part_rows(max_q, a.group);
-    a.tile_tokens = (few ? a.part_rows : 128) / a.group;
+    a.tile_tokens = (few ? a.part_rows : 128) / a.group;        // at least 1: group <= 64, and <= part_rows for few rows
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.causal = causal != 0;
@@ -684,6 +694,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.scale = scale == 0.f ? 1.f / sqrtf(static_cast<float>(D)) : scale;
     a.err = device_error_word();
     a.item_cost = few ? 1 : kItemCost;
+    a.whole = whole_items(B, Ttot, pv.n_kv, few ? a.tile_tokens : QT * a.tile_tokens, max_kv);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_state = reinterpret_cast<int*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + part_state_bytes());

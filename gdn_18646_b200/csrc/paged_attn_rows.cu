@@ -1,14 +1,14 @@
 // paged_attn_rows.cu -- paged attention where an item has few rows (a decode step, a few
-// drafted tokens: tokens x query heads of a kv head <= 64), on tcgen05.
+// drafted tokens: tokens x query heads of a kv head <= 32), on tcgen05.
 //
 // The mathematics, the rows and the line of work are those of paged_attn.cu.  Here the
 // keys stand in the MMA's wide dimension and the rows in its narrow one:
-//   S^T = K Q^T      M 128 positions, N rows (16, 32 or 64), SS    -> TMEM, lane = position
+//   S^T = K Q^T      M 128 positions, N rows (16 or 32), SS        -> TMEM, lane = position
 //   P^T (bf16)       thread = position, written to shared memory as the next B operand
 //   O^T += V^T P^T   M = D, N rows, SS (V as it lies, MN-major)    -> TMEM, lane = value index
 // so a tile of 128 keys costs N/128 of the tensor work of a 128-row tile, and its softmax
-// 128 threads x N exponentials instead of one warp x 128 a row (a tile took 2050 cycles that
-// way, which bound the kernel as soon as the clock fell; HBM delivers one in 2800).  The running
+// 128 threads x N exponentials instead of one warp x 128 a row (with rows in the wide
+// dimension a tile took 2050 cycles, near the 2800 in which HBM delivers one, and the clock fell).  The running
 // maximum is the same for all threads; only when some weight would pass 2^8 do they
 // reduce a new one and rescale.  The sums l stay per thread until the item ends.
 //
@@ -38,7 +38,7 @@ struct RowsShape {
     static constexpr int OFF_P = OFF_Q + 2 * Q_BYTES;
     static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
     static constexpr int SMEM = 1024 + OFF_Q + AFTER;
-    static constexpr int COLS = N == 16 ? 64 : N == 32 ? 128 : 256;     // TMEM: two S buffers, O
+    static constexpr int COLS = N == 16 ? 64 : 128;             // TMEM: two S buffers, O
     static constexpr int T_O = 2 * N;
     static_assert(SMEM <= 232448, "shared memory");
 };
@@ -49,8 +49,9 @@ struct RowsBars {
     uint64_t s_full[2], p_full[2];
     uint64_t o_full, pv_done;
     PieceScratch scratch;
-    float m[64], f[64];               // per row: reference maximum, factor of a rescale
-    float red[4][64];                 // per warp and row: tile maxima, then sums
+    alignas(16) float m[32];
+    float f[32];                      // per row: reference maximum, factor of a rescale
+    float red[4][32];                 // per warp and row: tile maxima, then sums
     uint32_t tmem;
     int abort;
 };
@@ -99,6 +100,12 @@ __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float (&v)[N]) {
         for (int i = 0; i < N / 32; ++i) tmem_ld32(taddr + i * 32, reinterpret_cast<float(&)[32]>(v[i * 32]));
     }
     tmem_ld_wait();
+}
+// eight values of shared memory (16-byte aligned)
+__device__ __forceinline__ void rows8(const float* at, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 // Eight rows' maxima (or sums) over the warp's lanes: halves of the rows go to halves of the
 // lanes, so lanes 4 i .. 4 i + 3 end with row i's.
@@ -265,7 +272,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         // ---------------- softmax and epilogue: thread = position of the tile, then value index.
         // What a tile always does is unrolled over the rows; the new maximum, the rescale and the
         // end of an item are loops over eight rows, because with those unrolled the code did not
-        // stay in the instruction cache (an item of one tile took 11 us at N 16, 24 us at N 64).
+        // stay in the instruction cache (an item of one tile took 11 us at N 16).
         // No early way out of a tile: a wait that gave up returns, and all warps keep
         // meeting at the barriers until their walk ends.
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
@@ -274,7 +281,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         uint32_t done = 0, items = 0;
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
-        if (tid < 64) sh->m[tid] = -INFINITY;
+        if (tid < 32) sh->m[tid] = -INFINITY;
         named_bar(1, 128);
         Walk w;
         for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
@@ -326,8 +333,10 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
 #pragma unroll
                 for (int q = 0; q < N; q += 8) {
                     if (q >= nr) break;
+                    float m[8];
+                    rows8(sh->m + q, m);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[q + i] - sh->m[q + i]) * c > 8.f;
+                    for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[q + i] - m[i]) * c > 8.f;
                 }
                 if (any_of_128(grow)) {
 #pragma unroll 1
@@ -356,7 +365,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                             float o[8];
                             tmem_ld8(tmem + lanes + S::T_O + q, o);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] *= q + i < nr ? sh->f[q + i] : 1.f;
+                            for (int i = 0; i < 8; ++i) o[i] *= q + i < nr ? sh->f[q + i] : 1.f;   // rows past the item's: any
                             tmem_st8(tmem + lanes + S::T_O + q, o);
                         }
                         tmem_st_wait();
@@ -370,12 +379,14 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
 #pragma unroll
                 for (int q = 0; q < N; q += 8) {
                     if (q >= nr) break;
+                    float m[8], p[8];                           // all loads before the stores, which might alias them
+                    rows8(sh->m + q, m);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) p[i] = ex2_approx(fmaf(s[q + i], c, m[i] == -INFINITY ? 0.f : -m[i] * c));
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float m = sh->m[q + i];
-                        const float p = ex2_approx(fmaf(s[q + i], c, m == -INFINITY ? 0.f : -m * c));
-                        l[q + i] += p;
-                        *reinterpret_cast<uint16_t*>(pb + sw128_off(q + i, tid & 63)) = f32_to_bf16_bits(p);
+                        l[q + i] += p[i];
+                        *reinterpret_cast<uint16_t*>(pb + sw128_off(q + i, tid & 63)) = f32_to_bf16_bits(p[i]);
                     }
                 }
                 fence_async_smem();
@@ -401,18 +412,19 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * a.part_rows;
 #pragma unroll 1
             for (int q = 0; q < nr; q += 8) {
-                float o[8];
+                float o[8], sum[8];                             // loads before stores here too
                 tmem_ld8(tmem + lanes + S::T_O + q, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] = (sh->red[0][q + i] + sh->red[1][q + i]) + (sh->red[2][q + i] + sh->red[3][q + i]);
                 int tok = q / a.group, g = q - tok * a.group;
                 if (tid < D)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int r = q + i;
-                        const float sum = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
                         if (r < nr) {
                             if (whole)
                                 a.out[(at0 + static_cast<long>(tok) * a.Hq + g) * D + tid] =
-                                    f32_to_bf16_bits(sum == 0.f ? 0.f : __fdividef(o[i], sum));
+                                    f32_to_bf16_bits(sum[i] == 0.f ? 0.f : __fdividef(o[i], sum[i]));
                             else
                                 a.part_o[(slot + r) * D + tid] = o[i];
                         }
@@ -430,7 +442,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                 else if (a.lse)
                     a.lse[row_at(tid)] = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
             }
-            if (tid < 64) sh->m[tid] = -INFINITY;               // for the next item
+            if (tid < 32) sh->m[tid] = -INFINITY;               // for the next item
             if (tid == 0 && !whole) {
                 int* ps = a.part_state + cta * 8;
                 if (w.t0 == 0) {
@@ -552,11 +564,13 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     cfg.attrs = pdl;
     cfg.numAttrs = launch_overlap() ? 1 : 0;
     cfg.stream = st;
-    cfg.gridDim = dim3(kMaxCtas);
+    cfg.gridDim = dim3(a.whole ? a.whole : kMaxCtas);
     cfg.blockDim = dim3(kRowsThreads);
     cfg.dynamicSmemBytes = S::SMEM;
     cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_rows_kernel<D, N>, maps, a);
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
+    if (a.whole) return launch_status(name);
+    cfg.gridDim = dim3(kMaxCtas);
     cfg.numAttrs = 1;                                           // starts while the first kernel ends
     cfg.blockDim = dim3(512);
     cfg.dynamicSmemBytes = 0;
@@ -568,8 +582,8 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int launch_attn_rows(const AttnMaps& maps, const AttnArgs& a, int D, cudaStream_t st) {
-    if (D == 64) return a.part_rows == 16 ? launch<64, 16>(maps, a, st) : a.part_rows == 32 ? launch<64, 32>(maps, a, st) : launch<64, 64>(maps, a, st);
-    return a.part_rows == 16 ? launch<128, 16>(maps, a, st) : a.part_rows == 32 ? launch<128, 32>(maps, a, st) : launch<128, 64>(maps, a, st);
+    if (D == 64) return a.part_rows == 16 ? launch<64, 16>(maps, a, st) : launch<64, 32>(maps, a, st);
+    return a.part_rows == 16 ? launch<128, 16>(maps, a, st) : launch<128, 32>(maps, a, st);
 }
 
 }  // namespace gdn

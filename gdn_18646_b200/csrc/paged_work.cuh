@@ -24,6 +24,7 @@ struct AttnArgs {
     int max_q, max_kv, causal, window;
     float scale;
     int item_cost;
+    int whole;                        // a CTA per item, no cut: few items of few tiles
     unsigned int* err;
     int* part_state;                  // [ctas][8]: what a CTA left unfinished
     int part_rows;                    // rows of a part
@@ -137,6 +138,7 @@ struct Seq {
     // cost of the items before `q` of one kv head
     __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
         if (q == 0) return 0;
+        if (a.whole) return q;
         long long s = static_cast<long long>(q) * a.item_cost;
         if (q <= 6) {                                           // as they are: the closed form costs as much as six
             for (int i = 0; i < q; ++i) {
@@ -191,12 +193,17 @@ struct Walk {
     __device__ __forceinline__ bool valid() const { return left > 0; }
     __device__ __forceinline__ void set(const AttnArgs& a, int tt) {
         s.tiles(a, item, tt, first, count, lo, hi);
+        if (a.whole) {
+            t0 = 0;
+            t1 = count;
+            return;
+        }
         const long long end = min(static_cast<long long>(count + a.item_cost), skip + left);
         t0 = max(skip - a.item_cost, 0);
         t1 = max(static_cast<int>(end) - a.item_cost, 0);
     }
     __device__ __forceinline__ void next(const AttnArgs& a, int tt) {
-        left -= count + a.item_cost - skip;
+        left -= a.whole ? 1 : count + a.item_cost - skip;
         skip = 0;
         if (left <= 0) return;
         if (++item == s.items) {
@@ -247,7 +254,7 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
         if (w < warp) start += v;
         total += v;
     }
-    const long long most = (total + kMinPiece - 1) / kMinPiece;
+    const long long most = a.whole ? total : (total + kMinPiece - 1) / kMinPiece;
     const int pieces = most < gridDim.x ? static_cast<int>(most) : gridDim.x;
     if (blockIdx.x < pieces) {
         // total x / pieces without a wide product; the quotient in two short divisions (total < 2^48)
@@ -360,7 +367,7 @@ inline size_t part_state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * si
 inline size_t part_ml_bytes(int rows) { return static_cast<size_t>(kMaxCtas) * 2 * rows * 2 * sizeof(float); }
 inline size_t part_o_bytes(int rows, int D) { return static_cast<size_t>(kMaxCtas) * 2 * rows * D * sizeof(float); }
 
-// paged_attn_rows.cu: at most 64 rows per item (a decode step, a few drafted tokens)
+// paged_attn_rows.cu: at most 32 rows per item (a decode step, a few drafted tokens)
 int launch_attn_rows(const AttnMaps& maps, const AttnArgs& a, int D, cudaStream_t st);
 
 }  // namespace gdn
