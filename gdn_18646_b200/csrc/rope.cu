@@ -85,7 +85,9 @@ template <int D, bool INTERLEAVED, bool APPEND>
 __global__ void __launch_bounds__(32 * kWarps) rope_kernel(const RopeArgs a) {
     constexpr int UNITS = D / 16;              // lanes per head
     constexpr int HPW = 32 / UNITS;            // heads a warp turns at once
-    constexpr int BATCH = 3;                   // such groups of heads whose loads are in flight together
+    // such groups of heads whose loads are in flight together (us at 11 K tokens of 20 heads, with 3
+    // and 5: append 23.1, 22.0; at 16 K tokens of 32 heads: plain 44.0, 45.9)
+    constexpr int BATCH = APPEND ? 5 : 3;
     const int lane = threadIdx.x & 31, unit = lane % UNITS, sub = lane / UNITS;
     const uint32_t job = blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int t = static_cast<int>(job / a.splits), split = static_cast<int>(job - t * a.splits);
@@ -229,18 +231,20 @@ int check_rows(const char* name, const char* what, const void* p, long ld, int H
     return GDN_OK;
 }
 
-// Warps per token: one when the tokens alone fill the GPU (its sines are then computed
-// once for all heads), one per group of heads when there are few tokens and latency counts.
-int splits_for(int T, int heads, int D) {
-    const int groups = (heads + 512 / D - 1) / (512 / D);
-    if (T >= 148 * 16) return 1;
-    const int want = (148 * 16 + T - 1) / T;
+// Warps per token: few tokens are spread over warps by groups of heads, down to one group
+// each, as latency counts.  With tokens enough for the GPU a warp of the append takes a
+// token whole (finding its page costs more than its heads: 11 K tokens 23.1 us with one warp a
+// token, 23.7 with two, 33.6 with three), of the plain rotation about half of one (16 K
+// tokens 44.0 us with one warp, 42.0 with two, 42.5 with three).
+int splits_for(int T, int heads, int D, bool append) {
+    const int groups = (heads + 512 / D - 1) / (512 / D), warps = 148 * (append ? 16 : 128);
+    const int want = T >= warps ? 1 : (warps + T - 1) / T;
     return want < groups ? want : groups;
 }
 
 template <bool APPEND>
 int launch(const char* name, RopeArgs& a, int style, int D, cudaStream_t st) {
-    a.splits = splits_for(a.T, a.Hq + a.Hk * (APPEND ? 2 : 1), D);
+    a.splits = splits_for(a.T, a.Hq + a.Hk * (APPEND ? 2 : 1), D, APPEND);
     const long jobs = static_cast<long>(a.T) * a.splits;
     const dim3 grid(static_cast<unsigned>((jobs + kWarps - 1) / kWarps));
 #define GDN_ROPE(DD)                                                                              \
