@@ -9,8 +9,8 @@
 // are exact for any m near the maximum, so a smaller growth leaves m and o where they are.
 //
 // Rows.  The G query heads that share a kv head are packed with their tokens into rows
-// (row = token G + g), floor(128 / G) tokens to a tile of 128, so a decode step and a
-// chunk run the same kernel and a key is read once for its whole group.
+// (row = token G + g), floor(128 / G) tokens to a tile of 128, so that a key is read once
+// for its whole group.
 //
 // Work.  An item is (sequence, kv head, two row tiles); its kv tiles are the ones that some
 // row of it sees.  All kv tiles of all items, with a constant cost per item, form one line
@@ -27,6 +27,12 @@
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // The tensor core works for one row tile while the softmax of the other runs.  Items of
 // at most 32 rows (a decode step) go to paged_attn_rows.cu.
+//
+// What bounds it.  A kv tile of both row tiles is 32 MMAs of about 61 cycles and 128 x 256
+// exponentials, 2048 cycles either; three pairs of eight take a polynomial on the FMA pipe
+// (2048 new tokens over 32768, 16 heads on 2, head dim 128: 572 us without, 496 with three
+// of eight, 555 with half of them).  In sustained passes the power cap sets the clock: 496 us
+// (1.07 PFLOP/s) at 1.6 GHz, 438 (1.22) in the first passes at 1.97 GHz.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -690,7 +696,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.causal = causal != 0;
-    a.window = window;
+    a.window = window >= max_kv ? 0 : window;                   // as wide as the cache: none (and no sum overflows)
     a.scale = scale == 0.f ? 1.f / sqrtf(static_cast<float>(D)) : scale;
     a.err = device_error_word();
     a.item_cost = few ? 1 : kItemCost;

@@ -20,10 +20,10 @@ struct AttnArgs {
     long table_ld;
     int num_pages, page_shift;
     int B, T, Hq, n_kv, group;        // group: query heads per kv head
-    int tile_tokens;                  // floor(128 / group)
+    int tile_tokens;                  // tokens of a row tile: floor(its rows / group)
     int max_q, max_kv, causal, window;
     float scale;
-    int item_cost;
+    int item_cost;                    // kv tiles that an item is worth beside its tiles
     int whole;                        // a CTA per item, no cut: few items of few tiles
     unsigned int* err;
     int* part_state;                  // [ctas][8]: what a CTA left unfinished
@@ -255,8 +255,8 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
         total += v;
     }
     const long long most = a.whole ? total : (total + kMinPiece - 1) / kMinPiece;
-    const int pieces = most < gridDim.x ? static_cast<int>(most) : gridDim.x;
-    if (blockIdx.x < pieces) {
+    const int pieces = most < gridDim.x ? static_cast<int>(most) : static_cast<int>(gridDim.x);
+    if (static_cast<int>(blockIdx.x) < pieces) {
         // total x / pieces without a wide product; the quotient in two short divisions (total < 2^48)
         const uint32_t top = static_cast<uint32_t>(total >> 24), q1 = top / pieces;
         const uint32_t low = (top - q1 * pieces) << 24 | static_cast<uint32_t>(total & 0xffffff), q0 = low / pieces;

@@ -897,6 +897,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0:
         return (out, lse) if return_lse else out
+    window = min(window, 0x7FFFFFFF)
     ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
     if workspace is None:
         workspace = q.new_empty(ws_bytes // 2)

@@ -58,9 +58,8 @@ class Batch:
         kv = self.lens[b][1]
         x = cache if self.layout == "bthd" else cache.transpose(1, 2)
         pages = self.table_np[b, :-(-kv // self.page)]
-        x = x.double().cpu().numpy()
         out = np.full((len(pages), self.page, self.Hk, self.D), np.nan)
-        for i, p in enumerate(pages):
-            if 0 <= p < self.pages:
-                out[i] = x[p]
+        use = np.flatnonzero((pages >= 0) & (pages < self.pages))
+        if len(use):
+            out[use] = x[pages[use].tolist()].double().cpu().numpy()
         return out.reshape(-1, self.Hk, self.D)[:kv]

@@ -95,11 +95,52 @@ def test_window(cuda_device, lens, Hq, Hk, D, page, window):
     check(b, out, lse, window=window, rows=24)
 
 
+@pytest.mark.parametrize("lens,Hq,Hk,D,page", [SINGLE[2], SINGLE[7], CHUNKS[3]])
+def test_windows_wider_than_the_cache(cuda_device, lens, Hq, Hk, D, page):
+    import torch
+    b = Batch(lens, Hq, Hk, D, page, seed=13)
+    want = run(b)
+    longest = max(kv for _, kv in lens)
+    for window in (longest, 2 ** 31 - 1, 2 ** 40):
+        assert torch.equal(run(b, window=window), want)
+    check(b, run(b, window=longest - 1), window=longest - 1, rows=24)
+
+
 @pytest.mark.parametrize("lens,Hq,Hk,D,page", [SINGLE[1], SINGLE[7], CHUNKS[2], CHUNKS[4], CHUNKS[6]])
 def test_all_positions_and_scale(cuda_device, lens, Hq, Hk, D, page):
     b = Batch(lens, Hq, Hk, D, page, seed=2)
     out, lse = run(b, causal=False, scale=0.3, return_lse=True)
     check(b, out, lse, scale=0.3, causal=False, rows=24)
+
+
+@pytest.mark.parametrize("few", [True, False])
+def test_many_sequences(cuda_device, few):
+    """More sequences than a CTA has threads, many of them without tokens or positions."""
+    rng = np.random.default_rng(17)
+    lens = [(int(rng.integers(0, 3 if few else 24)), int(rng.integers(0, 90))) for _ in range(700)] + [(1, 1500), (2, 0), (0, 700)]
+    b = Batch(lens, 6, 2, 64, 16, seed=21)
+    out, lse = run(b, return_lse=True)
+    check(b, out, lse)
+    b = Batch([(n, 0) for n, _ in lens[:50]], 6, 2, 64, 16, seed=22)          # nothing anywhere
+    out, lse = run(b, return_lse=True)
+    assert float(out.abs().max()) == 0 and bool((lse == -np.inf).all())
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_batches(cuda_device, seed):
+    rng = np.random.default_rng(100 + seed)
+    G, Hk, D = int(rng.choice([1, 2, 3, 5, 8, 13, 32, 64])), int(rng.choice([1, 2, 3])), int(rng.choice([64, 128]))
+    most = int(rng.choice([1, 4, 40, 300]))
+    lens = []
+    for _ in range(int(rng.integers(1, 9))):
+        n = int(rng.integers(0, most + 1))
+        lens.append((n, max(0, n + int(rng.integers(-2, 1200)) if rng.random() < 0.8 else int(rng.integers(0, 40)))))
+    lens.append((most, most + int(rng.integers(0, 3000))))
+    window = int(rng.choice([0, 0, 1, 63, 128, 500]))
+    b = Batch(lens, G * Hk, Hk, D, int(rng.choice([16, 32, 128, 512])), str(rng.choice(["bthd", "bhtd"])),
+              str(rng.choice(["plain", "pair"])), window=window, seed=seed)
+    out, lse = run(b, window=window, return_lse=True)
+    check(b, out, lse, window=window, rows=10)
 
 
 def test_large_scores(cuda_device):
