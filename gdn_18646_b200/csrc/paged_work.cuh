@@ -313,12 +313,17 @@ __device__ __forceinline__ bool load_tiles(const AttnArgs& a, const AttnMaps& ma
     const int units = kTile / page_rows * HALVES;               // <= 16
     const int my_page = lane / HALVES, my_half = lane % HALVES;
     const int* row = a.table + w.b * a.table_ld;
+    // the table is read a tile ahead, so that its latency is not between the copies
+    int pos = (w.first + w.t0) * kTile + my_page * page_rows;
+    auto seen = [&]() { return lane < units && pos + page_rows > w.lo && pos < w.hi; };
+    int ahead = seen() ? row[pos >> a.page_shift] : 0;
     for (int j = w.t0; j < w.t1; ++j) {
-        const int pos = (w.first + j) * kTile + my_page * page_rows;
-        const bool mine = lane < units && pos + page_rows > w.lo && pos < w.hi;
-        int page = 0;
+        const bool mine = seen();
+        int page = ahead;
+        const int in_page = pos & ((1 << a.page_shift) - 1);
+        pos += kTile;
+        ahead = j + 1 < w.t1 && seen() ? row[pos >> a.page_shift] : 0;
         if (mine) {
-            page = row[pos >> a.page_shift];
             if (page < 0 || page >= a.num_pages) {
                 page = a.num_pages;                             // outside: the copy fills zeros
                 atomicOr(a.err, DERR_PAGED);
@@ -331,7 +336,7 @@ __device__ __forceinline__ bool load_tiles(const AttnArgs& a, const AttnMaps& ma
             __syncwarp();
             if (mine)
                 tma_load_4d(kv_ring + stage * STAGE + my_half * 16384 + my_page * page_rows * 128, kv ? &maps.v : &maps.k,
-                            &full[stage], my_half * 64, pos & ((1 << a.page_shift) - 1), w.head, page);
+                            &full[stage], my_half * 64, in_page, w.head, page);
             ++issued;
             if (++stage == STAGES) {
                 stage = 0;
