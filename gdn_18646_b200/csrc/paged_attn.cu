@@ -176,7 +176,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                         tma_load_3d(sm + (t * S::HALVES + h) * 16384, &maps.q, &sh->q_full, h * 64, w.head * a.group,
                                     w.s.c0 + w.item * tt + t * a.tile_tokens);
             }
-            if (!load_tiles<D, S::STAGES>(a, maps, w, sm + S::OFF_KV, sh->full, sh->empty, stage, phase, issued, dead)) break;
+            if (!load_tiles<D, S::STAGES, 1>(a, maps, w, sm + S::OFF_KV, sh->full, sh->empty, stage, phase, issued, dead)) break;
         }
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer (one lane; the warp together clears unseen value rows).

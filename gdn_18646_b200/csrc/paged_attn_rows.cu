@@ -12,7 +12,9 @@
 // maximum is the same for all threads; only when some weight would pass 2^8 do they
 // reduce a new one and rescale.  The sums l stay per thread until the item ends.
 //
-// Bound by HBM: K and V are read once, 32 KB (D 128) per ring stage.
+// Bound by HBM: K and V are read once, 32 KB (D 128) per ring stage.  256 decode steps over up to
+// 8192 positions, 16 heads on 2: 166 us, 6.2 TB/s; 2 over up to 131072, 32 heads on 4: 73 us, 5.5 TB/s,
+// of which about 8 us are the start of the pieces and the join.
 #include <mutex>
 
 #include "common.cuh"
@@ -21,7 +23,12 @@
 namespace gdn {
 namespace {
 
-constexpr int kRowsThreads = 192;     // 4 softmax warps, MMA, load
+// A warp issues a copy in about 50 cycles, and a tile is 2 x 128 / page size x D / 64 of them,
+// so with small pages the issue, not HBM, sets the pace of one warp.  256 sequences of up to 8192
+// positions in pages of 16, head dim 128, with 1 / 2 / 4 warps: 194 / 169 / 166 us; 1 token over
+// 1000 positions: 18.7 / 14.8 / 13.7; pages of 64, 2 x 131072 positions: 72.5 / 72.7 / 73.2.
+constexpr int kLoadWarps = 4;
+constexpr int kRowsThreads = 160 + 32 * kLoadWarps;      // 4 softmax warps, MMA, load
 
 template <int D, int N>
 struct RowsShape {
@@ -144,7 +151,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
 
     if (tid == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(&sh->full[i], 1);
+            mbar_init(&sh->full[i], kLoadWarps);
             mbar_init(&sh->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -183,21 +190,25 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             phase ^= 1u;
         }
     };
-    if (warp == LOAD_WARP) {
-        // ---------------- TMA producer
+    if (warp >= LOAD_WARP) {
+        // ---------------- TMA producers, each with a share of every tile's copies; the first also loads Q
         Walk w;
         for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
             if (w.t0 >= w.t1) continue;
-            const int qb = q_loads & 1;
-            if (!warp_wait(&sh->q_empty[qb], ((q_loads >> 1) & 1u) ^ 1u, a.err, dead)) break;
-            ++q_loads;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&sh->q_full[qb], S::HALVES * tt * a.group * 128);
-                for (int h = 0; h < S::HALVES; ++h)
-                    tma_load_3d(sm + S::OFF_Q + qb * S::Q_BYTES + h * N * 128, &maps.q, &sh->q_full[qb], h * 64,
-                                w.head * a.group, w.s.c0 + w.item * tt);
+            if (warp == LOAD_WARP) {
+                const int qb = q_loads & 1;
+                if (!warp_wait(&sh->q_empty[qb], ((q_loads >> 1) & 1u) ^ 1u, a.err, dead)) break;
+                ++q_loads;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh->q_full[qb], S::HALVES * tt * a.group * 128);
+                    for (int h = 0; h < S::HALVES; ++h)
+                        tma_load_3d(sm + S::OFF_Q + qb * S::Q_BYTES + h * N * 128, &maps.q, &sh->q_full[qb], h * 64,
+                                    w.head * a.group, w.s.c0 + w.item * tt);
+                }
             }
-            if (!load_tiles<D, S::STAGES>(a, maps, w, sm, sh->full, sh->empty, stage, phase, issued, dead)) break;
+            if (!load_tiles<D, S::STAGES, kLoadWarps>(a, maps, w, sm, sh->full, sh->empty, stage, phase, issued, dead,
+                                                      warp - LOAD_WARP))
+                break;
         }
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer (one lane; the warp together clears unseen value rows)
@@ -459,7 +470,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
     }
     tc_fence_before();
     __syncthreads();
-    if (sh->abort && warp == LOAD_WARP) {
+    if (sh->abort && warp >= LOAD_WARP) {
         drain_ring(a, sh->full, S::STAGES, issued);
         for (uint32_t i = q_loads > 2 ? q_loads - 2 : 0; i < q_loads; ++i) mbar_wait(&sh->q_full[i & 1], (i >> 1) & 1u, a.err);
     }

@@ -303,19 +303,20 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
 
 // Loads the K and V tiles of the walk's item into the kv ring (warp together, a lane per page
 // of the tile and 64-value half); only pages that hold a position somebody sees.  False: gave up.
-template <int D, int STAGES>
+// WARPS warps share the copies of every tile, this one is `which`; each arrives at its barrier.
+template <int D, int STAGES, int WARPS>
 __device__ __forceinline__ bool load_tiles(const AttnArgs& a, const AttnMaps& maps, const Walk& w, uint8_t* kv_ring,
                                            uint64_t* full, uint64_t* empty, int& stage, uint32_t& phase, uint32_t& issued,
-                                           volatile int* dead) {
+                                           volatile int* dead, int which = 0) {
     constexpr int HALVES = D / 64, STAGE = kTile * D * 2;
     const int lane = threadIdx.x & 31;
     const int page_rows = min(1 << a.page_shift, kTile);
     const int units = kTile / page_rows * HALVES;               // <= 16
-    const int my_page = lane / HALVES, my_half = lane % HALVES;
+    const int unit = lane * WARPS + which, my_page = unit / HALVES, my_half = unit % HALVES;
     const int* row = a.table + w.b * a.table_ld;
     // the table is read a tile ahead, so that its latency is not between the copies
     int pos = (w.first + w.t0) * kTile + my_page * page_rows;
-    auto seen = [&]() { return lane < units && pos + page_rows > w.lo && pos < w.hi; };
+    auto seen = [&]() { return unit < units && pos + page_rows > w.lo && pos < w.hi; };
     int ahead = seen() ? row[pos >> a.page_shift] : 0;
     for (int j = w.t0; j < w.t1; ++j) {
         const bool mine = seen();
