@@ -13,8 +13,8 @@
 // reduce a new one and rescale.  The sums l stay per thread until the item ends.
 //
 // Bound by HBM: K and V are read once, 32 KB (D 128) per ring stage.  256 decode steps over up to
-// 8192 positions, 16 heads on 2: 166 us, 6.2 TB/s; 2 over up to 131072, 32 heads on 4: 73 us, 5.5 TB/s,
-// of which about 8 us are the start of the pieces and the join.
+// 8192 positions, 16 heads on 2: 162 us, 6.3 TB/s; 2 over up to 131072, 32 heads on 4: 73 us,
+// 5.5 TB/s, of which about 8 us are the start of the pieces and the join.
 #include <mutex>
 
 #include "common.cuh"
@@ -23,11 +23,11 @@
 namespace gdn {
 namespace {
 
-// A warp issues a copy in about 50 cycles, and a tile is 2 x 128 / page size x D / 64 of them,
-// so with small pages the issue, not HBM, sets the pace of one warp.  256 sequences of up to 8192
-// positions in pages of 16, head dim 128, with 1 / 2 / 4 warps: 194 / 169 / 166 us; 1 token over
-// 1000 positions: 18.7 / 14.8 / 13.7; pages of 64, 2 x 131072 positions: 72.5 / 72.7 / 73.2.
-constexpr int kLoadWarps = 4;
+// A warp issues a copy in about 60 cycles, and a tile is 2 x 128 / page size x D / 64 of them, so
+// with small pages the issue sets the pace of one warp while the ring fills.  With 1 / 2 / 4 warps,
+// us: 1 token over 1000 positions in pages of 16, head dim 128, 16.3 / 12.6 / 12.0; 256 sequences of
+// up to 8192 161 / 162 / 162; 2 of up to 131072 in pages of 64 72.5 / 72.8 / 73.2.
+constexpr int kLoadWarps = 2;
 constexpr int kRowsThreads = 160 + 32 * kLoadWarps;      // 4 softmax warps, MMA, load
 
 template <int D, int N>

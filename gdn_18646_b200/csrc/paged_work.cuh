@@ -73,40 +73,42 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3FFFFu) >> 4) | (lbo_bytes >> 4) << 16; }
 
-// A wait at a barrier given by its shared-memory address, for warps whose every step counts: it
-// ends with the warp together and says nothing when it gave up (the error word and *dead are
-// set then, all later waits return at once, and the warp runs on to its end over garbage).
-static __device__ __noinline__ void wait_slowly(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
-    const long long t0 = clock64(), budget = wait_budget();
-    uint32_t ok = 0;
-    while (!ok) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok || *dead) return;
-        if (clock64() - t0 > budget) {
-            if (err) atomicOr(err, DERR_TIMEOUT);
-            *dead = 1;
-            return;
-        }
-    }
-}
-__device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+// Waits at a barrier given by its shared-memory address, for warps whose every step counts: the
+// way of a barrier that is ready has no clock and no loop.
+__device__ __forceinline__ bool try_at(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (!ok) wait_slowly(bar, parity, err, dead);
+    return ok != 0;
+}
+static __device__ __noinline__ bool wait_slowly(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    const long long t0 = clock64(), budget = wait_budget();
+    while (!try_at(bar, parity)) {
+        if (*dead) return false;
+        if (clock64() - t0 > budget) {
+            if (err) atomicOr(err, DERR_TIMEOUT);
+            *dead = 1;
+            return false;
+        }
+    }
+    return true;
+}
+// Ends with the warp together and says nothing when it gave up (the error word and *dead are
+// set then, all later waits return at once, and the warp runs on to its end over garbage).
+__device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    if (!try_at(bar, parity)) wait_slowly(bar, parity, err, dead);
     __syncwarp();
 }
-
-// A wait that all lanes of a warp leave alike, also when it gives up.
+// One that all lanes of a warp leave alike; false: gave up.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, unsigned int* err, volatile int* dead) {
+    const bool ok = try_at(bar, parity);
+    return __all_sync(0xffffffffu, ok) || __all_sync(0xffffffffu, ok || wait_slowly(bar, parity, err, dead));
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* dead) {
-    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, err, dead));
+    return warp_wait(smem_u32(bar), parity, err, dead);
 }
 
 // One sequence as the kernel sees it; tt: tokens per item.
@@ -301,43 +303,63 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
     __syncthreads();
 }
 
-// Loads the K and V tiles of the walk's item into the kv ring (warp together, a lane per page
-// of the tile and 64-value half); only pages that hold a position somebody sees.  False: gave up.
-// WARPS warps share the copies of every tile, this one is `which`; each arrives at its barrier.
+// A copy of one page's rows of a kv tile, 64 values wide.
+__device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int value, int in_page, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(value), "r"(in_page), "r"(head), "r"(page)
+        : "memory");
+}
+
+// Loads the K and V tiles of the walk's item into the kv ring (warp together, a lane per page of
+// the tile); only pages that hold a position somebody sees.  False: gave up.  WARPS warps share
+// the copies of every tile, this one is `which`; each arrives at its barrier.  The lanes' copies
+// go out one by one, so whatever they have in common is made uniform before.
 template <int D, int STAGES, int WARPS>
 __device__ __forceinline__ bool load_tiles(const AttnArgs& a, const AttnMaps& maps, const Walk& w, uint8_t* kv_ring,
                                            uint64_t* full, uint64_t* empty, int& stage, uint32_t& phase, uint32_t& issued,
                                            volatile int* dead, int which = 0) {
     constexpr int HALVES = D / 64, STAGE = kTile * D * 2;
+    constexpr int MINE = WARPS >= HALVES ? 1 : HALVES;          // halves of a tile (64 values each) that this warp loads
+    constexpr int STEP = WARPS >= HALVES ? WARPS / HALVES : 1;  // of them every STEP-th page
     const int lane = threadIdx.x & 31;
     const int page_rows = min(1 << a.page_shift, kTile);
-    const int units = kTile / page_rows * HALVES;               // <= 16
-    const int unit = lane * WARPS + which, my_page = unit / HALVES, my_half = unit % HALVES;
+    const int half0 = MINE == 1 && HALVES > 1 ? uniform(which % HALVES) : 0;
+    const int my_page = lane * STEP + (MINE == 1 ? which / HALVES : 0);
     const int* row = a.table + w.b * a.table_ld;
+    const int head = uniform(w.head);
+    const uint32_t ring = smem_u32(kv_ring) + half0 * 16384, fulls = smem_u32(full), empties = smem_u32(empty);
+    const uint32_t mine_at = my_page * page_rows * 128;
     // the table is read a tile ahead, so that its latency is not between the copies
-    int pos = (w.first + w.t0) * kTile + my_page * page_rows;
-    auto seen = [&]() { return unit < units && pos + page_rows > w.lo && pos < w.hi; };
-    int ahead = seen() ? row[pos >> a.page_shift] : 0;
+    int at = uniform((w.first + w.t0) * kTile);                 // the tile's first position
+    auto seen = [&]() {
+        const int pos = at + my_page * page_rows;
+        return my_page * page_rows < kTile && pos + page_rows > w.lo && pos < w.hi;
+    };
+    auto look_up = [&]() { return row[(at + my_page * page_rows) >> a.page_shift]; };
+    int ahead = seen() ? look_up() : 0;
     for (int j = w.t0; j < w.t1; ++j) {
         const bool mine = seen();
+        const int in_page = at & ((1 << a.page_shift) - 1);     // 0 where a tile has several pages
         int page = ahead;
-        const int in_page = pos & ((1 << a.page_shift) - 1);
-        pos += kTile;
-        ahead = j + 1 < w.t1 && seen() ? row[pos >> a.page_shift] : 0;
-        if (mine) {
-            if (page < 0 || page >= a.num_pages) {
-                page = a.num_pages;                             // outside: the copy fills zeros
-                atomicOr(a.err, DERR_PAGED);
-            }
+        at += kTile;
+        if (j + 1 < w.t1 && seen()) ahead = look_up();
+        if (mine && (page < 0 || page >= a.num_pages)) {
+            page = a.num_pages;                                 // outside: the copy fills zeros
+            atomicOr(a.err, DERR_PAGED);
         }
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * page_rows * 128;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * page_rows * MINE * 128;
+#pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-            if (!warp_wait(&empty[stage], phase ^ 1u, a.err, dead)) return false;
-            if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+            const uint32_t st = uniform(stage), bar = fulls + st * 8, dst = ring + st * STAGE + mine_at;
+            if (!warp_wait(empties + st * 8, phase ^ 1u, a.err, dead)) return false;
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
             __syncwarp();
-            if (mine)
-                tma_load_4d(kv_ring + stage * STAGE + my_half * 16384 + my_page * page_rows * 128, kv ? &maps.v : &maps.k,
-                            &full[stage], my_half * 64, in_page, w.head, page);
+#pragma unroll
+            for (int h = 0; h < MINE; ++h)
+                if (mine) load_page(dst + h * 16384, kv ? &maps.v : &maps.k, bar, (half0 + h) * 64, in_page, head, page);
             ++issued;
             if (++stage == STAGES) {
                 stage = 0;
