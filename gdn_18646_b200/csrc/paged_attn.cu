@@ -46,6 +46,7 @@ namespace {
 
 constexpr int QT = 2;                 // row tiles of 128 per item
 constexpr int kItemCost = 3;          // kv tiles that starting and ending an item is worth, beside its tiles
+constexpr int kJoinThreads = 256, kJoinBlocks = 2;  // of the join kernel, per SM
 constexpr int kWholeTiles = 8;        // items of so many kv tiles are not cut when there are few
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
 constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
@@ -491,93 +492,124 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     }
 }
 
-// Joins the parts of the items that pieces cut: block (x, y) takes the item that CTA x
-// began and did not finish.  A warp takes 32 rows (a lane each, as the parts lie in
-// memory) and a quarter of the columns.  All loads of a batch are independent of one
-// another; one wave of blocks (each starts with a wait for the states).
-template <int D>
-__global__ void __launch_bounds__(512, 2) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
-    pdl_wait_prior();
-    const int rows = a.part_rows;
-    const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int V = D / 16;                                   // float4 of a quarter row
-    const int slice = warp & 7, colg = (blockIdx.y * 16 + warp) >> 3;
-    // the states of this CTA and of the 31 after it in one go
-    const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
-    const int head = __ldcg(a.part_state + x * 8 + 4);
-    int st = x + 1 + lane < ctas ? __ldcg(a.part_state + (x + 1 + lane) * 8) : 0;
-    if (mine.y == 0) return;
-    const int tok0 = mine.z, toks = mine.w;
-    const int row = slice * 32 + lane, r = row & 127;
+// What the join kernel knows of an item that CTA x began and did not finish.
+struct Cut {
+    int x, parts, tok0, toks, head;
+};
+
+// Joins 32 rows (a lane each, as the parts lie in memory) of a cut item, C float4 of their
+// values from float4 c0 on: one pass over the parts with a running maximum, loads in batches of
+// N parts under a predicate (a remainder loop would wait for each of them).
+template <int D, int C, int N>
+__device__ __forceinline__ void join_rows(const AttnArgs& a, const Cut& w, int slice, int c0) {
+    const int rows = a.part_rows, row = slice * 32 + (threadIdx.x & 31), r = row & 127;
     const int tl = r / a.group, tok = (row >> 7) * a.tile_tokens + tl;
-    const bool real = tl < a.tile_tokens && tok < toks;
-    int parts = 1;                                              // CTAs x, x + 1, ...: up to the one with the last part
-    for (int at = x + 1;;) {
-        const uint32_t end = __ballot_sync(0xffffffffu, st != 1);
-        if (end) {
-            const int k = __ffs(end) - 1;
-            parts += k + (__shfl_sync(0xffffffffu, st, k) == 2 ? 1 : 0);
-            break;
-        }
-        parts += 32;
-        at += 32;
-        st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
-    }
-    if (!real) return;
+    if (tl >= a.tile_tokens || tok >= w.toks) return;
     const float c = a.scale * 1.4426950408889634f;
     // part 0 is CTA x's slot 1, part p the slot 0 of CTA x + p
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (static_cast<long>(x) * 2) * rows + row;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o) +
-                       (static_cast<long>(x) * 2 * (D / 4) + colg * V) * rows + row;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<long>(w.x) * 2 * rows + row;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) + (static_cast<long>(w.x) * 2 * (D / 4) + c0) * rows + row;
     auto slot = [](int p) { return p == 0 ? 1 : 2 * p; };
-    const long at = static_cast<long>(tok0 + tok) * a.Hq + head * a.group + (r - tl * a.group);
-    // one pass with a running maximum; loads in batches under a predicate (a remainder loop
-    // would wait for each of them), four columns' float4 at a time
-    constexpr int C = 4, N = 2;
+    float m = -INFINITY, l = 0.f;
+    float4 o[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int c0 = 0; c0 < V; c0 += C) {
-        float m = -INFINITY, l = 0.f;
-        float4 o[C];
+    for (int p0 = 0; p0 < w.parts; p0 += N) {
+        float2 v[N];
+        float4 u[N][C];
+        float mn = m;
 #pragma unroll
-        for (int i = 0; i < C; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < parts; p0 += N) {
-            float2 v[N];
-            float4 u[N][C];
-            float mn = m;
+        for (int k = 0; k < N; ++k) {
+            v[k] = p0 + k < w.parts ? __ldcg(ml + slot(p0 + k) * rows) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                v[k] = p0 + k < parts ? __ldcg(ml + slot(p0 + k) * rows) : make_float2(0.f, 0.f);
+            for (int i = 0; i < C; ++i)
+                u[k][i] = p0 + k < w.parts ? __ldcg(po + (static_cast<long>(slot(p0 + k)) * (D / 4) + i) * rows)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll
-                for (int i = 0; i < C; ++i)
-                    u[k][i] = p0 + k < parts ? __ldcg(po + (static_cast<long>(slot(p0 + k)) * (D / 4) + c0 + i) * rows)
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+        for (int k = 0; k < N; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
+        const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
+        m = mn;
+        l *= keep;
 #pragma unroll
-            for (int k = 0; k < N; ++k) mn = fmaxf(mn, v[k].y == 0.f ? -INFINITY : v[k].x);
-            const float mc = mn == -INFINITY ? 0.f : mn * c, keep = ex2_approx(m * c - mc);
-            m = mn;
-            l *= keep;
+        for (int i = 0; i < C; ++i) {
+            o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float f = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
+            l += v[k].y * f;
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
-            }
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const float w = v[k].y == 0.f ? 0.f : ex2_approx(v[k].x * c - mc);
-                l += v[k].y * w;
-#pragma unroll
-                for (int i = 0; i < C; ++i) {
-                    o[i].x += u[k][i].x * w; o[i].y += u[k][i].y * w; o[i].z += u[k][i].z * w; o[i].w += u[k][i].w * w;
-                }
+                o[i].x += u[k][i].x * f; o[i].y += u[k][i].y * f; o[i].z += u[k][i].z * f; o[i].w += u[k][i].w * f;
             }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + colg * V + c0;
+    }
+    const long at = static_cast<long>(w.tok0 + tok) * a.Hq + w.head * a.group + (r - tl * a.group);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + c0;
 #pragma unroll
-        for (int i = 0; i < C; ++i)
-            dst[i] = l == 0.f ? make_uint2(0u, 0u)
-                              : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
-        if (a.lse && colg == 0 && c0 == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    for (int i = 0; i < C; ++i)
+        dst[i] = l == 0.f ? make_uint2(0u, 0u)
+                          : make_uint2(cvt_bf16x2(o[i].x * inv, o[i].y * inv), cvt_bf16x2(o[i].z * inv, o[i].w * inv));
+    if (a.lse && c0 == 0) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+}
+
+// Joins the parts of the items that pieces cut.  Every block lists the cut items (up to one per
+// CTA), then the warps of the grid share them: 32 rows x 16 values each, or, where the items are
+// too few for that to fill the GPU, which is also where they have many parts, 32 rows x 4 values
+// with four times the parts in flight (5 tokens over 32768, 8 kv heads,
+// 19 parts each: 9 us; 22 with 16 values).  Registers for the loads in flight count more than warps:
+// 256 threads twice per SM 13.6 us for 148 items of head dim 128, 512 threads with 64 registers 18.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) paged_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    constexpr int WORDS = (kMaxCtas + 31) / 32;
+    __shared__ Cut cut[kMaxCtas];
+    __shared__ uint32_t begun[WORDS], more[WORDS], last[WORDS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait_prior();
+    int4 st = make_int4(0, 0, 0, 0);
+    int head = 0;
+    if (warp < WORDS) {                                         // thread x: CTA x's state
+        if (tid < ctas) {
+            st = __ldcg(reinterpret_cast<const int4*>(a.part_state + tid * 8));
+            head = __ldcg(a.part_state + tid * 8 + 4);
+        }
+        const uint32_t b = __ballot_sync(0xffffffffu, st.y != 0), m = __ballot_sync(0xffffffffu, st.x == 1),
+                       e = __ballot_sync(0xffffffffu, st.x == 2);
+        if (lane == 0) {
+            begun[warp] = b;
+            more[warp] = m;
+            last[warp] = e;
+        }
+    }
+    __syncthreads();
+    int n = 0, mine = 0;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+        const int k = __popc(begun[i]);
+        if (i < warp) mine += k;
+        n += k;
+    }
+    if (st.y != 0) {
+        mine += __popc(begun[warp] & ((1u << lane) - 1));
+        int at = tid + 1;                                       // CTAs x + 1, ...: up to the one with the last part
+        while (at < ctas && (more[at >> 5] >> (at & 31) & 1)) ++at;
+        const int ends = at < ctas ? static_cast<int>(last[at >> 5] >> (at & 31) & 1) : 0;
+        cut[mine] = Cut{tid, at - tid + ends, st.z, st.w, head};
+    }
+    __syncthreads();
+    const int slices = a.part_rows / 32, warps = gridDim.x * (kJoinThreads / 32);
+    const bool wide = n * slices * (D / 16) * 2 >= warps;
+    const int cols = wide ? D / 16 : D / 4;
+    for (int u = blockIdx.x * (kJoinThreads / 32) + warp; u < n * slices * cols; u += warps) {
+        const int c = u % cols, slice = u / cols % slices;
+        const Cut& w = cut[u / cols / slices];
+        if (wide)
+            join_rows<D, 4, 4>(a, w, slice, c * 4);
+        else
+            join_rows<D, 1, 8>(a, w, slice, c);
     }
 }
 
@@ -623,8 +655,8 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3(kMaxCtas, 2);
-    cfg.blockDim = dim3(512);
+    cfg.gridDim = dim3(kJoinBlocks * kMaxCtas);                         // one wave
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, a, static_cast<int>(kMaxCtas));
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: join launch failed: %s", name, cudaGetErrorString(e));
