@@ -28,7 +28,7 @@ namespace {
 // us: 1 token over 1000 positions in pages of 16, head dim 128, 16.3 / 12.6 / 12.0; 256 sequences of
 // up to 8192 161 / 162 / 162; 2 of up to 131072 in pages of 64 72.5 / 72.8 / 73.2.
 constexpr int kLoadWarps = 2;
-constexpr int kRowsThreads = 160 + 32 * kLoadWarps;      // 4 softmax warps, MMA, load
+constexpr int kRowsThreads = 288 + 32 * kLoadWarps;      // 2 x 4 softmax warps, MMA, load
 
 template <int D, int N>
 struct RowsShape {
@@ -64,13 +64,13 @@ struct RowsBars {
 };
 static_assert(sizeof(RowsBars) <= 3072, "barrier block");
 
-// whether any of the 128 softmax threads says so
-__device__ __forceinline__ bool any_of_128(bool x) {
+// whether any of the 128 threads that meet at barrier `id` says so
+__device__ __forceinline__ bool any_of_128(int id, bool x) {
     uint32_t r;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(r)
-        : "r"(static_cast<uint32_t>(x))
+        : "r"(static_cast<uint32_t>(x)), "r"(id)
         : "memory");
     return r != 0;
 }
@@ -93,7 +93,10 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
 }
 template <int N>
 __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, float (&v)[N]) {
-    if constexpr (N == 16) {
+    if constexpr (N == 8) {
+        tmem_ld8(taddr, v);
+        return;
+    } else if constexpr (N == 16) {
         uint32_t r[16];
         asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -146,7 +149,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
     RowsBars* sh = reinterpret_cast<RowsBars*>(sm + S::OFF_BAR);
     volatile int* dead = &sh->abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int MMA_WARP = 4, LOAD_WARP = 5;
+    constexpr int MMA_WARP = 8, LOAD_WARP = 9;
     const int tt = a.tile_tokens, cta = blockIdx.x;
 
     if (tid == 0) {
@@ -158,7 +161,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             mbar_init(&sh->q_full[i], 1);
             mbar_init(&sh->q_empty[i], 1);
             mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->p_full[i], 4);
+            mbar_init(&sh->p_full[i], 8);
         }
         mbar_init(&sh->o_full, 1);
         mbar_init(&sh->pv_done, 1);
@@ -281,33 +284,37 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         }
     } else {
         // ---------------- softmax and epilogue: thread = position of the tile, then value index.
+        // Two groups of 128 threads, a half of the rows each: they share nothing but the MMAs.
         // What a tile always does is unrolled over the rows; the new maximum, the rescale and the
         // end of an item are loops over eight rows, because with those unrolled the code did not
         // stay in the instruction cache (an item of one tile took 11 us at N 16).
         // No early way out of a tile: a wait that gave up returns, and all warps keep
         // meeting at the barriers until their walk ends.
-        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        constexpr int R = N / 2;
+        const int group = tid >> 7, th = tid & 127, wg = warp & 3, r0 = group * R, bar = 1 + group;
+        const uint32_t lanes = static_cast<uint32_t>(wg * 32) << 16;
         const float c = a.scale * 1.4426950408889634f;
-        uint8_t* const p_base = sm + S::OFF_P + (tid >> 6) * (N * 128);
+        uint8_t* const p_base = sm + S::OFF_P + (th >> 6) * (N * 128);
         uint32_t done = 0, items = 0;
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
-        if (tid < 32) sh->m[tid] = -INFINITY;
-        named_bar(1, 128);
+        if (th < R) sh->m[r0 + th] = -INFINITY;
+        named_bar(bar, 128);
         Walk w;
         for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
-            const int toks = min(tt, w.s.n - w.item * tt), nr = toks * a.group;     // rows of the item
+            const int toks = min(tt, w.s.n - w.item * tt), rows = toks * a.group;   // of the item
             const long at0 = static_cast<long>(w.s.c0 + w.item * tt) * a.Hq + w.head * a.group;
+            const int nr = min(max(rows - r0, 0), R);           // rows of this half
             auto row_at = [&](int r) {                          // (token, head) row of the output
                 const int tok = r / a.group;
                 return at0 + static_cast<long>(tok) * a.Hq + (r - tok * a.group);
             };
             if (w.t0 >= w.t1) {
                 if (w.count == 0) {                             // sees nothing
-                    for (int r = 0; r < nr; ++r) {
+                    for (int r = r0; r < r0 + nr; ++r) {
                         const long at = row_at(r);
-                        if (tid < D) a.out[at * D + tid] = 0;
-                        if (a.lse && tid == 0) a.lse[at] = -INFINITY;
+                        if (th < D) a.out[at * D + th] = 0;
+                        if (a.lse && th == 0) a.lse[at] = -INFINITY;
                     }
                 }
                 continue;
@@ -315,41 +322,41 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             int lo0, hi0, lo1, hi1;                             // what the first and the last token see
             w.s.range(a, w.item * tt, w.item * tt, lo0, hi0);
             w.s.range(a, w.item * tt + toks - 1, w.item * tt + toks - 1, lo1, hi1);
-            float l[N];                                         // this thread's part of the rows' sums
+            float l[R];                                         // this thread's part of the rows' sums
 #pragma unroll
-            for (int r = 0; r < N; ++r) l[r] = 0.f;
+            for (int r = 0; r < R; ++r) l[r] = 0.f;
 #pragma unroll 1
             for (int j = w.t0; j < w.t1; ++j, ++done) {
-                const uint32_t buf = done & 1u, s_col = tmem + lanes + buf * N;
-                const int j0 = (w.first + j) * kTile, pos = j0 + tid;
-                // rows [from, to) see this position: those of the token that stands here and of the
+                const uint32_t buf = done & 1u, s_col = tmem + lanes + buf * N + r0;
+                const int j0 = (w.first + j) * kTile, pos = j0 + th;
+                // rows [from, to) of the half see this position: those of the token that stands here and of the
                 // tokens after it, up to the window's end
-                int from = 0, to = N;
+                int from = 0, to = R;
                 if (j0 + kTile > hi0 || j0 < lo1) {
                     const int tok = pos - (w.s.kv - w.s.n + w.item * tt);
-                    if (a.causal) from = min(max(tok, 0) * a.group, N);
-                    if (a.window > 0) to = min(max(tok + a.window, 0), N) * a.group;
-                    if (pos >= w.s.kv) from = N;
+                    if (a.causal) from = min(max(tok, 0) * a.group, N) - r0;
+                    if (a.window > 0) to = min(max(tok + a.window, 0), N) * a.group - r0;
+                    if (pos >= w.s.kv) from = R;
                 }
                 wait_at(smem_u32(&sh->s_full[buf]), (done >> 1) & 1u, a.err, dead);
                 tc_fence_after();
-                float s[N];
-                tmem_ld_rows<N>(s_col, s);
-                if (from > 0 || to < N) {
+                float s[R];
+                tmem_ld_rows<R>(s_col, s);
+                if (from > 0 || to < R) {
 #pragma unroll
-                    for (int r = 0; r < N; ++r)
+                    for (int r = 0; r < R; ++r)
                         if (r < from || r >= to) s[r] = -INFINITY;
                 }
                 bool grow = false;                              // m = -inf: true for any finite s
 #pragma unroll
-                for (int q = 0; q < N; q += 8) {
+                for (int q = 0; q < R; q += 8) {
                     if (q >= nr) break;
                     float m[8];
-                    rows8(sh->m + q, m);
+                    rows8(sh->m + r0 + q, m);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) grow |= q + i < nr && (s[q + i] - m[i]) * c > 8.f;
                 }
-                if (any_of_128(grow)) {
+                if (any_of_128(bar, grow)) {
 #pragma unroll 1
                     for (int q = 0; q < nr; q += 8) {
                         float x[8];
@@ -358,46 +365,47 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                         for (int i = 0; i < 8; ++i)
                             if (q + i < from || q + i >= to) x[i] = -INFINITY;
                         const float top = reduce8<true>(x);
-                        if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = top;
+                        if ((lane & 3) == 0) sh->red[wg][r0 + q + (lane >> 2)] = top;
                     }
-                    named_bar(1, 128);
-                    if (tid < nr) {
-                        const float x = fmaxf(fmaxf(sh->red[0][tid], sh->red[1][tid]), fmaxf(sh->red[2][tid], sh->red[3][tid]));
-                        const float m = sh->m[tid];
-                        sh->f[tid] = x > m ? ex2_approx((m - x) * c) : 1.f;
-                        if (x > m) sh->m[tid] = x;
+                    named_bar(bar, 128);
+                    if (th < nr) {
+                        const int r = r0 + th;
+                        const float x = fmaxf(fmaxf(sh->red[0][r], sh->red[1][r]), fmaxf(sh->red[2][r], sh->red[3][r]));
+                        const float m = sh->m[r];
+                        sh->f[r] = x > m ? ex2_approx((m - x) * c) : 1.f;
+                        if (x > m) sh->m[r] = x;
                     }
-                    named_bar(1, 128);
+                    named_bar(bar, 128);
                     if (j > w.t0) {                             // O once P V(j - 1) is in it
                         wait_at(smem_u32(&sh->pv_done), (done - 1) & 1u, a.err, dead);
                         tc_fence_after();
 #pragma unroll 1
                         for (int q = 0; q < nr; q += 8) {
                             float o[8];
-                            tmem_ld8(tmem + lanes + S::T_O + q, o);
+                            tmem_ld8(tmem + lanes + S::T_O + r0 + q, o);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] *= q + i < nr ? sh->f[q + i] : 1.f;   // rows past the item's: any
-                            tmem_st8(tmem + lanes + S::T_O + q, o);
+                            for (int i = 0; i < 8; ++i) o[i] *= q + i < nr ? sh->f[r0 + q + i] : 1.f;   // rows past the item's: any
+                            tmem_st8(tmem + lanes + S::T_O + r0 + q, o);
                         }
                         tmem_st_wait();
 #pragma unroll
-                        for (int r = 0; r < N; ++r)
-                            if (r < nr) l[r] *= sh->f[r];
+                        for (int r = 0; r < R; ++r)
+                            if (r < nr) l[r] *= sh->f[r0 + r];
                     }
                 }
                 uint8_t* const pb = p_base + buf * S::P_BYTES;
                 // rows past the item's go with the last eight (their columns go nowhere)
 #pragma unroll
-                for (int q = 0; q < N; q += 8) {
+                for (int q = 0; q < R; q += 8) {
                     if (q >= nr) break;
                     float m[8], p[8];                           // all loads before the stores, which might alias them
-                    rows8(sh->m + q, m);
+                    rows8(sh->m + r0 + q, m);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) p[i] = ex2_approx(fmaf(s[q + i], c, m[i] == -INFINITY ? 0.f : -m[i] * c));
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         l[q + i] += p[i];
-                        *reinterpret_cast<uint16_t*>(pb + sw128_off(q + i, tid & 63)) = f32_to_bf16_bits(p[i]);
+                        *reinterpret_cast<uint16_t*>(pb + sw128_off(r0 + q + i, th & 63)) = f32_to_bf16_bits(p[i]);
                     }
                 }
                 fence_async_smem();
@@ -407,15 +415,15 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             }
             // the sums of the threads, in order
 #pragma unroll
-            for (int q = 0; q < N; q += 8) {
+            for (int q = 0; q < R; q += 8) {
                 if (q >= nr) break;
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = l[q + i];
                 const float sum = reduce8<false>(x);
-                if ((lane & 3) == 0) sh->red[warp][q + (lane >> 2)] = sum;
+                if ((lane & 3) == 0) sh->red[wg][r0 + q + (lane >> 2)] = sum;
             }
-            named_bar(1, 128);
+            named_bar(bar, 128);
             wait_at(smem_u32(&sh->o_full), items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
@@ -424,20 +432,22 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
 #pragma unroll 1
             for (int q = 0; q < nr; q += 8) {
                 float o[8], sum[8];                             // loads before stores here too
-                tmem_ld8(tmem + lanes + S::T_O + q, o);
+                tmem_ld8(tmem + lanes + S::T_O + r0 + q, o);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] = (sh->red[0][q + i] + sh->red[1][q + i]) + (sh->red[2][q + i] + sh->red[3][q + i]);
-                int tok = q / a.group, g = q - tok * a.group;
-                if (tid < D)
+                for (int i = 0; i < 8; ++i) {
+                    const int r = r0 + q + i;
+                    sum[i] = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
+                }
+                int tok = (r0 + q) / a.group, g = r0 + q - tok * a.group;
+                if (th < D)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int r = q + i;
-                        if (r < nr) {
+                        if (q + i < nr) {
                             if (whole)
-                                a.out[(at0 + static_cast<long>(tok) * a.Hq + g) * D + tid] =
+                                a.out[(at0 + static_cast<long>(tok) * a.Hq + g) * D + th] =
                                     f32_to_bf16_bits(sum[i] == 0.f ? 0.f : __fdividef(o[i], sum[i]));
                             else
-                                a.part_o[(slot + r) * D + tid] = o[i];
+                                a.part_o[(slot + r0 + q + i) * D + th] = o[i];
                         }
                         if (++g == a.group) {
                             g = 0;
@@ -446,14 +456,15 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                     }
             }
             tc_fence_before();
-            if (tid < nr) {
-                const float sum = (sh->red[0][tid] + sh->red[1][tid]) + (sh->red[2][tid] + sh->red[3][tid]), m = sh->m[tid];
+            if (th < nr) {
+                const int r = r0 + th;
+                const float sum = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]), m = sh->m[r];
                 if (!whole)
-                    *reinterpret_cast<float2*>(a.part_ml + (slot + tid) * 2) = make_float2(m, sum);
+                    *reinterpret_cast<float2*>(a.part_ml + (slot + r) * 2) = make_float2(m, sum);
                 else if (a.lse)
-                    a.lse[row_at(tid)] = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
+                    a.lse[row_at(r)] = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
             }
-            if (tid < 32) sh->m[tid] = -INFINITY;               // for the next item
+            if (th < R) sh->m[r0 + th] = -INFINITY;             // for the next item
             if (tid == 0 && !whole) {
                 int* ps = a.part_state + cta * 8;
                 if (w.t0 == 0) {
@@ -465,7 +476,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                     ps[0] = w.t1 == w.count ? 2 : 1;             // 2: the item's last part
                 }
             }
-            named_bar(1, 128);
+            named_bar(bar, 128);
         }
     }
     tc_fence_before();
