@@ -26,7 +26,7 @@
 //   P (bf16) overwrites S in TMEM      (rounded to bf16: 2^-9 rms of each weight)
 //   O += P V    M 128, N D (TS)        -> TMEM, fp32 over the whole pass
 // The tensor core works for one row tile while the softmax of the other runs.  Items of
-// at most 32 rows (a decode step) go to paged_attn_rows.cu.
+// at most 64 rows (a decode step) go to paged_attn_rows.cu.
 //
 // What bounds it.  A kv tile of both row tiles is 32 MMAs of about 61 cycles and 128 x 256
 // exponentials, 2048 cycles either; three pairs of eight take a polynomial on the FMA pipe
@@ -613,15 +613,16 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) paged_attn_join_ker
     }
 }
 
-// Kernel by the rows (tokens x heads of a group) of the longest chunk: up to 32 the one for
+// Kernel by the rows (tokens x heads of a group) of the longest chunk: up to 64 the one for
 // few rows, which keeps them in the MMA's narrow dimension, else the one with 128-row tiles.
-// Both sides, us: 25 rows (16 x 5 tokens over 4096, head dim 64) 51 / 61; 40 rows (5 tokens over
-// 32768) 58 / 62; 64 rows (4 tokens x 16 heads over 4096) 64 / 50, (8 x 8 over 32768) 72 / 62.
-bool few_rows(int max_q, int group) { return static_cast<long>(max_q > 1 ? max_q : 1) * group <= 32; }
+// Both sides, us: 25 rows (16 x 5 tokens over 4096, head dim 64) 43 / 65; 40 (5 tokens over 32768)
+// 41 / 51, (32 x 5 over 4096, head dim 64) 96 / 115; 64 (8 tokens x 8 heads over 32768) 45 / 52,
+// (4 x 16 over 4096) 44 / 51, (1 x 64 over 100000, head dim 64) 40 / 54.
+bool few_rows(int max_q, int group) { return static_cast<long>(max_q > 1 ? max_q : 1) * group <= 64; }
 
 // Rows of an unfinished item's part.
 int part_rows(int max_q, int group) {
-    return !few_rows(max_q, group) ? QT * 128 : max_q * group <= 16 && group <= 16 ? 16 : 32;
+    return !few_rows(max_q, group) ? QT * 128 : max_q * group <= 16 && group <= 16 ? 16 : max_q * group <= 32 && group <= 32 ? 32 : 64;
 }
 
 // CTAs for a call whose items are few and short enough to be left whole, one per item, so

@@ -1,13 +1,13 @@
 // paged_attn_rows.cu -- paged attention where an item has few rows (a decode step, a few
-// drafted tokens: tokens x query heads of a kv head <= 32), on tcgen05.
+// drafted tokens: tokens x query heads of a kv head <= 64), on tcgen05.
 //
 // The mathematics, the rows and the line of work are those of paged_attn.cu.  Here the
 // keys stand in the MMA's wide dimension and the rows in its narrow one:
-//   S^T = K Q^T      M 128 positions, N rows (16 or 32), SS        -> TMEM, lane = position
+//   S^T = K Q^T      M 128 positions, N rows (16, 32 or 64), SS        -> TMEM, lane = position
 //   P^T (bf16)       thread = position, written to shared memory as the next B operand
 //   O^T += V^T P^T   M = D, N rows, SS (V as it lies, MN-major)    -> TMEM, lane = value index
 // so a tile of 128 keys costs N/128 of the tensor work of a 128-row tile, and its softmax
-// 128 threads x N exponentials instead of one warp x 128 a row (with rows in the wide
+// 256 threads x N / 2 exponentials instead of one warp x 128 a row (with rows in the wide
 // dimension a tile took 2050 cycles, near the 2800 in which HBM delivers one, and the clock fell).  The running
 // maximum is the same for all threads; only when some weight would pass 2^8 do they
 // reduce a new one and rescale.  The sums l stay per thread until the item ends.
@@ -45,7 +45,7 @@ struct RowsShape {
     static constexpr int OFF_P = OFF_Q + 2 * Q_BYTES;
     static constexpr int OFF_BAR = OFF_P + 2 * P_BYTES;
     static constexpr int SMEM = 1024 + OFF_Q + AFTER;
-    static constexpr int COLS = N == 16 ? 64 : 128;             // TMEM: two S buffers, O
+    static constexpr int COLS = N == 16 ? 64 : N == 32 ? 128 : 256;             // TMEM: two S buffers, O
     static constexpr int T_O = 2 * N;
     static_assert(SMEM <= 232448, "shared memory");
 };
@@ -56,9 +56,9 @@ struct RowsBars {
     uint64_t s_full[2], p_full[2];
     uint64_t o_full, pv_done;
     PieceScratch scratch;
-    alignas(16) float m[32];
-    float f[32];                      // per row: reference maximum, factor of a rescale
-    float red[4][32];                 // per warp and row: tile maxima, then sums
+    alignas(16) float m[64];
+    float f[64];                      // per row: reference maximum, factor of a rescale
+    float red[4][64];                 // per warp and row: tile maxima, then sums
     uint32_t tmem;
     int abort;
 };
@@ -491,12 +491,14 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
     }
 }
 
-// Joins the parts of the items that pieces cut: block x takes the item that CTA x began and
-// did not finish, a warp per row, the lanes along its values.
+// Joins the parts of the items that pieces cut: blocks (x, y) take the item that CTA x began and
+// did not finish, 16 rows each, a warp per row, the lanes along its values.
+// Six parts in flight and two blocks per SM, against 16 and one: 44.7 / 49.2 us (whole call) for 64
+// rows over 32768 positions, 8 kv heads (8 items of 19 parts), 70 / 75.5 for 256 items of 2048.
 template <int D>
-__global__ void __launch_bounds__(512) paged_attn_rows_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(512, 2) paged_attn_rows_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
     pdl_wait_prior();
-    constexpr int V = D / 32, BATCH = 16;
+    constexpr int V = D / 32, BATCH = 6;
     const int x = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the states of this CTA and of the 31 after it in one go
     const int4 mine = __ldcg(reinterpret_cast<const int4*>(a.part_state + x * 8));
@@ -516,7 +518,8 @@ __global__ void __launch_bounds__(512) paged_attn_rows_join_kernel(const __grid_
         st = at + lane < ctas ? __ldcg(a.part_state + (at + lane) * 8) : 0;
     }
     const float c = a.scale * 1.4426950408889634f;
-    for (int r = warp; r < mine.w * a.group; r += 16) {
+    const int r = blockIdx.y * 16 + warp;
+    if (r < mine.w * a.group) {
         // part 0 is CTA x's slot 1, part p the slot 0 of CTA x + p
         auto row = [&](int p) { return (static_cast<long>(x) * 2 + (p == 0 ? 1 : 2 * p)) * a.part_rows + r; };
         float m = -INFINITY, l = 0.f, o[V] = {};
@@ -592,7 +595,7 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
     cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attn_rows_kernel<D, N>, maps, a);
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
     if (a.whole) return launch_status(name);
-    cfg.gridDim = dim3(kMaxCtas);
+    cfg.gridDim = dim3(kMaxCtas, N / 16);
     cfg.numAttrs = 1;                                           // starts while the first kernel ends
     cfg.blockDim = dim3(512);
     cfg.dynamicSmemBytes = 0;
@@ -604,8 +607,13 @@ int launch(const AttnMaps& maps, const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int launch_attn_rows(const AttnMaps& maps, const AttnArgs& a, int D, cudaStream_t st) {
-    if (D == 64) return a.part_rows == 16 ? launch<64, 16>(maps, a, st) : launch<64, 32>(maps, a, st);
-    return a.part_rows == 16 ? launch<128, 16>(maps, a, st) : launch<128, 32>(maps, a, st);
+    if (D == 64)
+        return a.part_rows == 16   ? launch<64, 16>(maps, a, st)
+               : a.part_rows == 32 ? launch<64, 32>(maps, a, st)
+                                   : launch<64, 64>(maps, a, st);
+    return a.part_rows == 16   ? launch<128, 16>(maps, a, st)
+           : a.part_rows == 32 ? launch<128, 32>(maps, a, st)
+                               : launch<128, 64>(maps, a, st);
 }
 
 }  // namespace gdn

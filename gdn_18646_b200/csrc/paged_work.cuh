@@ -395,7 +395,7 @@ inline size_t part_state_bytes() { return static_cast<size_t>(kMaxCtas) * 8 * si
 inline size_t part_ml_bytes(int rows) { return static_cast<size_t>(kMaxCtas) * 2 * rows * 2 * sizeof(float); }
 inline size_t part_o_bytes(int rows, int D) { return static_cast<size_t>(kMaxCtas) * 2 * rows * D * sizeof(float); }
 
-// paged_attn_rows.cu: at most 32 rows per item (a decode step, a few drafted tokens)
+// paged_attn_rows.cu: at most 64 rows per item (a decode step, a few drafted tokens)
 int launch_attn_rows(const AttnMaps& maps, const AttnArgs& a, int D, cudaStream_t st);
 
 }  // namespace gdn

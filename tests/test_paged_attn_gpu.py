@@ -280,3 +280,34 @@ def test_refusals(cuda_device):
               dict(out=b.q[:1]), dict(workspace=torch.zeros(4, device="cuda"))):
         with pytest.raises(RuntimeError):
             G.paged_attention(**dict(ok, **d))
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 16), (128, 128)])
+@pytest.mark.parametrize("n,group", [(1, 9), (2, 8), (3, 8), (1, 31), (8, 4), (11, 3), (3, 16), (5, 10), (64, 1), (1, 63), (9, 7), (2, 32)])
+def test_row_counts_of_few_rows(cuda_device, n, group, D, page):
+    """Up to 64 rows of an item, most of them not a multiple of eight; short and cut sequences,
+    an empty one, one with more tokens than positions, and a window that starts inside a tile."""
+    lens = [(n, 3300), (n, 130), (0, 50), (max(1, n - 1), n + 1), (n, max(0, n - 2)), (1, 0)]
+    b = Batch(lens, 2 * group, 2, D, page, seed=n + group)
+    out, lse = run(b, return_lse=True)
+    check(b, out, lse, rows=8)
+    b = Batch(lens, 2 * group, 2, D, page, window=201, seed=n + group)
+    out, lse = run(b, window=201, return_lse=True)
+    check(b, out, lse, window=201, rows=8)
+    b = Batch(lens, 2 * group, 2, D, page, seed=n + group)      # without a window: its pages are not poisoned
+    out = run(b, causal=False)
+    check(b, out, causal=False, rows=2)
+
+
+@pytest.mark.parametrize("lens,Hq,Hk,D,page", [
+    ([(70, 30000)], 2, 1, 128, 64),                       # an item in nearly as many parts as there are CTAs
+    ([(5, 60000)], 13, 1, 64, 256),                       # 65 rows
+    ([(9, 40000)], 7, 1, 128, 16),                        # 63 rows
+    ([(140, 9000), (3, 12000)], 6, 3, 128, 32),
+    ([(300, 700 + 60 * i) for i in range(20)], 12, 3, 128, 64),
+    ([(130, 500 + 40 * i) for i in range(32)], 8, 4, 64, 16),
+])
+def test_items_cut_into_parts(cuda_device, lens, Hq, Hk, D, page):
+    b = Batch(lens, Hq, Hk, D, page, seed=31)
+    out, lse = run(b, return_lse=True)
+    check(b, out, lse, rows=6)
