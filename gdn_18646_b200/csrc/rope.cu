@@ -7,7 +7,9 @@
 // Bound by HBM: every head row is read once and written once.  A warp takes a token;
 // its lanes split into groups of D/16, each lane holding the 8 pairs (16 values, two
 // 16-byte pieces) of one unit of a head, so the 8 sines and cosines that a lane needs
-// are the same for every head it turns and are computed once.
+// are the same for every head it turns and are computed once.  269 MB of q and k turned:
+// 42.0 us, 6.4 TB/s; 112 MB of q, k, v appended (11 K tokens): 22.0 us, 5.1 TB/s, held back by
+// the chain token -> sequence -> page -> address before a token's first store.
 //
 // The angle is reduced in fp32 with the product's rounding error carried along
 // (pos * f = hi + lo exactly by an fma) and 2 pi in two parts, after Cody and Waite, so a

@@ -524,13 +524,16 @@ int gdn_rope_append(const void* q, long q_ld, const void* k, long k_ld, const vo
  *   lse        f32 [Ttot, Hq] or NULL
  *   cu_seqlens int32 [B + 1], kv_lens int32 [B], on the device
  *   max_q, max_kv  at least the longest q_len and kv_len (host; they size the launch)
- *   scale      0.0f -> 1/sqrt(D)
+ *   window     0, or one of max_kv and more: none
+ *   scale      0.0f -> 1/sqrt(D); negative or not finite: GDN_ERR_ARG
  * What the cache holds at positions that no token of a sequence sees may be
  * anything, NaN included, and so may the block_table entries of pages that hold
- * only such positions.  A longer q_len or kv_len than max_q or max_kv, and pages
- * outside the cache, are reported by gdn_check_device_error(); the pages are
- * taken as zeros.  D in {64, 128}, Hq / n_kv <= 64.
- * workspace: gdn_paged_attn_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes).
+ * only such positions.  A sequence with a longer q_len or kv_len than max_q or
+ * max_kv is left out (its rows of out are not written), a page outside the cache
+ * is taken as zeros; gdn_check_device_error() reports both.  D in {64, 128},
+ * Hq / n_kv <= 64.
+ * workspace: gdn_paged_attn_workspace_bytes(...) bytes, 16-byte aligned, required
+ * unless Ttot is 0; under 40 MB for any batch and length.
  * No counterpart in the reference (it has no softmax attention).
  */
 int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cache* cache, const int* cu_seqlens,
@@ -624,7 +627,8 @@ const char* gdn_last_error(void);
 /*
  * Per calling host thread (default 0): with on != 0 the decode-step kernels
  * (gdn_decode_proj_fwd, gdn_decode_step[_ex], gdn_rmsnorm_fwd,
- * gdn_gated_rmsnorm_fwd) launch with programmatic stream serialisation: each
+ * gdn_gated_rmsnorm_fwd, gdn_block_norm_fwd, and gdn_paged_attn_fwd where a kv
+ * head has at most 64 new rows of a sequence) launch with programmatic stream serialisation: each
  * lets the next kernel of the stream launch early and waits for its own
  * predecessors before reading their outputs, and gdn_decode_proj_fwd streams its
  * weights before that wait.  Weight operands must therefore not be written by
