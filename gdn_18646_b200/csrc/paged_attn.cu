@@ -322,7 +322,11 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     const uint32_t s_col = tmem + lanes + t * kTile;
                     const int j0 = (w.first + j) * kTile;
                     float s[kTile];
-                    auto load_s = [&]() {
+                    // once, or, after a rescale (a row of S and one of O do not fit the registers), twice: a
+                    // loop, because the code of an item's rare parts would push the rest out of the
+                    // instruction cache
+#pragma unroll 1
+                    for (;;) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) tmem_ld32(s_col + q * 32, reinterpret_cast<float(&)[32]>(s[q * 32]));
                         tmem_ld_wait();
@@ -336,25 +340,25 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                                     if (!(bits & (1u << i))) s[q * 32 + i] = -INFINITY;
                             }
                         }
-                    };
-                    load_s();
-                    // four chains, two values an instruction
-                    float mx4[4] = {s[0], s[1], s[2], s[3]};
+                        // four chains, two values an instruction
+                        float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i < kTile; i += 8)
+                        for (int i = 4; i < kTile; i += 8)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mx4[e] = i + 4 + e < kTile ? max3(mx4[e], s[i + e], s[i + 4 + e]) : fmaxf(mx4[e], s[i + e]);
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    const bool grow = real && (mx - m) * c > 8.f;        // m = -inf: true for any finite mx
-                    if (j == w.t0) {
-                        m = mx;
-                    } else if (__any_sync(0xffffffffu, grow)) {
+                            for (int e = 0; e < 4; ++e)
+                                mx4[e] = i + 4 + e < kTile ? max3(mx4[e], s[i + e], s[i + 4 + e]) : fmaxf(mx4[e], s[i + e]);
+                        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                        if (j == w.t0) {
+                            m = mx;
+                            break;
+                        }
+                        const bool grow = real && (mx - m) * c > 8.f;    // m = -inf: true for any finite mx
+                        if (!__any_sync(0xffffffffu, grow)) break;
                         const float r = grow ? ex2_approx((m - mx) * c) : 1.f;
                         if (grow) m = mx;
                         l *= r;
                         // O is at rest: S(j) was issued after P V(j - 1)
-#pragma unroll
+#pragma unroll 1
                         for (int q = 0; q < D / 32; ++q) {
                             float o[32];
                             tmem_ld32(o_col + q * 32, o);
@@ -363,7 +367,6 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                             for (int i = 0; i < 32; ++i) o[i] *= r;
                             tmem_st32(o_col + q * 32, o);
                         }
-                        load_s();                                        // again: a row of S and one of O do not fit the registers
                     }
                     const float mc = m == -INFINITY ? 0.f : m * c;
                     const uint64_t c2 = pack2(c, c), mc2 = pack2(-mc, -mc);
@@ -417,9 +420,9 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     const float inv = l > 0.f ? 1.f / l : 0.f;
                     const long mine = real ? at : -1;
                     uint8_t* buf = sm + S::OFF_OUT + warp * 4096;
-#pragma unroll
+#pragma unroll 1
                     for (int hf = 0; hf < S::HALVES; ++hf) {
-#pragma unroll
+#pragma unroll 1
                         for (int q = 0; q < 2; ++q) {
                             float o[32];
                             tmem_ld32(o_col + hf * 64 + q * 32, o);
@@ -450,7 +453,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     // slot 0: a part that does not hold the item's first tile; 1: the first part
                     const long part = static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0), slot = part * a.part_rows + t * 128 + row;
                     float4* dst = reinterpret_cast<float4*>(a.part_o) + part * (D / 4) * a.part_rows + t * 128 + row;
-#pragma unroll
+#pragma unroll 1
                     for (int q = 0; q < D / 32; ++q) {
                         float o[32];
                         tmem_ld32(o_col + q * 32, o);
