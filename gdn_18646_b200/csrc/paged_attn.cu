@@ -294,7 +294,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         if (tid == 0)
             for (int i = 0; i < 8; ++i) a.part_state[cta * 8 + i] = 0;
         Walk w;
-        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+        for (w.start(a, piece, tt); w.valid();) {
             const int rel = w.item * tt + t * a.tile_tokens + tok;      // token within the chunk
             const bool real = tok < a.tile_tokens && rel < w.s.n;
             const int first_tok = w.item * tt + t * a.tile_tokens;
@@ -308,6 +308,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     for (int i = 0; i < D / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
                     if (a.lse) a.lse[at] = -INFINITY;
                 }
+                w.next(a, tt);
                 continue;
             }
             int lo, hi, dummy, hi_first, lo_last;
@@ -408,12 +409,14 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 if (lane == 0) mbar_arrive(&sh->p_full[t]);
                 ++done;
             }
+            const bool begins = w.t0 == 0, ends = w.t1 == w.count, whole = begins && ends;
+            const int tok0 = w.s.c0 + w.item * tt, toks = min(tt, w.s.n - w.item * tt), head = w.head;
+            w.next(a, tt);                                              // beside the last P V
             wait_at(o_full, items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
             if (m == -INFINITY) l = 0.f;                                // saw nothing (the polynomial gives 2^-125 for 2^-inf)
             if (busy) {
-                const bool whole = w.t0 == 0 && w.t1 == w.count;
                 if (whole) {
                     // through shared memory, so that a store instruction writes whole lines: 64
                     // values of the warp's 32 rows at a time, 16-byte pieces swizzled by the row
@@ -451,7 +454,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     if (a.lse && real) a.lse[at] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
                 } else {
                     // slot 0: a part that does not hold the item's first tile; 1: the first part
-                    const long part = static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0), slot = part * a.part_rows + t * 128 + row;
+                    const long part = static_cast<long>(cta) * 2 + (begins ? 1 : 0), slot = part * a.part_rows + t * 128 + row;
                     float4* dst = reinterpret_cast<float4*>(a.part_o) + part * (D / 4) * a.part_rows + t * 128 + row;
 #pragma unroll 1
                     for (int q = 0; q < D / 32; ++q) {
@@ -470,15 +473,15 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                 }
                 tc_fence_before();
             }
-            if (tid == 0 && !(w.t0 == 0 && w.t1 == w.count)) {
+            if (tid == 0 && !whole) {
                 int* ps = a.part_state + cta * 8;
-                if (w.t0 == 0) {
+                if (begins) {
                     ps[1] = 1;
-                    ps[2] = w.s.c0 + w.item * tt;                        // first token
-                    ps[3] = min(tt, w.s.n - w.item * tt);                // tokens
-                    ps[4] = w.head;
+                    ps[2] = tok0;                                        // first token
+                    ps[3] = toks;
+                    ps[4] = head;
                 } else {
-                    ps[0] = w.t1 == w.count ? 2 : 1;                     // 2: the item's last part
+                    ps[0] = ends ? 2 : 1;                                // 2: the item's last part
                 }
             }
         }
