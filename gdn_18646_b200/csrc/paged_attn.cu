@@ -30,9 +30,10 @@
 //
 // What bounds it.  A kv tile of both row tiles is 32 MMAs of about 61 cycles and 128 x 256
 // exponentials, 2048 cycles either; three pairs of eight take a polynomial on the FMA pipe
-// (2048 new tokens over 32768, 16 heads on 2, head dim 128: 572 us without, 496 with three
-// of eight, 555 with half of them).  In sustained passes the power cap sets the clock: 496 us
-// (1.07 PFLOP/s) at 1.6 GHz, 438 (1.22) in the first passes at 1.97 GHz.
+// (2048 new tokens over 32768, 16 heads on 2, head dim 128: 486 us; 495 with a quarter or two
+// fifths; before the last steps 496 us with three of eight, 572 without, 555 with a half).  Both take 3400 cycles of the softmax warps, two to a
+// scheduler, 600 to 900 of which wait for the MMAs.  In sustained passes the power cap sets the
+// clock: 486 us (1.10 PFLOP/s) at 1.64 GHz, 430 (1.24) in the first passes at 1.97 GHz.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -45,7 +46,9 @@ namespace gdn {
 namespace {
 
 constexpr int QT = 2;                 // row tiles of 128 per item
-constexpr int kItemCost = 3;          // kv tiles that starting and ending an item is worth, beside its tiles
+// kv tiles that starting and ending an item is worth, beside its tiles.  With 1 / 2 / 3, us: 40 chunks of up to
+// 130 tokens over 500 36.9 / 32.8 / 35.5, 16 of 300 over 3000 73 / 62 / 62, 32 of 200 over 200 31 / 28.7 / 27
+constexpr int kItemCost = 2;
 constexpr int kJoinThreads = 256, kJoinBlocks = 2;  // of the join kernel, per SM
 constexpr int kWholeTiles = 8;        // items of so many kv tiles are not cut when there are few
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
@@ -634,7 +637,7 @@ int part_rows(int max_q, int group) {
 // CTAs for a call whose items are few and short enough to be left whole, one per item, so
 // that no second launch has to join parts; 0: the work is cut.  Both sides on the device, us,
 // whole / cut: 1 token over 1000 positions 13.0 / 13.2 (and 3 less on the host), 8 x 1 over 1000
-// 13.1 / 14.8, 100 over 1000 24.5 / 29.7, 1 over 2000 19.2 / 12.7, 100 over 2000 38 / 33.
+// 13.1 / 14.8, 100 over 1000 23.5 / 29.7, 1 over 2000 19.2 / 12.7, 100 over 2000 38 / 33.
 int whole_items(int B, int T, int n_kv, int item_tokens, int max_kv) {
     const long most = static_cast<long>(n_kv) * (static_cast<long>(B) + T / item_tokens);
     return most <= kMaxCtas && max_kv <= kWholeTiles * kTile ? static_cast<int>(most) : 0;

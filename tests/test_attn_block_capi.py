@@ -135,3 +135,16 @@ def attn(**over):
 def test_paged_attn_rejects(lib, over, code):
     assert _lib.call_status("gdn_paged_attn_fwd", *attn(**over)) == code
     assert "gdn_paged_attn_fwd" in _lib.last_error()
+
+
+@pytest.mark.parametrize("scale", [-1.0, float("nan"), float("inf"), -float("inf")])
+def test_paged_attn_rejects_scales(lib, scale):
+    assert lib.gdn_paged_attn_fwd(*attn(scale=scale)) == _lib.GDN_ERR_ARG
+
+
+def test_paged_attn_workspace_does_not_shrink(lib):
+    """A workspace for calls up to some sizes serves every smaller one."""
+    for D in (64, 128):
+        for Hq, n_kv in ((1, 1), (16, 2), (48, 1), (64, 1)):
+            sizes = [lib.gdn_paged_attn_workspace_bytes(4, 4096, Hq, n_kv, D, q, 65536, 0) for q in (0, 1, 2, 3, 4, 5, 8, 9, 17, 33, 64, 65, 1000)]
+            assert sizes[0] > 0 and sizes == sorted(sizes) and sizes[-1] < 40e6
