@@ -301,7 +301,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
         if (th < R) sh->m[r0 + th] = -INFINITY;
         named_bar(bar, 128);
         Walk w;
-        for (w.start(a, piece, tt); w.valid(); w.next(a, tt)) {
+        for (w.start(a, piece, tt); w.valid();) {
             const int toks = min(tt, w.s.n - w.item * tt), rows = toks * a.group;   // of the item
             const long at0 = static_cast<long>(w.s.c0 + w.item * tt) * a.Hq + w.head * a.group;
             const int nr = min(max(rows - r0, 0), R);           // rows of this half
@@ -317,6 +317,7 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                         if (a.lse && th == 0) a.lse[at] = -INFINITY;
                     }
                 }
+                w.next(a, tt);
                 continue;
             }
             int lo0, hi0, lo1, hi1;                             // what the first and the last token see
@@ -423,12 +424,14 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
                 const float sum = reduce8<false>(x);
                 if ((lane & 3) == 0) sh->red[wg][r0 + q + (lane >> 2)] = sum;
             }
+            const bool begins = w.t0 == 0, ends = w.t1 == w.count, whole = begins && ends;
+            const int tok0 = w.s.c0 + w.item * tt, head = w.head;
+            const long slot = (static_cast<long>(cta) * 2 + (begins ? 1 : 0)) * a.part_rows;
+            w.next(a, tt);                                      // beside the last P V
             named_bar(bar, 128);
             wait_at(smem_u32(&sh->o_full), items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
-            const bool whole = w.t0 == 0 && w.t1 == w.count;
-            const long slot = (static_cast<long>(cta) * 2 + (w.t0 == 0 ? 1 : 0)) * a.part_rows;
 #pragma unroll 1
             for (int q = 0; q < nr; q += 8) {
                 float o[8], sum[8];                             // loads before stores here too
@@ -467,13 +470,13 @@ paged_attn_rows_kernel(const __grid_constant__ AttnMaps maps, const __grid_const
             if (th < R) sh->m[r0 + th] = -INFINITY;             // for the next item
             if (tid == 0 && !whole) {
                 int* ps = a.part_state + cta * 8;
-                if (w.t0 == 0) {
+                if (begins) {
                     ps[1] = 1;
-                    ps[2] = w.s.c0 + w.item * tt;                // first token
+                    ps[2] = tok0;                                // first token
                     ps[3] = toks;
-                    ps[4] = w.head;
+                    ps[4] = head;
                 } else {
-                    ps[0] = w.t1 == w.count ? 2 : 1;             // 2: the item's last part
+                    ps[0] = ends ? 2 : 1;                        // 2: the item's last part
                 }
             }
             named_bar(bar, 128);
