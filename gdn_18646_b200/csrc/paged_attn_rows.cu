@@ -13,7 +13,7 @@
 // reduce a new one and rescale.  The sums l stay per thread until the item ends.
 //
 // Bound by HBM: K and V are read once, 32 KB (D 128) per ring stage.  256 decode steps over up to
-// 8192 positions, 16 heads on 2: 162 us, 6.3 TB/s; 2 over up to 131072, 32 heads on 4: 73 us,
+// 8192 positions, 16 heads on 2: 160 us, 6.4 TB/s; 2 over up to 131072, 32 heads on 4: 72 us,
 // 5.5 TB/s, of which about 8 us are the start of the pieces and the join.
 #include <mutex>
 
