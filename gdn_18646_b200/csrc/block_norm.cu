@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) block_norm_fwd_kernel(c
     float wp[8], wq[8];                        // gamma_post (times the gate that all rows share), gamma_pre
     weight8(a.gamma_post, col, on, wp);
     weight8(a.gamma_pre, col, on, wq);
+    pdl_wait_prior();                          // y, h and the gate (an activation too) come from earlier kernels
     if (one_gate && on) {
         float g[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(a.gate + col)), g);
+        unpack8(__ldcg(reinterpret_cast<const uint4*>(a.gate + col)), g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) wp[i] *= g[i];
     }
-    pdl_wait_prior();                          // y and h come from earlier kernels
     Piece<false> ny, ng;
     Piece<F32> nh;
     ny.zero();

@@ -630,9 +630,10 @@ const char* gdn_last_error(void);
  * gdn_gated_rmsnorm_fwd, gdn_block_norm_fwd, and gdn_paged_attn_fwd where a kv
  * head has at most 64 new rows of a sequence) launch with programmatic stream serialisation: each
  * lets the next kernel of the stream launch early and waits for its own
- * predecessors before reading their outputs, and gdn_decode_proj_fwd streams its
- * weights before that wait.  Weight operands must therefore not be written by
- * the kernels just before it on the stream.  Works inside CUDA graph capture.
+ * predecessors before reading their outputs.  Before that wait gdn_decode_proj_fwd
+ * streams its weights and gdn_block_norm_fwd reads gamma_post and gamma_pre (its
+ * gate, like y and h, is read after it).  Those weights must therefore not be written
+ * by the kernels just before them on the stream.  Works inside CUDA graph capture.
  * No counterpart in the reference.
  */
 int gdn_set_launch_overlap(int on);
