@@ -67,6 +67,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^x for two x <= 128 on the FMA pipe: x = n + f, |f| <= 1/2, n by adding 1.5 2^23; 2^f by
 // the degree-4 polynomial of least relative error (2.7e-6, found by linear programming
 // over Chebyshev nodes); n goes into the exponent bits.  x below -125 counts as -125.
+// The integer add makes a NaN (0x7fffffff) the largest finite number, which the caller has
+// to look for.
 __device__ __forceinline__ void exp2_poly2(float& x0, float& x1) {
     constexpr float kRound = 12582912.f;
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-125.f));
@@ -401,7 +403,9 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
                     }
                     float l0, l1;
                     unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
-                    l += l0 + l1;
+                    // a NaN score (or inf - inf) makes the row NaN: its weight is one too, or, from the polynomial,
+                    // the largest number, where all others are at most 2^8
+                    l = l0 + l1 < 1e30f ? l + (l0 + l1) : __int_as_float(0x7fffffff);
                     tmem_st_wait();
                 } else {
                     __syncwarp();
@@ -418,12 +422,12 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             wait_at(o_full, items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
-            if (m == -INFINITY) l = 0.f;                                // saw nothing (the polynomial gives 2^-125 for 2^-inf)
+            if (m == -INFINITY && l < 1.f) l = 0.f;                     // saw nothing (the polynomial gives 2^-125 for 2^-inf)
             if (busy) {
                 if (whole) {
                     // through shared memory, so that a store instruction writes whole lines: 64
                     // values of the warp's 32 rows at a time, 16-byte pieces swizzled by the row
-                    const float inv = l > 0.f ? 1.f / l : 0.f;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;          // NaN for a NaN
                     const long mine = real ? at : -1;
                     uint8_t* buf = sm + S::OFF_OUT + warp * 4096;
 #pragma unroll 1
@@ -556,7 +560,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const Cut& w, int s
         }
     }
     const long at = static_cast<long>(w.tok0 + tok) * a.Hq + w.head * a.group + (r - tl * a.group);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     uint2* dst = reinterpret_cast<uint2*>(a.out + at * D) + c0;
 #pragma unroll
     for (int i = 0; i < C; ++i)

@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(512, 2) paged_attn_rows_join_kernel(const __gr
                 for (int i = 0; i < V; ++i) o[i] += u[k][i] * f;
             }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const int tok = r / a.group;
         const long at = static_cast<long>(mine.z + tok) * a.Hq + head * a.group + (r - tok * a.group);
         uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * D + lane * V);
