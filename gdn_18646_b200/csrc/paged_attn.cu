@@ -66,13 +66,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 2^x for two x <= 128 on the FMA pipe: x = n + f, |f| <= 1/2, n by adding 1.5 2^23; 2^f by
 // the degree-4 polynomial of least relative error (2.7e-6, found by linear programming
-// over Chebyshev nodes); n goes into the exponent bits.  x below -125 counts as -125.
-// The integer add makes a NaN (0x7fffffff) the largest finite number, which the caller has
-// to look for.
+// over Chebyshev nodes); n goes into the exponent bits, so results below 2^-126 are off by up
+// to 2^-127.  x below -127 + 2^-10 (a masked position's -inf) counts as that, whose bits, 8e-42,
+// are 0 in bf16.  The integer add makes a NaN (0x7fffffff) the largest finite number, which the
+// caller has to look for.
 __device__ __forceinline__ void exp2_poly2(float& x0, float& x1) {
-    constexpr float kRound = 12582912.f;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-125.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-125.f));
+    constexpr float kRound = 12582912.f, kLeast = -126.9990234375f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(kLeast));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(kLeast));
     const uint64_t x = pack2(x0, x1);
     const uint64_t t = add2(x, pack2(kRound, kRound));
     const uint64_t n = add2(t, pack2(-kRound, -kRound));
@@ -422,7 +423,7 @@ paged_attn_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
             wait_at(o_full, items & 1u, a.err, dead);
             ++items;
             tc_fence_after();
-            if (m == -INFINITY && l < 1.f) l = 0.f;                     // saw nothing (the polynomial gives 2^-125 for 2^-inf)
+            if (m == -INFINITY && l < 1.f) l = 0.f;                     // saw nothing (the polynomial gives 8e-42 for 2^-inf)
             if (busy) {
                 if (whole) {
                     // through shared memory, so that a store instruction writes whole lines: 64

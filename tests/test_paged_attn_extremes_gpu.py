@@ -1,6 +1,7 @@
 """paged_attention over keys and values that are not ordinary numbers: a NaN or infinite score
 that a row sees makes that row NaN and no other, wherever it lies in a tile and in either
-kernel; a score of -inf weighs nothing.  Tolerances as in test_paged_attn_gpu.py."""
+kernel; a score of -inf weighs nothing; a value that a row does not see weighs exactly nothing,
+however large.  Tolerances as in test_paged_attn_gpu.py."""
 import numpy as np
 import pytest
 
@@ -100,3 +101,15 @@ def test_scores_of_minus_infinity(cuda_device, n, kv, Hq, Hk, D):
         o, l, mag = A.attention(_np(b.q[i:i + 1]), k[see], v[see], D ** -0.5)
         assert (np.abs(out[i] - o[0]) <= (2.0 ** -7 + 1e-4) * mag[0]).all()
         assert (np.abs(lse[i] - l[0]) <= 1e-5 * (1 + np.abs(l[0]))).all()
+
+
+@pytest.mark.parametrize("n,Hq,D", [(140, 2, 128), (140, 2, 64), (60, 1, 64)])
+def test_large_values_that_a_row_does_not_see(cuda_device, n, Hq, D):
+    """Values of 1e37 that later tokens of the chunk see: a weight of 2^-125 instead of 0 on
+    one of them would be 0.24 in the rows before them."""
+    b = Batch([(n, n)], Hq, 1, D, 16, seed=n + D, poison=False)
+    at = n - 44
+    for j in range(at, at + 22):
+        b.v[_place(b, j)] *= 1e37
+    out, lse = _run(b, 0)
+    _others(b, out, lse, range(0, n, 5), range(Hq), 0)
