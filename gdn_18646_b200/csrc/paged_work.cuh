@@ -38,7 +38,7 @@ struct alignas(64) AttnMaps {
 
 // sum over i in [0, n) of floor((a i + b) / 128) for a <= 256 (the Euclid-like reduction);
 // after the first reduction every operand is small, so the divisions are 32-bit
-__device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
+__host__ __device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t a, uint32_t b) {
     uint32_t m = kTile;
     long long s = 0;
     while (n > 0) {
@@ -126,19 +126,19 @@ struct Seq {
         items = (n + tt - 1) / tt;
     }
     // positions [lo, hi) that tokens first .. last of the chunk see between them
-    __device__ __forceinline__ void range(const AttnArgs& a, int first, int last, int& lo, int& hi) const {
+    __host__ __device__ __forceinline__ void range(const AttnArgs& a, int first, int last, int& lo, int& hi) const {
         const int p = kv - n;
         hi = a.causal ? max(0, min(p + last + 1, kv)) : kv;
         lo = a.window > 0 ? max(0, p + first + 1 - a.window) : 0;
         if (hi <= lo) lo = hi = 0;
     }
-    __device__ __forceinline__ void tiles(const AttnArgs& a, int item, int tt, int& first, int& count, int& lo, int& hi) const {
+    __host__ __device__ __forceinline__ void tiles(const AttnArgs& a, int item, int tt, int& first, int& count, int& lo, int& hi) const {
         range(a, item * tt, min((item + 1) * tt, n) - 1, lo, hi);
         first = lo / kTile;
         count = hi > 0 ? (hi + kTile - 1) / kTile - first : 0;
     }
     // cost of the items before `q` of one kv head
-    __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
+    __host__ __device__ __forceinline__ long long cost(const AttnArgs& a, int q, int tt) const {
         if (q == 0) return 0;
         if (a.whole) return q;
         long long s = static_cast<long long>(q) * a.item_cost;
@@ -163,6 +163,14 @@ struct Seq {
             if (i1 < q) s -= floor_sum(q - i1, tt, w + i1 * tt);
         }
         return s;
+    }
+    // Whether unit `off` of one kv head lies in its item i, and how far into it.  A head's units pass
+    // 32 bits (a chunk of 2^21 tokens at 64 query heads a kv head has 2^32), an item's do not.
+    __host__ __device__ __forceinline__ bool holds(const AttnArgs& a, int i, int tt, long long off, int& skip) const {
+        const long long before = cost(a, i, tt);
+        if (off < before || off >= cost(a, i + 1, tt)) return false;
+        skip = static_cast<int>(off - before);
+        return true;
     }
 };
 
@@ -225,6 +233,7 @@ struct Walk {
 // Scratch of find_piece in shared memory.
 struct PieceScratch {
     Piece piece;
+    long long off;                    // where the piece starts, in units of its kv head
     long long scan[16];
 };
 
@@ -283,21 +292,21 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, PieceScratch* sh, 
             p.b = b;
             p.head = head;
             p.item = 0;
-            p.skip = static_cast<int>(off);                     // within the head, so far
+            p.skip = static_cast<int>(off);                     // of a head's only item; else found below
             p.units = to - from;
+            sh->off = off;
         }
     }
     __syncthreads();
     if (sh->piece.units == 0) return;
     s = sh->piece.s;
-    const int off = sh->piece.skip;
     if (s.items == 1) return;
-    __syncthreads();
+    const long long off = sh->off;
     for (int i = tid; i < s.items; i += nt) {
-        const long long c0 = s.cost(a, i, tt);
-        if (c0 <= off && off < s.cost(a, i + 1, tt)) {
+        int skip;
+        if (s.holds(a, i, tt, off, skip)) {
             sh->piece.item = i;
-            sh->piece.skip = off - static_cast<int>(c0);
+            sh->piece.skip = skip;
         }
     }
     __syncthreads();
