@@ -723,6 +723,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long q_ld, const gdn_paged_cach
     if (!aligned16(workspace)) return fail(GDN_ERR_ALIGN, "%s: workspace must be 16-byte aligned", name);
     if ((st = check_sm100()) != GDN_OK) return st;
     if (Ttot == 0) return GDN_OK;
+    if (max_kv > kMaxPositions) max_kv = kMaxPositions;         // a longer sequence is one outside the cache
     AttnArgs a = {};
     a.out = static_cast<uint16_t*>(out);
     a.lse = lse;

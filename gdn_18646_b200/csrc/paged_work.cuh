@@ -9,6 +9,7 @@ namespace gdn {
 
 constexpr int kTile = 128;            // positions per kv tile
 constexpr int kMaxCtas = 148;         // pieces of the work line: one CTA per SM of a B200
+constexpr int kMaxPositions = 0x7fffffff - 511;   // of a sequence: sums with a tile's and an item's size stay ints
 constexpr int kMinPiece = 4;          // shortest piece: splitting finer costs more to join
 
 struct AttnArgs {

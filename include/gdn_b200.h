@@ -529,7 +529,8 @@ int gdn_rope_append(const void* q, long q_ld, const void* k, long k_ld, const vo
  * What the cache holds at positions that no token of a sequence sees may be
  * anything, NaN included, and so may the block_table entries of pages that hold
  * only such positions.  A sequence with a longer q_len or kv_len than max_q or
- * max_kv is left out (its rows of out are not written), a page outside the cache
+ * max_kv, or with more than 2^31 - 512 positions, is left out (its rows of out, and
+ * rows past the last sequence's tokens, are not written), a page outside the cache
  * is taken as zeros; gdn_check_device_error() reports both.  D in {64, 128},
  * Hq / n_kv <= 64.
  * workspace: gdn_paged_attn_workspace_bytes(...) bytes, 16-byte aligned, required
