@@ -747,8 +747,10 @@ def _rope_spec(positions, inv_freq, sections, style, T):
     axes = len(sections)
     if not positions.is_contiguous() or positions.numel() != axes * T:
         raise RuntimeError(f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis)")
-    return _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.addressof(_int_array(sections)), axes,
-                         2 * pairs, code)
+    counts = _int_array(sections)
+    spec = _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.addressof(counts), axes, 2 * pairs, code)
+    spec.counts = counts            # the structure holds an address only
+    return spec
 
 
 def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=False, q_out=None, k_out=None):
