@@ -745,8 +745,9 @@ def _rope_spec(positions, inv_freq, sections, style, T):
     pairs = inv_freq.shape[0]
     sections = (pairs,) if sections is None else tuple(sections)
     axes = len(sections)
-    if not positions.is_contiguous() or positions.numel() != axes * T:
-        raise RuntimeError(f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis)")
+    shape = positions.shape
+    if not positions.is_contiguous() or positions.numel() != axes * T or (axes > 1 and (len(shape) < 2 or shape[0] != axes)):
+        raise RuntimeError(f"positions must be contiguous, [{axes}, tokens] ([tokens] for one axis), got {tuple(shape)}")
     counts = _int_array(sections)
     spec = _lib.RopeSpec(positions.data_ptr(), T, inv_freq.data_ptr(), ctypes.addressof(counts), axes, 2 * pairs, code)
     spec.counts = counts            # the structure holds an address only
