@@ -323,11 +323,36 @@ def prefill_backward(q, k, v, A_log, a, b_logits, dO, *, dt_bias=0.0, mask=None,
     return g
 
 
+class _FirstDerivative(torch.autograd.Function):
+    """run(), a gradient of functions of ``tensors``, as a node that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, run, *tensors):
+        return run()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this operator's gradient is computed by a kernel: it is differentiable once only")
+
+
+def _once(backward):
+    """For Function.backward: under create_graph the gradients stay tied to what they were
+    computed from, so that a second derivative is an error rather than a number without their
+    share (torch's once_differentiable ties them to nothing, and torch.autograd.grad passes
+    over its error)."""
+    @functools.wraps(backward)
+    def tied(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        return _FirstDerivative.apply(lambda: backward(ctx, *grads), *grads, *ctx.saved_tensors)
+    return tied
+
+
 class PrefillFunction(torch.autograd.Function):
     """``prefill`` as an autograd op (layout "bhtd", Hqk == Hv): forward is the
     chunked tcgen05 prefill, backward gdn_prefill_backward.  Differentiable
-    inputs: q, k, v, A_log, a, b_logits, dt_bias (tensor) and state_in;
-    outputs (o, state_out)."""
+    inputs (once): q, k, v, A_log, a, b_logits, dt_bias (tensor) and
+    state_in; outputs (o, state_out)."""
 
     @staticmethod
     def forward(ctx, q, k, v, A_log, a, b_logits, dt_bias, state_in, scale):
@@ -337,6 +362,7 @@ class PrefillFunction(torch.autograd.Function):
         return o, S
 
     @staticmethod
+    @_once
     def backward(ctx, do, dS):
         q, k, v, A_log, a, b_logits, dt_bias, state_in = ctx.saved_tensors
         if do is None:
@@ -672,7 +698,7 @@ def block_norm_backward(y, h_out, dh_out=None, dx=None, *, gamma_post=None, gate
 
 class BlockNormFunction(torch.autograd.Function):
     """``block_norm`` as an autograd op: differentiable in y, h, gamma_post, gate and
-    gamma_pre; outputs (h', x)."""
+    gamma_pre, once; outputs (h', x)."""
 
     @staticmethod
     def forward(ctx, y, h, gamma_post, gate, gamma_pre, residual_scale, eps):
@@ -683,6 +709,7 @@ class BlockNormFunction(torch.autograd.Function):
         return h_out, x
 
     @staticmethod
+    @_once
     def backward(ctx, dh, dx):
         y, h_out, gamma_post, gate, gamma_pre = ctx.saved_tensors
         if dx is None and gamma_pre is not None:
@@ -787,7 +814,7 @@ def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=Fals
 
 
 class RopeFunction(torch.autograd.Function):
-    """``rope`` as an autograd op, differentiable in q and k."""
+    """``rope`` as an autograd op, differentiable in q and k, once."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, sections, style):
@@ -796,6 +823,7 @@ class RopeFunction(torch.autograd.Function):
         return rope(q, k, positions, inv_freq, sections, style=style)
 
     @staticmethod
+    @_once
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         dq, dk = rope(dq.contiguous(), None if dk is None else dk.contiguous(), positions, inv_freq, ctx.sections,
