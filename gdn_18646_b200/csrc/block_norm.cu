@@ -513,31 +513,36 @@ struct SumJob {
     int n;
 };
 constexpr int kSumWarps = 16;
-__global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const SumJob j0, const SumJob j1, const SumJob j2, int D) {
+constexpr int kMaxGridY = 65535;        // more gate rows take turns
+__global__ void __launch_bounds__(32 * kSumWarps)
+column_sum_kernel(const SumJob j0, const SumJob j1, const SumJob j2, int groups, int D) {
     __shared__ float part[kSumWarps][32];
     pdl_wait_prior();
     // blockIdx.y 0: dgamma_post, 1: dgamma_pre, 2 + g: gate row g
     const SumJob& j = blockIdx.y == 0 ? j0 : blockIdx.y == 1 ? j1 : j2;
     if (!j.out) return;
-    const long o = blockIdx.y < 2 ? 0 : blockIdx.y - 2;
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
-    float s = 0.f;
-    if (c < D) {
-        const float* p = j.in + o * j.o_stride + c;
-        for (int n0 = k; n0 < j.n; n0 += 8 * kSumWarps) {
-            float v[8];
+    const int end = blockIdx.y < 2 ? 1 : groups, step = blockIdx.y < 2 ? 1 : gridDim.y - 2;
+    for (long o = blockIdx.y < 2 ? 0 : blockIdx.y - 2; o < end; o += step) {
+        float s = 0.f;
+        if (c < D) {
+            const float* p = j.in + o * j.o_stride + c;
+            for (int n0 = k; n0 < j.n; n0 += 8 * kSumWarps) {
+                float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = n0 + i * kSumWarps < j.n ? __ldcg(p + (n0 + i * kSumWarps) * j.n_stride) : 0.f;
+                for (int i = 0; i < 8; ++i) v[i] = n0 + i * kSumWarps < j.n ? __ldcg(p + (n0 + i * kSumWarps) * j.n_stride) : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+                for (int i = 0; i < 8; ++i) s += v[i];
+            }
         }
-    }
-    part[k][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (k == 0 && c < D) {
+        __syncthreads();                                       // `part` has been read
+        part[k][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (k == 0 && c < D) {
 #pragma unroll
-        for (int i = 1; i < kSumWarps; ++i) s += part[i][threadIdx.x & 31];
-        j.out[o * D + c] = s;
+            for (int i = 1; i < kSumWarps; ++i) s += part[i][threadIdx.x & 31];
+            j.out[o * D + c] = s;
+        }
     }
 }
 
@@ -717,7 +722,6 @@ extern "C" int gdn_block_norm_bwd(const void* y, const void* h_out, int h_dtype,
         return e == cudaSuccess ? GDN_OK : fail(GDN_ERR_CUDA, "%s: cudaMemsetAsync: %s", name, cudaGetErrorString(e));
     }
     const int sg = gate ? summed_gates(R, gate_rows) : 0, groups = sg ? sg : 1;
-    if (groups > 65533) return fail(GDN_ERR_SHAPE, "%s: at most 65533 gate rows that are shared (got %d)", name, groups);
     const BwdPlan p = bwd_plan(R, D, groups);
     BlockNormArgs a = {};
     a.y = static_cast<const uint16_t*>(y);
@@ -754,9 +758,9 @@ extern "C" int gdn_block_norm_bwd(const void* y, const void* h_out, int h_dtype,
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cfg.stream = s;
-    cfg.gridDim = dim3((D + 31) / 32, 2 + (part_gate ? groups : 0));
+    cfg.gridDim = dim3((D + 31) / 32, 2 + (part_gate ? (groups < kMaxGridY - 2 ? groups : kMaxGridY - 2) : 0));
     cfg.blockDim = dim3(32 * kSumWarps);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, column_sum_kernel, j0, j1, j2, D);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, column_sum_kernel, j0, j1, j2, groups, D);
     if (e != cudaSuccess) return fail(GDN_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
     return launch_status("gdn_block_norm_bwd (column sums)");
 }

@@ -1,0 +1,27 @@
+"""block_norm and its gradient at the ends of their ranges; tolerances and the comparison with
+the 64-bit oracle as in test_block_norm_gpu.py."""
+import pytest
+
+from tests import test_block_norm_gpu as T
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("R,D,gate", [(140000, 8, 70000), (131066, 8, 65533), (131068, 8, 65534)])
+def test_many_shared_gate_rows(cuda_device, R, D, gate):
+    """More gate rows with a summed gradient than the y extent of a grid."""
+    T.test_forward(cuda_device, R, D, gate, False, True, True)
+    T.test_backward(cuda_device, R, D, gate, False, True, True)
+
+
+def test_many_shared_gate_rows_of_wide_rows(cuda_device):
+    """The rows of a gate row are summed by themselves: halves of the batch give the same bits."""
+    import torch
+    import gdn_18646_b200 as G
+    s = T._inputs(132000, 264, 66000, False, True, True)
+    w = dict(gamma_post=s["gamma_post"], gamma_pre=s["gamma_pre"])
+    whole = G.block_norm_backward(s["y"], s["h"], s["dh"], s["dx"], gate=s["gate"], **w)
+    for a, b in ((0, 33000), (33000, 66000)):
+        r = slice(2 * a, 2 * b)
+        part = G.block_norm_backward(s["y"][r], s["h"][r], s["dh"][r], s["dx"][r], gate=s["gate"][a:b], **w)
+        assert torch.equal(part["dgate"], whole["dgate"][a:b]) and torch.equal(part["dy"], whole["dy"][r])
