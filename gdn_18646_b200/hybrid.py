@@ -71,13 +71,21 @@ class PagedKV:
         self.host_lens = [0] * B
         self.free = list(range(pages - 1, -1, -1))
 
-    def grow(self, n: int):
-        """Room for n more tokens of every sequence, counted as theirs from now on."""
+    def room(self, B: int, n: int):
+        """Pages that the sequences have, and need with n more tokens each; raises, with nothing
+        changed, where this is not the cache of B sequences or the pages do not suffice."""
+        if B != len(self.host_lens) or n < 0:
+            raise RuntimeError(f"PagedKV: {n} tokens of {B} sequences for a cache of {len(self.host_lens)} sequences")
         need = [-(-(m + n) // self.page_size) for m in self.host_lens]
         have = [-(-m // self.page_size) for m in self.host_lens]
         if sum(need) - sum(have) > len(self.free) or max(need) > self.table.shape[1]:
             raise RuntimeError(f"PagedKV: {n} more tokens need {sum(need) - sum(have)} pages, {len(self.free)} are free, "
                                f"at most {self.table.shape[1]} per sequence")
+        return have, need
+
+    def grow(self, n: int):
+        """Room for n more tokens of every sequence, counted as theirs from now on."""
+        have, need = self.room(len(self.host_lens), n)
         for b, (lo, hi) in enumerate(zip(have, need)):
             if hi > lo:
                 mine = [self.free.pop() for _ in range(hi - lo)]
@@ -101,8 +109,10 @@ class AttentionLayer:
         place in the sequence, on every axis).  Returns y [B,T,D] bf16."""
         c, w = self.cfg, self.w
         B, T, D = x.shape
+        if T < 1:
+            raise RuntimeError("x must hold at least one token of every sequence")
         start = list(kv.host_lens)
-        kv.grow(T)
+        kv.room(B, T)                                  # tokens count as the cache's only once nothing can refuse them
         if positions is None:
             positions = (torch.arange(T, device=x.device, dtype=torch.int32) +
                          torch.tensor(start, dtype=torch.int32, device=x.device)[:, None]).reshape(1, -1) \
@@ -113,6 +123,8 @@ class AttentionLayer:
             q, k, v = ops.decode_proj(x.reshape(B, D), seg)
         else:
             q, k, v = ops.proj_multi(x.reshape(1, B * T, D), seg)
+        ops._rope_spec(positions, self.inv_freq, c.sections, c.style, B * T)
+        kv.grow(T)
         q = ops.rope_append(q.view(B * T, c.n_q, c.head_dim), k.view(B * T, c.n_kv, c.head_dim),
                             v.view(B * T, c.n_kv, c.head_dim), positions, self.inv_freq, c.sections, kv.k, kv.v, kv.table, cu,
                             kv.lens, style=c.style)
@@ -141,8 +153,12 @@ class HybridStack:
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, states: list):
-        """x [B,T,D] bf16, the next T tokens' embeddings; ``states`` is updated.  Returns the
-        normed residual stream [B,T,D] bf16 after the last layer."""
+        """x [B,T,D] bf16, the next T tokens' embeddings; ``states`` is updated (not if a cache
+        has no room for them).  Returns the normed residual stream [B,T,D] bf16 after the last
+        layer."""
+        for s in states:
+            if isinstance(s, PagedKV):
+                s.room(x.shape[0], x.shape[1])
         h = x.float()
         xn = ops.rmsnorm(x, self.norms[0]["gamma_pre"], self.eps)
         for i, m in enumerate(self.layers):
