@@ -593,7 +593,7 @@ int launch_fwd(const BlockNormArgs& a, cudaStream_t st) {
     cfg.blockDim = dim3(nt);
     const int rows = a.D <= kNarrow ? kNarrowRows : 1;
     // as many CTAs as are resident at once (48 registers a thread), each for several rows
-    const int most = 148 * (1024 / nt > 0 ? 1024 / nt : 1), need = (a.R + rows - 1) / rows;
+    const int most = 148 * (1024 / nt > 0 ? 1024 / nt : 1), need = a.R / rows + (a.R % rows != 0);
     cfg.gridDim = dim3(need < most ? need : most);
     cudaError_t e;
     if (a.D <= kNarrow)

@@ -589,6 +589,14 @@ def decode_proj(x, segments, *, norm_gamma=None, eps=1e-6):
 # ---------------------------------------------------------------------------
 
 
+_INT_MAX = 0x7FFFFFFF
+
+
+def _int(n):
+    """n as a C int that compares with every size as n does (ctypes would take its low 32 bits)."""
+    return max(-1, min(n, _INT_MAX))
+
+
 def _dense(t, name, dtype):
     """A contiguous CUDA tensor of that type (one test on the way that is right)."""
     if not (t.dtype is dtype and t.is_cuda and t.is_contiguous()):
@@ -616,6 +624,8 @@ def _norm_args(y, h, hname, gamma_post, gate, gamma_pre):
     _dense(h, hname, h.dtype)
     D = y.shape[-1]
     R = y.numel() // D
+    if R > _INT_MAX:
+        raise RuntimeError(f"at most {_INT_MAX} rows, got {R}")
     for name, w in (("gamma_post", gamma_post), ("gamma_pre", gamma_pre)):
         if w is not None:
             _dense(w, name, torch.bfloat16)
@@ -928,7 +938,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0:
         return (out, lse) if return_lse else out
-    window = min(window, 0x7FFFFFFF)
+    max_q, max_kv, window = _int(max_q), _int(max_kv), _int(window)
     ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
     if workspace is None:
         workspace = q.new_empty(ws_bytes // 2)
@@ -942,7 +952,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
 
 def paged_attention_workspace(B, T, Hq, n_kv, head_dim, max_q, max_kv, window=0):
     """Bytes of workspace ``paged_attention`` needs for calls up to these sizes."""
-    return int(_lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, n_kv, head_dim, max_q, max_kv, window))
+    return int(_lib.lib().gdn_paged_attn_workspace_bytes(_int(B), _int(T), _int(Hq), _int(n_kv), _int(head_dim), _int(max_q),
+                                                         _int(max_kv), _int(window)))
 
 
 # ---------------------------------------------------------------------------
