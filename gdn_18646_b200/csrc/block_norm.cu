@@ -276,11 +276,12 @@ __device__ __forceinline__ void weight_pairs(const uint16_t* p, long at, bool on
 //   sum y^2, sum h'^2, A = sum g2 h', B = sum w y dh', C = sum w y g2, E = sum w y h'
 //   mean(g2 n2) = r2 A / D,  sum g1 n1 = r1 (B + r2 C - r2^3 (A / D) E)
 // Where the rows of an item share their gate row, dgate and dgamma_post both follow from
-// q = sum dt n1, so one sum serves both.
+// q = sum dt n1, so one sum serves both.  Without a norm its input is not looked at (h' is 0
+// then, y in dgate only): an infinity there would reach the result as 0 times infinity.
 template <bool F32, bool WARP>
 struct BwdRow {
     uint64_t gq[4], w[4], q[4], sum_pre[4];    // gamma_pre; gate gamma_post; column sums
-    // y, h, dx, dt (dh'): the row's values; gate, sum_post: of a row with a gate row of its own
+    // y, h, dx (both 0 without gamma_pre), dt (dh'): the row's values; gate, sum_post: of a row with a gate row of its own
     template <class AfterSums>
     __device__ __forceinline__ void run(const BlockNormArgs& a, uint64_t (&y)[4], uint64_t (&h)[4], uint64_t (&dx)[4],
                                         uint64_t (&dt)[4], const uint64_t* gate, const uint64_t* gp, uint64_t* sum_post,
@@ -327,7 +328,8 @@ struct BwdRow {
             } else {
                 q[i] = fma2(dt[i], n1, q[i]);
             }
-            y[i] = mul2(r1_2, fma2(n1, m_2, mul2(dt[i], w[i])));                    // dy
+            const uint64_t g1 = mul2(dt[i], w[i]);
+            y[i] = mul2(r1_2, a.gamma_post ? fma2(n1, m_2, g1) : g1);               // dy
         }
         if (!on) return;
         write_pairs<F32>(a.h_out, at, out);
@@ -398,8 +400,10 @@ block_norm_bwd_narrow_kernel(const BlockNormArgs a, const BwdPlan plan, void* dg
             uint64_t y[4] = {}, h[4] = {}, dx[4] = {}, dt[4] = {}, gt[4] = {};
             if (on) {
                 read_pairs<false>(a.y + at, y);
-                read_pairs<F32>(static_cast<const uint8_t*>(a.h) + at * (F32 ? 4 : 2), h);
-                if (a.gamma_pre) read_pairs<false>(a.dx + at, dx);
+                if (a.gamma_pre) {
+                    read_pairs<F32>(static_cast<const uint8_t*>(a.h) + at * (F32 ? 4 : 2), h);
+                    read_pairs<false>(a.dx + at, dx);
+                }
                 if (a.dh_out) read_pairs<F32>(static_cast<const uint8_t*>(a.dh_out) + at * (F32 ? 4 : 2), dt);
                 if (row_gate) {
                     read_pairs<false>(a.gate + at, gt);
@@ -460,10 +464,12 @@ block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, const BwdRing r
         uint64_t* bar = &full[n % ring.stages];
         const uint32_t e = a.D;
         const long at = r * a.D;
-        mbar_arrive_expect_tx(bar, e * (2 + HB) + (a.gamma_pre ? e * 2 : 0) + (a.dh_out ? e * HB : 0) + (row_gate ? e * 2 : 0));
+        mbar_arrive_expect_tx(bar, e * 2 + (a.gamma_pre ? e * (2 + HB) : 0) + (a.dh_out ? e * HB : 0) + (row_gate ? e * 2 : 0));
         bulk_load(s, a.y + at, e * 2, bar);
-        bulk_load(s + ring.off_h, static_cast<const uint8_t*>(a.h) + at * HB, e * HB, bar);
-        if (a.gamma_pre) bulk_load(s + ring.off_dx, a.dx + at, e * 2, bar);
+        if (a.gamma_pre) {
+            bulk_load(s + ring.off_h, static_cast<const uint8_t*>(a.h) + at * HB, e * HB, bar);
+            bulk_load(s + ring.off_dx, a.dx + at, e * 2, bar);
+        }
         if (a.dh_out) bulk_load(s + ring.off_dh, static_cast<const uint8_t*>(a.dh_out) + at * HB, e * HB, bar);
         if (row_gate) bulk_load(s + ring.off_gate, a.gate + at, e * 2, bar);
     };
@@ -480,8 +486,10 @@ block_norm_bwd_kernel(const BlockNormArgs a, const BwdPlan plan, const BwdRing r
             uint64_t y[4] = {}, h[4] = {}, dx[4] = {}, dt[4] = {}, gt[4] = {};
             if (on) {
                 read_pairs<false>(s + col * 2, y);
-                read_pairs<F32>(s + ring.off_h + col * HB, h);
-                if (a.gamma_pre) read_pairs<false>(s + ring.off_dx + col * 2, dx);
+                if (a.gamma_pre) {
+                    read_pairs<F32>(s + ring.off_h + col * HB, h);
+                    read_pairs<false>(s + ring.off_dx + col * 2, dx);
+                }
                 if (a.dh_out) read_pairs<F32>(s + ring.off_dh + col * HB, dt);
                 if (row_gate) {
                     read_pairs<false>(s + ring.off_gate + col * 2, gt);
@@ -612,7 +620,7 @@ BwdRing bwd_ring(const BlockNormArgs& a, bool f32, bool row_gate) {
     const int row = a.D * 2, hrow = a.D * (f32 ? 4 : 2);
     r.off_dx = row;
     r.off_h = r.off_dx + (a.gamma_pre ? row : 0);
-    r.off_dh = r.off_h + hrow;
+    r.off_dh = r.off_h + (a.gamma_pre ? hrow : 0);
     r.off_gate = r.off_dh + (a.dh_out ? hrow : 0);
     r.bytes = r.off_gate + (row_gate ? row : 0);
     const int room = (220 * 1024) / bwd_resident(a.D) - (bwd_resident(a.D) > 1 ? 4096 : 0);

@@ -425,7 +425,8 @@ int gdn_block_norm_fwd(const void* y, const void* h, int h_dtype, const void* ga
                        int R, int D, float eps, void* stream);
 
 /*
- * Gradients of gdn_block_norm_fwd, from y and the stored h_out:
+ * Gradients of gdn_block_norm_fwd, from y and the stored h_out (not read without
+ * gamma_pre, when no gradient depends on it):
  *   dh_out      [R, D] in h_dtype or NULL (0), dx bf16 [R, D] (NULL without gamma_pre)
  *   dy          bf16 [R, D]; dh [R, D] in h_dtype (may be dh_out's buffer)
  *   dgate       [gate_rows, D] in dgate_dtype: f32, or bf16 when every row has its

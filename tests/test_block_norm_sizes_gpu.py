@@ -25,3 +25,27 @@ def test_many_shared_gate_rows_of_wide_rows(cuda_device):
         r = slice(2 * a, 2 * b)
         part = G.block_norm_backward(s["y"][r], s["h"][r], s["dh"][r], s["dx"][r], gate=s["gate"][a:b], **w)
         assert torch.equal(part["dgate"], whole["dgate"][a:b]) and torch.equal(part["dy"], whole["dy"][r])
+
+
+@pytest.mark.parametrize("D", [64, 512, 4096, 4104])
+@pytest.mark.parametrize("gate", [1, "row"])
+@pytest.mark.parametrize("f32", [False, True])
+def test_infinities_where_no_norm_looks(cuda_device, D, gate, f32):
+    """Without gamma_pre no gradient depends on h', without gamma_post dy does not depend on y:
+    infinities and NaN there leave them as they are."""
+    import torch
+    import gdn_18646_b200 as G
+    s = T._inputs(7, D, gate, f32, False, False)
+    clean = G.block_norm_backward(s["y"], s["h"], s["dh"], gate=s["gate"])
+    bad_h = s["h"].clone()
+    bad_h[2, 5], bad_h[3, 0], bad_h[6] = float("inf"), float("nan"), float("-inf")
+    got = G.block_norm_backward(s["y"], bad_h, s["dh"], gate=s["gate"])
+    assert all(clean[k] is None or torch.equal(got[k], clean[k]) for k in clean)
+    bad_y = s["y"].clone()
+    bad_y[1, 3], bad_y[4, 7] = float("inf"), float("nan")
+    got = G.block_norm_backward(bad_y, bad_h, s["dh"], gate=s["gate"])
+    assert torch.equal(got["dy"], clean["dy"]) and torch.equal(got["dh"], clean["dh"])
+    s = T._inputs(7, D, gate, f32, True, False)
+    clean = G.block_norm_backward(s["y"], s["h"], s["dh"], gate=s["gate"], gamma_post=s["gamma_post"])
+    got = G.block_norm_backward(s["y"], bad_h, s["dh"], gate=s["gate"], gamma_post=s["gamma_post"])
+    assert all(clean[k] is None or torch.equal(got[k], clean[k]) for k in clean)
