@@ -49,3 +49,17 @@ def test_infinities_where_no_norm_looks(cuda_device, D, gate, f32):
     clean = G.block_norm_backward(s["y"], s["h"], s["dh"], gate=s["gate"], gamma_post=s["gamma_post"])
     got = G.block_norm_backward(s["y"], bad_h, s["dh"], gate=s["gate"], gamma_post=s["gamma_post"])
     assert all(clean[k] is None or torch.equal(got[k], clean[k]) for k in clean)
+
+
+@pytest.mark.parametrize("R,D,gate,f32", [
+    (200, 8192, "row", True),          # a ring of one stage, several rows a CTA
+    (200, 8192, "row", False),
+    (301, 8192, 1, True),
+    (333, 5120, 3, True),
+    (320, 7168, 4, False),
+    (150, 4104, "row", True),
+])
+def test_wide_rows(cuda_device, R, D, gate, f32):
+    """Rows above 4096 columns, more of them than CTAs."""
+    T.test_forward(cuda_device, R, D, gate, f32, True, True)
+    T.test_backward(cuda_device, R, D, gate, f32, True, True)
