@@ -14,8 +14,11 @@
 // written once; a row stays in registers between its two reductions.  A thread owns
 // 8 consecutive columns (one 16-byte piece of a bf16 row).  Rows of at most 256 columns
 // belong to one warp (shuffles only), wider ones to a CTA.  16384 rows of 2048: forward with
-// a bf16 stream 46.3 us (268 MB, 5.8 TB/s), backward with an fp32 stream 118.4 us (604 MB,
-// 5.1 TB/s; 7 us of it the column sums); 8 rows of 2048 forward 2.4 us.
+// a bf16 stream 46.1 us (268 MB, 5.8 TB/s), backward with an fp32 stream 117 us (604 MB,
+// 5.2 TB/s; 7 us of it the column sums); 8 rows of 2048 forward 2.4 us.  Above 4096 columns the
+// backward's 1024 threads have 64 registers each, the whole register file, for values that take
+// 125: they spill, and 8192 columns run at 2.3 TB/s with an fp32 stream (1.7 with bf16, where the
+// spills weigh more), against 5.3 at 4096.
 #include "common.cuh"
 
 namespace gdn {

@@ -29,11 +29,12 @@
 // at most 64 rows (a decode step) go to paged_attn_rows.cu.
 //
 // What bounds it.  A kv tile of both row tiles is 32 MMAs of about 61 cycles and 128 x 256
-// exponentials, 2048 cycles either; three pairs of eight take a polynomial on the FMA pipe
-// (2048 new tokens over 32768, 16 heads on 2, head dim 128: 486 us; 495 with a quarter or two
-// fifths; before the last steps 496 us with three of eight, 572 without, 555 with a half).  Both take 3400 cycles of the softmax warps, two to a
-// scheduler, 600 to 900 of which wait for the MMAs.  In sustained passes the power cap sets the
-// clock: 486 us (1.10 PFLOP/s) at 1.64 GHz, 430 (1.24) in the first passes at 1.97 GHz.
+// exponentials, 2048 cycles either if nothing else ran.  The softmax takes 3400 cycles of its
+// warps, two to a scheduler: loads of S, maxima, exponentials, conversions and stores of P one
+// after the other, 128 scores of a row in 168 registers (264 bytes a thread spilled), and 600 to
+// 900 cycles of waiting for the MMAs.  2048 new tokens over 32768, 16 heads on 2, head dim 128:
+// 430 us (1.24 PFLOP/s) at 1.97 GHz, 487 (1.09) in sustained passes, where the power cap lowers
+// the clock to 1.64 GHz.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -52,7 +53,9 @@ constexpr int kItemCost = 2;
 constexpr int kJoinThreads = 256, kJoinBlocks = 2;  // of the join kernel, per SM
 constexpr int kWholeTiles = 8;        // items of so many kv tiles are not cut when there are few
 constexpr int kEarly = 3;             // quarters of a tile's P after which P V starts
-constexpr int kPolyPairs = 3, kPolyOf = 8;   // pairs of weights in every so many that take the polynomial
+// pairs of weights in every so many that take the polynomial on the FMA pipe, the others the MUFU
+// (2048 tokens over 32768: 486 us with three of eight, 495 with a quarter or two fifths)
+constexpr int kPolyPairs = 3, kPolyOf = 8;
 
 // umma_commit to a barrier given by its shared-memory address
 __device__ __forceinline__ void commit_to(uint32_t bar) {

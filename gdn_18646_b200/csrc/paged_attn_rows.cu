@@ -25,8 +25,8 @@ namespace {
 
 // A warp issues a copy in about 60 cycles, and a tile is 2 x 128 / page size x D / 64 of them, so
 // with small pages the issue sets the pace of one warp while the ring fills.  With 1 / 2 / 4 warps,
-// us: 1 token over 1000 positions in pages of 16, head dim 128, 16.3 / 12.6 / 12.0; 256 sequences of
-// up to 8192 161 / 162 / 162; 2 of up to 131072 in pages of 64 72.5 / 72.8 / 73.2.
+// us: 1 token over 1000 positions in pages of 16, head dim 128, 16.5 / 13.0 / 12.3; 256 sequences of
+// up to 8192 159.8 / 162.5 / 164.3; 2 of up to 131072 in pages of 64 72.2 / 72.7 / 73.0.
 constexpr int kLoadWarps = 2;
 constexpr int kRowsThreads = 288 + 32 * kLoadWarps;      // 2 x 4 softmax warps, MMA, load
 
