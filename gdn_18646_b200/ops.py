@@ -797,7 +797,7 @@ def rope(q, k, positions, inv_freq, sections=None, *, style="half", inverse=Fals
     where ``sections`` counts the pairs of each axis in turn (None: one axis).
 
     q [..., Hq, D], k [..., Hk, D] bf16 or None (tokens may be strided rows); positions
-    int32 [axes, tokens]; inv_freq f32 [rot / 2]; style "half" pairs values (i, i + rot/2),
+    int32 [axes, tokens] ([tokens] for one axis); inv_freq f32 [rot / 2]; style "half" pairs values (i, i + rot/2),
     "interleaved" (2i, 2i + 1).  ``inverse`` turns back, which is the gradient.
     Returns (q_out, k_out), contiguous; ``q_out=q`` works in place."""
     T, Hq, D, q_ld = _token_rows(q, "q")
@@ -921,7 +921,9 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
     ``workspace``: uint8 CUDA tensor of at least paged_attention_workspace(...) bytes
     (allocated per call if None).  Returns out [T, Hq, D] bf16, with ``return_lse`` also
     the log of the softmax's sum, f32 [T, Hq].  A token that sees nothing gets zeros
-    and -inf."""
+    and -inf, one that sees a score of NaN or +inf gets NaN in both; rows of q past
+    cu_seqlens[B] are not written.  The softmax's weights are rounded to bf16 before
+    they meet the values (fp32 sums)."""
     T, Hq, D, q_ld = _token_rows(q, "q")
     cache = _paged_cache(k_cache, v_cache, block_table, layout)
     B = _sequences(cu_seqlens, kv_lens, block_table)
@@ -938,7 +940,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, *, ma
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0:
         return (out, lse) if return_lse else out
-    max_q, max_kv, window = _int(max_q), _int(max_kv), _int(window)
+    if not (0 <= max_q <= _INT_MAX and 0 <= max_kv <= _INT_MAX and 0 <= window <= _INT_MAX):
+        max_q, max_kv, window = _int(max_q), _int(max_kv), _int(window)
     ws_bytes = _lib.lib().gdn_paged_attn_workspace_bytes(B, T, Hq, cache.n_kv, D, max_q, max_kv, window)
     if workspace is None:
         workspace = q.new_empty(ws_bytes // 2)
