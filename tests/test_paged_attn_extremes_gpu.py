@@ -113,3 +113,24 @@ def test_large_values_that_a_row_does_not_see(cuda_device, n, Hq, D):
         b.v[_place(b, j)] *= 1e37
     out, lse = _run(b, 0)
     _others(b, out, lse, range(0, n, 5), range(Hq), 0)
+
+
+@pytest.mark.parametrize("what", ["nan", "inf"])
+@pytest.mark.parametrize("n,kv,Hq,Hk,D", [(3, 30000, 8, 2, 128), (20, 9000, 4, 2, 64), (140, 12000, 4, 2, 128), (300, 9000, 2, 2, 64)])
+def test_a_score_that_is_no_number_in_one_part_of_many(cuda_device, n, kv, Hq, Hk, D, what):
+    """Items cut into parts that are joined: one part of the rows is NaN."""
+    b = Batch([(n, kv)], Hq, Hk, D, 16, seed=n, poison=False)
+    group = Hq // Hk
+    b.q.copy_((b.q.abs() + 0.1) if what == "inf" else b.q)
+    for j in (0, 700, kv // 2, kv - n - 200, kv - n // 2 - 1, kv - 1):
+        at = _place(b, j)
+        kept = b.k[at][0].clone()
+        b.k[at][0] = float(what)
+        out, lse = _run(b, 0)
+        b.k[at][0] = kept
+        hit = _sees(n, kv, 0, j)
+        assert np.isnan(out[hit][:, :group]).all() and np.isnan(lse[hit][:, :group]).all(), j
+        assert np.isfinite(out[~hit]).all() and np.isfinite(lse[~hit]).all(), j
+        assert np.isfinite(out[:, group:]).all() and np.isfinite(lse[:, group:]).all(), j
+    out, lse = _run(b, 0)
+    _others(b, out, lse, (0, n - 1), range(Hq), 0)
